@@ -1,0 +1,83 @@
+// The 4-bit KV cache format, shared by its writer, its reader and the attention kernels.
+//
+// A cache row holds the D values of one (token, K or V, kv head). They are cut into groups of 32 channels; a
+// group keeps its minimum lo and a step s = T((max - lo) / 15), both in the type T of the rows (fp16 / bf16), and
+// a 4-bit code c = clamp(rint((x - lo) / s), 0, 15) per value. The group stands for lo + s * c.
+//
+//   row bytes:  D / 2 code bytes | D / 32 x (lo, s)          (80 bytes for D = 128, against 256 in 16 bits)
+//   code word:  8 channels in 32 bits; nibble i of the low half is channel 2 i, of the high half channel 2 i + 1
+//
+// The nibble order is the one the tensor-core kernels want: (w >> 4 i) & 0x000f000f is a pair of adjacent
+// channels, and the same mask on two tokens' interleaved halves is a pair of adjacent tokens. Pages are
+// [2, kv heads, page, row] like the 16-bit cache's, so the 16 rows of a head are one contiguous run.
+#pragma once
+#include "common.cuh"
+
+namespace mlcb {
+
+constexpr int KV4_GROUP = 32;
+__host__ __device__ constexpr int kv4_row_bytes(int d) { return d / 2 + d / KV4_GROUP * 4; }
+
+// Values are clamped to this bound before quantisation (NaN becomes 0), so that lo + 15 s stays finite in T
+// however s was rounded: fp16 65440 (max + 131008 / 2048 < 65520), bf16 2^126.
+template <typename T>
+struct Kv4Type;
+template <>
+struct Kv4Type<__half> {
+  using Pair = __half2;
+  static constexpr float BOUND = 65440.f;
+  // out[i] = pair of s * c_i + lo for the nibbles at bits 4 i of both halves. A nibble under the exponent of
+  // 1024 (bits 0-3) or of 64 (bits 4-7) is the exact number 1024 + c or 64 + c: no int-to-float conversion, one
+  // shift per word, and one rounding in the final fma.
+  static __device__ __forceinline__ void expand4(uint32_t w, uint32_t s2, uint32_t lo2, uint32_t (&out)[4]) {
+    const uint32_t w8 = w >> 8;
+    const uint32_t x[4] = {(w & 0x000f000fu) | 0x64006400u, (w & 0x00f000f0u) | 0x54005400u,
+                           (w8 & 0x000f000fu) | 0x64006400u, (w8 & 0x00f000f0u) | 0x54005400u};
+    const uint32_t bias[2] = {0x64006400u, 0x54005400u};
+    const __half2 s = *reinterpret_cast<const __half2*>(&s2), lo = *reinterpret_cast<const __half2*>(&lo2);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const __half2 c = __hsub2(*reinterpret_cast<const __half2*>(&x[i]), *reinterpret_cast<const __half2*>(&bias[i & 1]));
+      const __half2 v = __hfma2(c, s, lo);
+      out[i] = *reinterpret_cast<const uint32_t*>(&v);
+    }
+  }
+  static __device__ __forceinline__ uint32_t pack(float a, float b) {
+    const __half2 v = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
+};
+template <>
+struct Kv4Type<__nv_bfloat16> {
+  using Pair = __nv_bfloat162;
+  static constexpr float BOUND = 8.507059173023461586e37f;  // 2^126
+  // as above; bf16 has 7 mantissa bits, so only the nibble at bits 0-3 fits (under the exponent of 128)
+  static __device__ __forceinline__ void expand4(uint32_t w, uint32_t s2, uint32_t lo2, uint32_t (&out)[4]) {
+    const uint32_t bias = 0x43004300u;
+    const __nv_bfloat162 s = *reinterpret_cast<const __nv_bfloat162*>(&s2);
+    const __nv_bfloat162 lo = *reinterpret_cast<const __nv_bfloat162*>(&lo2);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t x = ((w >> (4 * i)) & 0x000f000fu) | 0x43004300u;
+      const __nv_bfloat162 c =
+          __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&x), *reinterpret_cast<const __nv_bfloat162*>(&bias));
+      const __nv_bfloat162 v = __hfma2(c, s, lo);
+      out[i] = *reinterpret_cast<const uint32_t*>(&v);
+    }
+  }
+  static __device__ __forceinline__ uint32_t pack(float a, float b) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
+};
+
+// Code of channel `ch` (0..7) of a word.
+__device__ __forceinline__ int kv4_code(uint32_t w, int ch) { return (w >> ((ch & 1) * 16 + (ch >> 1) * 4)) & 15; }
+
+// cap * tanh(x / cap) through exp2: tanh(y) = 1 - 2 / (1 + e^2y), off by about 1e-7 * cap, where the hardware's
+// tanh approximation is off by 5e-4 of the value. `k` = 2 log2(e) * scale / cap. (e^2y = inf gives cap; NaN stays.)
+__device__ __forceinline__ float kv4_softcap(float raw, float k, float cap) {
+  return cap - __fdividef(2.f * cap, 1.f + exp2f(raw * k));
+}
+
+}  // namespace mlcb

@@ -15,7 +15,9 @@ import torch
 
 from .. import quantization as Q
 from . import reference as ref
+from . import kv4
 from ._lib import DTYPE_CODE, KernelError, check, check_status, lib, ptr, status_word, stream_ptr
+from .kv4 import is_kv4, kv4_cache, kv4_plan, kv4_read, kv4_row
 
 c_int = ctypes.c_int
 c_float = ctypes.c_float
@@ -360,6 +362,11 @@ def embed(ids: torch.Tensor, table, hidden: int, dtype: torch.dtype, scale: floa
 def rope_append(qkv: torch.Tensor, kv_pages: torch.Tensor, pos: torch.Tensor, slot: torch.Tensor,
                 inv_freq: Optional[torch.Tensor], hq: int, hkv: int, d: int, rot_dim: int, page: int,
                 attn_factor: float = 1.0) -> None:
+    """Rotate the q and k heads of ``qkv [T, (hq + 2 hkv) d]`` in place and write k and v to their slots of one layer's
+    cache (negative slot: rotate only). A packed cache (``ops.kv4_cache``) is written in 4 bits."""
+    if is_kv4(kv_pages, d):
+        kv4.append(qkv, kv_pages, pos, slot, inv_freq, hq, hkv, d, rot_dim, page, attn_factor)
+        return
     if not qkv.is_cuda:
         ref.rope_append(qkv, kv_pages, pos, slot, inv_freq, hq, hkv, d, rot_dim, page, attn_factor)
         return
@@ -383,7 +390,11 @@ def paged_attention(q: torch.Tensor, kv_pages: torch.Tensor, q_seq: torch.Tensor
                     q_kvstart: Optional[torch.Tensor] = None, sink: int = 0,
                     tree_mask: Optional[torch.Tensor] = None, softcap: float = 0.0,
                     return_lse: bool = False, plan=None):
-    """``q``: ``[T, hq*d]`` view (row stride may exceed ``hq*d``). Returns ``[T, hq*d]``."""
+    """``q``: ``[T, hq*d]`` view (row stride may exceed ``hq*d``). Returns ``[T, hq*d]``. ``kv_pages`` may be a packed
+    4-bit cache (``ops.kv4_cache``), with a plan from ``ops.kv4_plan`` or none."""
+    if is_kv4(kv_pages, d):
+        return kv4.attend(q, kv_pages, q_seq, q_kvlen, page_indptr, page_indices, hq, hkv, d, page, sm_scale, q_kvstart,
+                          sink, tree_mask, softcap, return_lse, plan)
     t = q.shape[0]
     if not q.is_cuda:
         res = ref.paged_attention(q.reshape(t, hq, d), kv_pages, q_seq, q_kvlen, page_indptr,

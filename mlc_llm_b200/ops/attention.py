@@ -60,6 +60,7 @@ class AttentionPlan:
     num_dec: int = 0
     dec_splits: int = 1
     max_pages: int = 0
+    dec_rows: int = 16  # most query rows (tokens x heads of a group) of any decode item
 
 
 def attention_tcgen05(q: torch.Tensor, kv_pages: torch.Tensor, out: torch.Tensor,
@@ -81,13 +82,17 @@ def attention_tcgen05(q: torch.Tensor, kv_pages: torch.Tensor, out: torch.Tensor
 _SM_COUNT = {}
 
 
-def choose_splits(num_items: int, hkv: int, max_pages: int, device: torch.device) -> int:
-    """Split the KV range when (items x kv heads) alone cannot fill the GPU (few long sequences)."""
+def sm_count(device: torch.device) -> int:
     key = device.index or 0
     if key not in _SM_COUNT:
         _SM_COUNT[key] = torch.cuda.get_device_properties(device).multi_processor_count
+    return _SM_COUNT[key]
+
+
+def choose_splits(num_items: int, hkv: int, max_pages: int, device: torch.device) -> int:
+    """Split the KV range when (items x kv heads) alone cannot fill the GPU (few long sequences)."""
     ctas = num_items * hkv
-    target = 2 * _SM_COUNT[key]  # the decode kernel keeps two persistent CTAs per SM
+    target = 2 * sm_count(device)  # the decode kernel keeps two persistent CTAs per SM
     if ctas >= target or max_pages < 16:
         return 1
     return int(max(1, min(32, target // max(1, ctas), max_pages // 8)))

@@ -140,6 +140,61 @@ def rope_attention_factor(scaling: Optional[dict]) -> float:
     return 1.0
 
 
+# --------------------------------------------------------------------------- 4-bit KV cache rows
+KV4_GROUP = 32
+KV4_BOUND = {torch.float16: 65440.0, torch.bfloat16: 2.0 ** 126, torch.float32: 2.0 ** 126}
+
+
+def kv4_row(d: int, dtype: torch.dtype) -> int:
+    """Elements of a packed row of ``d`` values (format: ``ops.kv4``)."""
+    if d <= 0 or d % KV4_GROUP or dtype not in KV4_BOUND:
+        raise ValueError(f"a 4-bit cache row needs a multiple of {KV4_GROUP} channels in fp16, bf16 or fp32, got {d} "
+                         f"in {dtype}")
+    return d // 2 // dtype.itemsize + 2 * (d // KV4_GROUP)
+
+
+def is_kv4(kv_pages: torch.Tensor, d: int) -> bool:
+    """Whether a cache for heads of ``d`` holds packed rows (a packed row is shorter than ``d`` elements)."""
+    return kv_pages.dtype in KV4_BOUND and d > 0 and d % KV4_GROUP == 0 and kv_pages.shape[-1] == kv4_row(d, kv_pages.dtype)
+
+
+def kv4_pack(x: torch.Tensor) -> torch.Tensor:
+    """Rows ``[..., d]`` -> packed rows ``[..., kv4_row(d)]`` of the same type."""
+    bound, d = KV4_BOUND[x.dtype], x.shape[-1]
+    g = torch.nan_to_num(x.float(), nan=0.0, posinf=bound, neginf=-bound).clamp(-bound, bound)
+    g = g.reshape(*x.shape[:-1], d // KV4_GROUP, KV4_GROUP)
+    lo, hi = g.amin(-1, keepdim=True), g.amax(-1, keepdim=True)
+    s = ((hi - lo) / 15.0).to(x.dtype).float()
+    c = torch.where(s > 0, torch.round((g - lo) / torch.where(s > 0, s, torch.ones_like(s))), torch.zeros_like(g))
+    c = c.clamp(0, 15).to(torch.uint8).reshape(*x.shape[:-1], d // 8, 8)
+    # nibble i of a word's low half is channel 2 i, of its high half channel 2 i + 1
+    byte = [c[..., 0] | (c[..., 2] << 4), c[..., 4] | (c[..., 6] << 4),
+            c[..., 1] | (c[..., 3] << 4), c[..., 5] | (c[..., 7] << 4)]
+    codes = torch.stack(byte, dim=-1).reshape(*x.shape[:-1], d // 2).contiguous().view(x.dtype)
+    meta = torch.cat([lo, s], dim=-1).to(x.dtype).reshape(*x.shape[:-1], 2 * (d // KV4_GROUP))
+    return torch.cat([codes, meta], dim=-1)
+
+
+def kv4_unpack(rows: torch.Tensor, d: int) -> torch.Tensor:
+    """Packed rows ``[..., kv4_row(d)]`` -> the values they stand for, fp32 ``[..., d]``."""
+    n = d // 2 // rows.element_size()
+    byte = rows[..., :n].contiguous().view(torch.uint8).reshape(*rows.shape[:-1], d // 8, 4)
+    b0, b1, b2, b3 = byte.unbind(-1)
+    c = torch.stack([b0 & 15, b2 & 15, b0 >> 4, b2 >> 4, b1 & 15, b3 & 15, b1 >> 4, b3 >> 4], dim=-1)
+    meta = rows[..., n:].float().reshape(*rows.shape[:-1], d // KV4_GROUP, 2)
+    c = c.reshape(*rows.shape[:-1], d // KV4_GROUP, KV4_GROUP).float()
+    return (meta[..., :1] + meta[..., 1:] * c).reshape(*rows.shape[:-1], d)
+
+
+def kv4_read(kv_pages: torch.Tensor, slot: torch.Tensor, d: int):
+    """Values of the rows at ``slot`` of one layer's packed cache: ``k, v [T, hkv, d]``; negative slots read as 0."""
+    page = kv_pages.shape[3]
+    sl = slot.long().clamp(min=0)
+    rows = kv4_unpack(kv_pages[sl // page, :, :, sl % page, :], d).to(kv_pages.dtype)  # [T, 2, hkv, d]
+    rows = rows * (slot >= 0).view(-1, 1, 1, 1)
+    return rows[:, 0].contiguous(), rows[:, 1].contiguous()
+
+
 def rope_append(qkv: torch.Tensor, kv_pages: torch.Tensor, pos: torch.Tensor, slot: torch.Tensor,
                 inv_freq: Optional[torch.Tensor], hq: int, hkv: int, d: int, rot_dim: int, page: int,
                 attn_factor: float = 1.0) -> None:
@@ -148,7 +203,18 @@ def rope_append(qkv: torch.Tensor, kv_pages: torch.Tensor, pos: torch.Tensor, sl
     if t == 0:
         return
     heads = qkv.view(t, hq + 2 * hkv, d)
-    if inv_freq is not None and rot_dim > 0:
+    packed = is_kv4(kv_pages, d)
+    if packed and inv_freq is not None and rot_dim > 0:
+        # a key on the wrong side of a rounding border becomes another code: rotate in 64 bits
+        ang = pos.to(torch.float64).unsqueeze(-1) * inv_freq[: rot_dim // 2].to(qkv.device).double().unsqueeze(0)
+        cos = (torch.cos(ang) * attn_factor).unsqueeze(1)
+        sin = (torch.sin(ang) * attn_factor).unsqueeze(1)
+        half = rot_dim // 2
+        qk = heads[:, : hq + hkv, :rot_dim].double()
+        a, b = qk[..., :half], qk[..., half:]
+        heads[:, : hq + hkv, :half] = (a * cos - b * sin).float().to(qkv.dtype)
+        heads[:, : hq + hkv, half:rot_dim] = (b * cos + a * sin).float().to(qkv.dtype)
+    elif inv_freq is not None and rot_dim > 0:
         ang = pos.to(torch.float32).unsqueeze(-1) * inv_freq.to(qkv.device).unsqueeze(0)  # [T, rot/2]
         cos = (torch.cos(ang) * attn_factor).unsqueeze(1)
         sin = (torch.sin(ang) * attn_factor).unsqueeze(1)
@@ -162,8 +228,9 @@ def rope_append(qkv: torch.Tensor, kv_pages: torch.Tensor, pos: torch.Tensor, sl
     if valid.any():
         sl = slot[valid].long()
         pg, off = sl // page, sl % page
-        kv_pages[pg, 0, :, off, :] = heads[valid, hq : hq + hkv, :]
-        kv_pages[pg, 1, :, off, :] = heads[valid, hq + hkv :, :]
+        k, v = heads[valid, hq : hq + hkv, :], heads[valid, hq + hkv :, :]
+        kv_pages[pg, 0, :, off, :] = kv4_pack(k) if packed else k
+        kv_pages[pg, 1, :, off, :] = kv4_pack(v) if packed else v
 
 
 # --------------------------------------------------------------------------- attention
@@ -192,6 +259,8 @@ def paged_attention(q: torch.Tensor, kv_pages: torch.Tensor, q_seq: torch.Tensor
         pages = page_indices[int(page_indptr[b]) : int(page_indptr[b + 1])].long()
         npg = (total + page - 1) // page
         kv = kv_pages[pages[:npg]]  # [npg, 2, hkv, page, d]
+        if is_kv4(kv, d):
+            kv = kv4_unpack(kv, d)
         k = kv[:, 0].permute(1, 0, 2, 3).reshape(hkv, npg * page, d)[:, :total].float()
         v = kv[:, 1].permute(1, 0, 2, 3).reshape(hkv, npg * page, d)[:, :total].float()
         idx = torch.arange(total, device=q.device)
