@@ -18,6 +18,13 @@ namespace mlcb {
 constexpr int KV4_GROUP = 32;
 __host__ __device__ constexpr int kv4_row_bytes(int d) { return d / 2 + d / KV4_GROUP * 4; }
 
+// (w & mask) | bits in one instruction.
+__device__ __forceinline__ uint32_t kv4_and_or(uint32_t w, uint32_t mask, uint32_t bits) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(w), "r"(mask), "r"(bits));
+  return r;
+}
+
 // Values are clamped to this bound before quantisation (NaN becomes 0), so that lo + 15 s stays finite in T
 // however s was rounded: fp16 65440 (max + 131008 / 2048 < 65520), bf16 2^126.
 template <typename T>
@@ -31,8 +38,8 @@ struct Kv4Type<__half> {
   // shift per word, and one rounding in the final fma.
   static __device__ __forceinline__ void expand4(uint32_t w, uint32_t s2, uint32_t lo2, uint32_t (&out)[4]) {
     const uint32_t w8 = w >> 8;
-    const uint32_t x[4] = {(w & 0x000f000fu) | 0x64006400u, (w & 0x00f000f0u) | 0x54005400u,
-                           (w8 & 0x000f000fu) | 0x64006400u, (w8 & 0x00f000f0u) | 0x54005400u};
+    const uint32_t x[4] = {kv4_and_or(w, 0x000f000fu, 0x64006400u), kv4_and_or(w, 0x00f000f0u, 0x54005400u),
+                           kv4_and_or(w8, 0x000f000fu, 0x64006400u), kv4_and_or(w8, 0x00f000f0u, 0x54005400u)};
     const uint32_t bias[2] = {0x64006400u, 0x54005400u};
     const __half2 s = *reinterpret_cast<const __half2*>(&s2), lo = *reinterpret_cast<const __half2*>(&lo2);
 #pragma unroll
@@ -58,7 +65,7 @@ struct Kv4Type<__nv_bfloat16> {
     const __nv_bfloat162 lo = *reinterpret_cast<const __nv_bfloat162*>(&lo2);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const uint32_t x = ((w >> (4 * i)) & 0x000f000fu) | 0x43004300u;
+      const uint32_t x = kv4_and_or(w >> (4 * i), 0x000f000fu, 0x43004300u);
       const __nv_bfloat162 c =
           __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&x), *reinterpret_cast<const __nv_bfloat162*>(&bias));
       const __nv_bfloat162 v = __hfma2(c, s, lo);

@@ -2,28 +2,32 @@
 // at most 16 query rows per (sequence, kv head) -- the G = hq / hkv heads of the group times the appended tokens.
 //
 // Floor: the cached bytes, 160 per token and kv head at D = 128 (K and V), once. At 44 bytes per ns and SM that
-// leaves 112 clocks, 448 issue slots, per 16 tokens and SM, of which expanding the nibbles takes about 200; the
-// kernel therefore wastes nothing on the query side:
+// leaves 112 clocks, 448 issue slots, per 16 tokens and SM. The nibbles decide whether that is met:
 //
 //   S^T = K Q^T   m16n8k16 with the 16 tokens of a page as M and 8 query rows as N: half the instructions of the
-//                 usual orientation, whose M = 16 rows are mostly padding. A lane's A fragments are two tokens
-//                 and one quarter of the channels -- at D = 128 exactly one quantisation group, so a row is one
-//                 16-byte load of codes and one (lo, s) word. The order of channels along K is free (Q is loaded
-//                 in the same order), which makes the lane's channels contiguous.
+//                 usual orientation, whose M = 16 rows would be mostly padding. Two k-steps cover one quantisation
+//                 group, so K needs no expansion: the fragments hold the integers bias + c that a nibble is
+//                 under a suitable exponent (64 + c in fp16, 128 + c in bf16: one and-or), and the group's step
+//                 multiplies the fp32 result. Bias and minimum are one more k-step: lo_g and s_g against
+//                 sum_g(q) and -bias * sum_g(q), those split into two (bf16: three) terms of the rows' type. K is
+//                 thus never rounded. fp16 queries of 32 and more are first scaled by a power of two, so that the
+//                 sums stay finite.
 //   softmax       in the S^T accumulators: a lane has two query rows and 4 tokens of 16. The reference maximum is
 //                 raised only when some score exceeds it by more than 8 (log2), so the usual step has no shuffle
 //                 and no rescaling; P stays below 2^8 and the final division by the row sum makes it exact.
 //   O^T += V^T P^T  M = 16 channels, N = 8 query rows; P^T fragments come from the S^T accumulators by one
 //                 8 x 8 transpose (movmatrix) per 8 tokens. A fragments want pairs of tokens: two tokens' code
-//                 words are interleaved by halves (prmt) and expanded with the same masks.
+//                 words are interleaved by halves (prmt) and expanded, lo + s c rounded once to the rows' type.
+//                 (The step cannot move to P as it does for K: p * s underflows fp16 for small s.)
 //
-// K and V are rounded to the type of the rows after lo + s c (one rounding), P to the same type; sums, maxima and
-// accumulators are fp32.
+// P is rounded to the rows' type; sums, maxima and accumulators are fp32.
 //
-// Work: a unit is one (sequence, kv head, row block of 8 or 16, KV split). CTAs are persistent; a producer warp
-// streams the units' pages back to back through a ring of 32-token slots (two pages, up to four bulk copies) so
-// that loads never stop between units, four consumer warps take the slots round-robin and merge at the end of
-// each unit. Every wait is bounded (common.cuh).
+// Work: a unit is one (sequence, kv head, block of 8 or 16 query rows). All units' slots of 32 tokens (two pages),
+// laid end to end, are cut into equal shares, one per persistent CTA, so ragged batches and single long sequences
+// load every SM alike; a unit cut between CTAs leaves fp32 partial results that a second kernel joins. In a CTA
+// a producer warp streams the share's pages (bulk copies into a ring of slots) and, per unit, its query rows and a
+// descriptor, ahead of four consumer warps that take the slots round-robin and merge at the end of each unit.
+// Every wait is bounded (common.cuh).
 #include "kv4.cuh"
 
 namespace mlcb {
@@ -31,19 +35,25 @@ namespace mlcb {
 constexpr int KV4_PAGE = 16;
 constexpr int KV4_DEC_THREADS = 160;
 
+
+constexpr int KV4_DEC_ITEMS = 1024;   // items per launch: their prefix sums sit in shared memory
+constexpr int KV4_DEC_MIN_SHARE = 4;  // slots per CTA at least: one per consumer warp
+
 struct Kv4DecParams {
   const void* q;
   const uint8_t* pages;
   void* out;
   float* lse;
-  float* part_o;   // [items, hkv, splits, 16, D] fp32 (splits > 1)
-  float* part_ml;  // [items, hkv, splits, 16, 2]
+  float* part_o;   // [2 CTAs][16][D] fp32: partial rows of a share's first and last unit
+  float* part_ml;  // [2 CTAs][16][2]
+  int* part_unit;  // [CTAs][4]: unit begun here and cut (item or -1, kv head * row blocks + block, pieces)
   const int *item_seq, *item_qstart, *item_ntok, *q_kvlen, *page_indptr, *page_indices;
   const int* q_kvstart;
   const unsigned long long* tree_mask;
   int* status;
   long long q_stride, num_pages;
-  int hq, hkv, group, splits, row_blocks, num_units, sink;
+  int hq, hkv, group, row_blocks, num_items, sink;
+  uint32_t q_flip;           // sign bits of a pair where sm_scale is negative: scale_log2 is its magnitude
   float scale_log2;          // sm_scale * log2(e)
   float cap_k, cap_log2;     // soft cap: scores are kv4_softcap(raw, cap_k, cap_log2); 0 = none
 };
@@ -56,31 +66,20 @@ __device__ __forceinline__ bool kv4_visible(int pos, int kvlen, int start, int s
   return r < 64 && ((tm >> r) & 1ull);
 }
 
-struct Kv4Unit {
-  int item, hk, split, rb, qstart, ntok, valid_rows;
-  int pg_begin, npg;        // pages of this unit, counted over the pages the item visits
-  int sink_pg, skip;        // pages [sink_pg, sink_pg + skip) lie outside every row's window: never fetched
-  int all_from, all_to;     // positions that every row sees: [all_from, all_to), and [0, all_sink) below the window
+// What one item visits: pages [0, npg) of its list, less those that lie outside every row's window.
+struct Kv4Item {
+  int qstart, ntok, npg;
+  int sink_pg, skip;        // pages [sink_pg, sink_pg + skip) of the list are never fetched
+  int all_from, all_to;     // positions [all_from, all_to) are seen by every row (so is the sink below the window)
   const int* list;
-  __device__ __forceinline__ int page_index(int i) const {
-    const int li = pg_begin + i;
-    return li < sink_pg ? li : li + skip;
-  }
 };
 
 template <bool EXT>
-__device__ __forceinline__ Kv4Unit kv4_unit(const Kv4DecParams& p, int u) {
-  Kv4Unit d;
-  d.split = u % p.splits;
-  int r = u / p.splits;
-  d.rb = r % p.row_blocks;
-  r /= p.row_blocks;
-  d.hk = r % p.hkv;
-  d.item = r / p.hkv;
-  const int b = p.item_seq[d.item];
-  d.qstart = p.item_qstart[d.item];
-  d.ntok = p.item_ntok[d.item];
-  d.valid_rows = d.ntok * p.group;
+__device__ __forceinline__ Kv4Item kv4_item(const Kv4DecParams& p, int item) {
+  Kv4Item d;
+  const int b = p.item_seq[item];
+  d.qstart = p.item_qstart[item];
+  d.ntok = p.item_ntok[item];
   int reach = 0, to = 0x7fffffff, from = 0, first = 0x7fffffff;
   for (int i = 0; i < d.ntok; ++i) {
     const int n = p.q_kvlen[d.qstart + i];
@@ -113,12 +112,18 @@ __device__ __forceinline__ Kv4Unit kv4_unit(const Kv4DecParams& p, int u) {
     if (p.status) atomicCAS(p.status, 0, ERR_BAD_INDEX);
     upto = held;
   }
-  const int total = max(0, upto - d.skip);
-  const int per = ((total + p.splits - 1) / p.splits + 1) & ~1;  // whole slots
-  d.pg_begin = d.split * per;
-  d.npg = max(0, min(total, d.pg_begin + per) - d.pg_begin);
+  d.npg = max(0, upto - d.skip);
   return d;
 }
+
+// A unit's part inside one share, handed from the producer to the consumers through shared memory.
+struct Kv4Piece {
+  int qstart, ntok, hk, row0;
+  int slot0, slots;         // slots of the unit: first, count (0: nothing visible)
+  int npg, sink_pg, skip, all_from, all_to;
+  int part;                 // -1: the whole unit, written to out; else the row block of part_o it goes to
+  int last;                 // the share ends here
+};
 
 __device__ __forceinline__ uint32_t kv4_movmatrix(uint32_t v) {
   uint32_t r;
@@ -127,29 +132,87 @@ __device__ __forceinline__ uint32_t kv4_movmatrix(uint32_t v) {
 }
 
 template <typename T>
-__device__ __forceinline__ void kv4_mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                        uint32_t b1);
+__device__ __forceinline__ void kv4_mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                        uint32_t b1, const float (&c)[4]);
 template <>
-__device__ __forceinline__ void kv4_mma<__half>(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
-                                                uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+__device__ __forceinline__ void kv4_mma<__half>(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                                uint32_t b0, uint32_t b1, const float (&c)[4]) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
 }
 template <>
-__device__ __forceinline__ void kv4_mma<__nv_bfloat16>(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
-                                                       uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+__device__ __forceinline__ void kv4_mma<__nv_bfloat16>(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                                uint32_t b0, uint32_t b1, const float (&c)[4]) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
+}
+// Pairs of integers bias + c for the nibbles at bits 4 i of both halves.
+template <typename T>
+__device__ __forceinline__ void kv4_raw4(uint32_t w, uint32_t (&out)[4]);
+template <>
+__device__ __forceinline__ void kv4_raw4<__half>(uint32_t w, uint32_t (&out)[4]) {
+  out[0] = kv4_and_or(w << 4, 0x00f000f0u, 0x54005400u);
+  out[1] = kv4_and_or(w, 0x00f000f0u, 0x54005400u);
+  out[2] = kv4_and_or(w >> 4, 0x00f000f0u, 0x54005400u);
+  out[3] = kv4_and_or(w >> 8, 0x00f000f0u, 0x54005400u);
+}
+template <>
+__device__ __forceinline__ void kv4_raw4<__nv_bfloat16>(uint32_t w, uint32_t (&out)[4]) {
+  out[0] = kv4_and_or(w, 0x000f000fu, 0x43004300u);
+  out[1] = kv4_and_or(w >> 4, 0x000f000fu, 0x43004300u);
+  out[2] = kv4_and_or(w >> 8, 0x000f000fu, 0x43004300u);
+  out[3] = kv4_and_or(w >> 12, 0x000f000fu, 0x43004300u);
+}
+template <typename T>
+struct Kv4Bias;
+template <>
+struct Kv4Bias<__half> {
+  static constexpr float BIAS = 64.f;
+  static constexpr uint32_t MINUS = 0xd400d400u;  // a pair of -64
+  static constexpr int TERMS = 2;                 // 11 bits each: the group sums to 2^-22
+};
+template <>
+struct Kv4Bias<__nv_bfloat16> {
+  static constexpr float BIAS = 128.f;
+  static constexpr uint32_t MINUS = 0xc300c300u;  // a pair of -128
+  static constexpr int TERMS = 3;                 // 8 bits each: 2^-24
+};
+
+// s of a (lo, s) word as fp32
+template <typename T>
+__device__ __forceinline__ float kv4_step(uint32_t meta);
+template <>
+__device__ __forceinline__ float kv4_step<__half>(uint32_t meta) {
+  return __high2float(*reinterpret_cast<const __half2*>(&meta));
+}
+template <>
+__device__ __forceinline__ float kv4_step<__nv_bfloat16>(uint32_t meta) {
+  return __uint_as_float(meta & 0xffff0000u);
 }
 
-// N code words from shared memory (rows are 16-, 8- or 4-byte aligned for N = 4, 2, 1).
+// (a.x, a.y) * (b.x, b.y) + (c.x, c.y), and a sum of pairs, in one instruction each.
+__device__ __forceinline__ float2 kv4_fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("fma.rn.ftz.f32x2 %0, %1, %2, %3;"
+      : "=l"(reinterpret_cast<unsigned long long&>(d))
+      : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)),
+        "l"(reinterpret_cast<unsigned long long&>(c)));
+  return d;
+}
+__device__ __forceinline__ float2 kv4_add2(float2 a, float2 b) {
+  float2 d;
+  asm("add.rn.ftz.f32x2 %0, %1, %2;"
+      : "=l"(reinterpret_cast<unsigned long long&>(d))
+      : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)));
+  return d;
+}
+
+// N words from shared memory (the address is aligned to 16, 8 or 4 bytes for N = 4, 2, 1).
 template <int N>
 __device__ __forceinline__ void kv4_words(const uint8_t* p, uint32_t (&w)[N]) {
-  if (N % 4 == 0) {
+  if constexpr (N % 4 == 0) {
 #pragma unroll
     for (int i = 0; i < N / 4; ++i) {
       const uint4 v = reinterpret_cast<const uint4*>(p)[i];
@@ -158,13 +221,27 @@ __device__ __forceinline__ void kv4_words(const uint8_t* p, uint32_t (&w)[N]) {
       w[4 * i + 2] = v.z;
       w[4 * i + 3] = v.w;
     }
-  } else if (N == 2) {
+  } else if constexpr (N == 2) {
     const uint2 v = *reinterpret_cast<const uint2*>(p);
     w[0] = v.x;
     w[1] = v.y;
   } else {
     w[0] = *reinterpret_cast<const uint32_t*>(p);
   }
+}
+
+// Row `row` (of the item's rows) of the output: acc[c] = channel 32 c + lane, scaled by 1 / L. A row that sees nothing
+// is 0 with log-sum-exp -inf; NaN stays NaN.
+template <typename T, int D>
+__device__ __forceinline__ void kv4_finish_row(const Kv4DecParams& p, int qstart, int hk, int row, float M, float L,
+                                               const float (&acc)[D / 32]) {
+  const int lane = threadIdx.x & 31;
+  const size_t at = static_cast<size_t>(qstart + row / p.group) * p.hq + hk * p.group + row % p.group;
+  const float inv = L == 0.f ? 0.f : 1.f / L;
+  T* dst = reinterpret_cast<T*>(p.out) + at * D;
+#pragma unroll
+  for (int c = 0; c < D / 32; ++c) dst[c * 32 + lane] = Cvt<T>::from_f(acc[c] * inv);
+  if (p.lse && lane == 0) p.lse[at] = L == 0.f ? -INFINITY : (M + log2f(L)) * 0.6931471805599453f;
 }
 
 template <int D, int NT>
@@ -174,68 +251,170 @@ struct Kv4DecShape {
   static constexpr int SLOT_BYTES = 4 * PAGE_BYTES;            // K, V of two pages
   static constexpr int SLOTS = D == 256 ? 4 : 8;               // a multiple of the four consumer warps
   static constexpr int ROWS = 8 * NT;
+  static constexpr int CTAS = D < 256 && NT == 1 ? 3 : 2;      // resident per SM: what the registers allow
+  static constexpr int Q_BYTES = ROWS * D * 2;                 // query rows of a piece; two pieces are held
   static constexpr int MERGE_BYTES = 4 * ROWS * (D + 2) * 4;   // four warps' O rows and (m, l) pairs
-  static constexpr int SMEM = SLOTS * SLOT_BYTES + MERGE_BYTES + 16 * SLOTS + 16;
+  static constexpr int OFF_Q = SLOTS * SLOT_BYTES;
+  static constexpr int OFF_MERGE = OFF_Q + 2 * Q_BYTES;
+  static constexpr int OFF_BAR = OFF_MERGE + MERGE_BYTES;
+  static constexpr int OFF_PIECE = OFF_BAR + 8 * (2 * SLOTS + 4);
+  static constexpr int OFF_SCAN = OFF_PIECE + 2 * 64;          // item prefix sums, sized by the launch
+  static_assert(sizeof(Kv4Piece) <= 64, "a piece descriptor has 64 bytes");
 };
 
 template <typename T, int D, int NT, bool EXT>
-__global__ void __launch_bounds__(KV4_DEC_THREADS, 2) kv4_decode_kernel(const Kv4DecParams p) {
+__global__ void __launch_bounds__(KV4_DEC_THREADS, Kv4DecShape<D, NT>::CTAS) kv4_decode_kernel(const Kv4DecParams p) {
   using Shape = Kv4DecShape<D, NT>;
   constexpr int ROW = Shape::ROW, PB = Shape::PAGE_BYTES, SLOTS = Shape::SLOTS, ROWS = Shape::ROWS;
-  constexpr int KW = D / 32;   // K code words per lane and token
+  constexpr int GROUPS = D / KV4_GROUP;
   constexpr int VW = D / 64;   // V code words per lane and token
   pdl_launch_dependents();
   extern __shared__ __align__(128) uint8_t smem[];
-  float* sm_o = reinterpret_cast<float*>(smem + SLOTS * Shape::SLOT_BYTES);  // [4][ROWS][D]
-  float* sm_ml = sm_o + 4 * ROWS * D;                                       // [4][ROWS][2]
-  uint64_t* full = reinterpret_cast<uint64_t*>(sm_ml + 4 * ROWS * 2);
+  float* sm_o = reinterpret_cast<float*>(smem + Shape::OFF_MERGE);  // [4][ROWS][D]
+  float* sm_ml = sm_o + 4 * ROWS * D;                               // [4][ROWS][2]
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + Shape::OFF_BAR);
   uint64_t* empty = full + SLOTS;
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(empty + SLOTS);
+  uint64_t* piece_full = empty + SLOTS;   // [2]
+  uint64_t* piece_empty = piece_full + 2; // [2]
+  Kv4Piece* pieces = reinterpret_cast<Kv4Piece*>(smem + Shape::OFF_PIECE);  // [2], 64 bytes apart
+  int* scan = reinterpret_cast<int*>(smem + Shape::OFF_SCAN);               // [num_items + 1]
+  __shared__ int abort_word, leave_word;
+  volatile int* abort_flag = &abort_word;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x < SLOTS) {
     mbar_init(&full[threadIdx.x], 1);
     mbar_init(&empty[threadIdx.x], 1);
-    mbar_fence_init();
   }
-  if (threadIdx.x == 0) *abort_flag = 0;
+  if (threadIdx.x < 2) {
+    mbar_init(&piece_full[threadIdx.x], 1);
+    mbar_init(&piece_empty[threadIdx.x], 4);
+  }
+  mbar_fence_init();
+  if (threadIdx.x == 0) abort_word = 0;
+  // slots of every item (an item without a visible position takes one, so that its rows get written)
+  for (int i = threadIdx.x; i < p.num_items; i += KV4_DEC_THREADS) scan[i] = max(1, (kv4_item<EXT>(p, i).npg + 1) >> 1);
   __syncthreads();
+  if (warp == 0) {
+    int sum = 0;
+    for (int base = 0; base < p.num_items; base += 32) {
+      const int n = base + lane < p.num_items ? scan[base + lane] : 0;
+      int x = n;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
+      }
+      if (base + lane < p.num_items) scan[base + lane] = sum + x - n;
+      sum += __shfl_sync(0xffffffffu, x, 31);
+    }
+    if (lane == 0) scan[p.num_items] = sum;
+  }
+  __syncthreads();
+  const int per_item = p.hkv * p.row_blocks;
+  const long long total = static_cast<long long>(scan[p.num_items]) * per_item;
+  const long long share = max((total + gridDim.x - 1) / gridDim.x, static_cast<long long>(KV4_DEC_MIN_SHARE));
+  const long long begin = blockIdx.x * share, end = min(total, begin + share);
+  if (begin >= end) {
+    if (threadIdx.x == 0) p.part_unit[blockIdx.x * 4] = -1;
+    return;
+  }
 
   if (warp == 4) {
     // ---------------------------------------------------------------- producer
-    // Lane i holds the page number of the unit's page base + i (one coalesced load per 32 pages); lanes 0..3 each
-    // issue one copy of a slot (K and V of its two pages).
-    uint32_t g = 0;
+    int lo = 0, hi = p.num_items - 1;  // the item that holds slot `begin`
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (static_cast<long long>(scan[mid]) * per_item <= begin) lo = mid;
+      else hi = mid - 1;
+    }
+    int item = lo;
+    long long at = begin;
+    uint32_t g = 0, k = 0;
     bool ok = true;
-    for (int u = blockIdx.x; u < p.num_units && ok; u += gridDim.x) {
-      const Kv4Unit d = kv4_unit<EXT>(p, u);
-      for (int base = 0; base < d.npg && ok; base += 32) {
+    Kv4Item d = kv4_item<EXT>(p, item);
+    while (at < end && ok) {
+      if (at >= static_cast<long long>(scan[item + 1]) * per_item) d = kv4_item<EXT>(p, ++item);
+      const int n = scan[item + 1] - scan[item];
+      const int local = static_cast<int>(at - static_cast<long long>(scan[item]) * per_item);
+      const int unit = local / n, slot0 = local % n;
+      const int take = static_cast<int>(min(static_cast<long long>(n - slot0), end - at));
+      const bool begins = slot0 == 0, ends = slot0 + take == n;
+      const int hk = unit / p.row_blocks, row0 = unit % p.row_blocks * ROWS;
+      const int rows = min(ROWS, d.ntok * p.group - row0);
+      // ---- descriptor and query rows
+      const int e = k & 1;
+      if (k >= 2) {
+        ok = mbar_wait(&piece_empty[e], ((k >> 1) & 1) ^ 1, abort_flag, p.status, ERR_WAIT_PRODUCER);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+      }
+      if (lane == 0) {
+        Kv4Piece* pc = reinterpret_cast<Kv4Piece*>(reinterpret_cast<uint8_t*>(pieces) + e * 64);
+        pc->qstart = d.qstart;
+        pc->ntok = d.ntok;
+        pc->hk = hk;
+        pc->row0 = row0;
+        pc->slot0 = slot0;
+        pc->slots = min(take, (d.npg + 1) / 2 - slot0);
+        pc->npg = d.npg;
+        pc->sink_pg = d.sink_pg;
+        pc->skip = d.skip;
+        pc->all_from = d.all_from;
+        pc->all_to = d.all_to;
+        pc->part = begins && ends ? -1 : static_cast<int>(blockIdx.x) * 2 + (begins ? 1 : 0);
+        pc->last = at + take >= end;
+        if (at + take >= end) {
+          // pieces of a unit that begins here and runs on: this share's and those of the CTAs after it
+          const long long rest = n - take;
+          int* pu = p.part_unit + blockIdx.x * 4;
+          pu[0] = begins && !ends ? item : -1;
+          pu[1] = unit;
+          pu[2] = 1 + static_cast<int>((rest + share - 1) / share);
+        }
+        mbar_expect_tx(&piece_full[e], max(0, rows) * D * 2);
+      }
+      __syncwarp();
+      for (int tok = row0 / p.group + lane; tok * p.group < row0 + rows; tok += 32) {
+        const int r0 = max(row0, tok * p.group), r1 = min(row0 + rows, (tok + 1) * p.group);
+        const uint8_t* src = reinterpret_cast<const uint8_t*>(p.q) +
+                             (static_cast<size_t>(d.qstart + tok) * p.q_stride +
+                              static_cast<size_t>(hk * p.group + r0 - tok * p.group) * D) * 2;
+        bulk_load(smem + Shape::OFF_Q + e * Shape::Q_BYTES + (r0 - row0) * D * 2, src, (r1 - r0) * D * 2, &piece_full[e]);
+      }
+      ++k;
+      // ---- pages: lane i holds the number of page base + i (one coalesced load per 32); lanes 0..3 issue a slot's
+      // copies (K and V of its two pages)
+      const int pg0 = slot0 * 2, pg1 = min(d.npg, (slot0 + take) * 2);
+      for (int base = pg0; base < pg1 && ok; base += 32) {
         int mine = 0;
-        if (base + lane < d.npg) {
-          mine = d.list[d.page_index(base + lane)];
+        if (base + lane < pg1) {
+          const int li = base + lane;
+          mine = d.list[li < d.sink_pg ? li : li + d.skip];
           if (mine >= p.num_pages) {
             if (p.status) atomicCAS(p.status, 0, ERR_BAD_INDEX);
             mine = 0;
           }
           if (mine < 0) mine = 0;  // released by a sliding window: every position of it is masked
         }
-        const int n = min(32, d.npg - base);
-        for (int i = 0; i < n; i += 2, ++g) {
+        const int m = min(32, pg1 - base);
+        for (int i = 0; i < m; i += 2, ++g) {
           const int s = g % SLOTS;
           if (g >= SLOTS) {
             ok = mbar_wait(&empty[s], ((g / SLOTS) & 1) ^ 1, abort_flag, p.status, ERR_WAIT_PRODUCER);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
           }
-          const int here = min(2, n - i);
+          const int here = min(2, m - i);
           if (lane == 0) mbar_expect_tx(&full[s], here * 2 * PB);
           __syncwarp();
           const int pg = __shfl_sync(0xffffffffu, mine, i + ((lane >> 1) & 1));
           if (lane < 2 * here) {
-            const size_t block = (static_cast<size_t>(pg) * 2 + (lane & 1)) * p.hkv + d.hk;
+            const size_t block = (static_cast<size_t>(pg) * 2 + (lane & 1)) * p.hkv + hk;
             bulk_load(smem + s * Shape::SLOT_BYTES + lane * PB, p.pages + block * PB, PB, &full[s]);
           }
         }
       }
+      at += take;
     }
     return;
   }
@@ -243,42 +422,82 @@ __global__ void __launch_bounds__(KV4_DEC_THREADS, 2) kv4_decode_kernel(const Kv
   // ------------------------------------------------------------------ consumers
   const int r = lane >> 2, t = lane & 3;
   uint32_t g0 = 0;
-  for (int u = blockIdx.x; u < p.num_units; u += gridDim.x) {
-    const Kv4Unit d = kv4_unit<EXT>(p, u);
-    const int row0 = d.rb * ROWS;                           // first query row of this unit
-    const int rows = min(ROWS, d.valid_rows - row0);        // may be <= 0: an empty row block
-    // Q^T fragments: lane (r, t) holds row r (+ 8 per n-tile), channels [t D / 4, (t + 1) D / 4)
-    uint32_t qb[NT][D / 16][2];
+  for (uint32_t k = 0;; ++k) {
+    const int e = k & 1;
+    bool ok = mbar_wait(&piece_full[e], (k >> 1) & 1, abort_flag, p.status, ERR_WAIT_TMA);
+    ok = __all_sync(0xffffffffu, ok);
+    const Kv4Piece pc = *reinterpret_cast<const Kv4Piece*>(reinterpret_cast<const uint8_t*>(pieces) + e * 64);
+    // may be <= 0: an empty row block. After a wait that ran out nothing of the piece is touched.
+    const int rows = ok ? min(ROWS, pc.ntok * p.group - pc.row0) : 0;
+    const int npg = pc.npg;
+    // Q^T fragments: lane (r, t) holds channels 8 t .. 8 t + 7 of every group of row r (+ 8 per n-tile): two k-steps
+    uint32_t qb[NT][GROUPS][4];
+    uint32_t top_bits = 0;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      const int row = nt * 8 + r;
-      const bool live = row < rows;
-      const int tok = d.qstart + (live ? (row0 + row) / p.group : 0), head = d.hk * p.group + (live ? (row0 + row) % p.group : 0);
-      const uint8_t* src = reinterpret_cast<const uint8_t*>(p.q) +
-                           (static_cast<size_t>(tok) * p.q_stride + static_cast<size_t>(head) * D + t * (D / 4)) * 2;
+      const uint4* src = reinterpret_cast<const uint4*>(smem + Shape::OFF_Q + e * Shape::Q_BYTES + (nt * 8 + r) * D * 2) + t;
+      const bool live = nt * 8 + r < rows;
 #pragma unroll
-      for (int i = 0; i < D / 32; ++i) {
-        const uint4 v = live ? reinterpret_cast<const uint4*>(src)[i] : make_uint4(0, 0, 0, 0);
-        qb[nt][2 * i][0] = v.x;
-        qb[nt][2 * i][1] = v.y;
-        qb[nt][2 * i + 1][0] = v.z;
-        qb[nt][2 * i + 1][1] = v.w;
+      for (int grp = 0; grp < GROUPS; ++grp) {
+        const uint4 v = live ? src[grp * 4] : make_uint4(0, 0, 0, 0);
+        qb[nt][grp][0] = v.x ^ p.q_flip;
+        qb[nt][grp][1] = v.y ^ p.q_flip;
+        qb[nt][grp][2] = v.z ^ p.q_flip;
+        qb[nt][grp][3] = v.w ^ p.q_flip;
+        if constexpr (Kv4Bias<T>::TERMS == 2) {
+          const uint32_t mag = 0x7fff7fffu;
+          top_bits = __vmaxu2(top_bits, __vmaxu2(__vmaxu2(v.x & mag, v.y & mag), __vmaxu2(v.z & mag, v.w & mag)));
+        }
       }
     }
-    // this lane's score columns: rows 2 t and 2 t + 1 of each n-tile
-    int kvlen[NT][2], start[NT][2];
-    unsigned long long tm[NT][2];
+    float unit_scale = 1.f;
+    if constexpr (Kv4Bias<T>::TERMS == 2) {
+      // fp16: the largest magnitude's exponent field is 20 for 32 <= |q| < 64; below 32, 64 sum|q| stays finite
+      const uint32_t all = __reduce_max_sync(0xffffffffu, max(top_bits & 0xffffu, top_bits >> 16));
+      const int over = static_cast<int>(all >> 10) - 19;
+      if (over > 0 && over < 12) {  // 12: infinity or NaN, left alone
+        const __half2 f = __float2half2_rn(exp2f(static_cast<float>(-over)));
+        unit_scale = exp2f(static_cast<float>(over));
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        const int row = nt * 8 + 2 * t + c;
-        const bool live = row < rows;
-        const int tok = d.qstart + (live ? (row0 + row) / p.group : 0);
-        kvlen[nt][c] = live ? p.q_kvlen[tok] : 0;
-        start[nt][c] = EXT && live && p.q_kvstart ? p.q_kvstart[tok] : 0;
-        tm[nt][c] = EXT && live && p.tree_mask ? p.tree_mask[tok] : 0ull;
+          for (int grp = 0; grp < GROUPS; ++grp)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              const __half2 v = __hmul2(*reinterpret_cast<const __half2*>(&qb[nt][grp][x]), f);
+              qb[nt][grp][x] = *reinterpret_cast<const uint32_t*>(&v);
+            }
       }
+    }
+    // scores in log2 units are raw * scale (or capped: kv4_softcap(raw, cap_k, cap_log2), scale 1)
+    const float cap_k = EXT ? p.cap_k * unit_scale : 0.f;
+    const float scale = EXT && p.cap_log2 != 0.f ? 1.f : p.scale_log2 * unit_scale;
+    // B fragments of the minimum / bias k-step: sums of q over groups 2 t and 2 t + 1 of row r, and -bias times them
+    uint32_t ql[NT][Kv4Bias<T>::TERMS][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      float sum[2] = {0.f, 0.f};
+#pragma unroll
+      for (int grp = 0; grp < GROUPS; ++grp) {
+        const float zero[4] = {0.f, 0.f, 0.f, 0.f};
+        float c[4];
+        constexpr uint32_t mb = Kv4Bias<T>::MINUS;
+        kv4_mma<T>(c, mb, mb, mb, mb, qb[nt][grp][0], qb[nt][grp][1], zero);
+        kv4_mma<T>(c, mb, mb, mb, mb, qb[nt][grp][2], qb[nt][grp][3], c);
+        // c[0], c[1] are columns 2 t, 2 t + 1; column r sits in the lanes with t = r / 2
+        const float x = __shfl_sync(0xffffffffu, c[0], (lane & 28) | (r >> 1));
+        const float y = __shfl_sync(0xffffffffu, c[1], (lane & 28) | (r >> 1));
+        if (grp / 2 == t) sum[grp & 1] = (r & 1) ? y : x;
+      }
+#pragma unroll
+      for (int k2 = 0; k2 < Kv4Bias<T>::TERMS; ++k2) {
+        const float h0 = Cvt<T>::to_f(Cvt<T>::from_f(sum[0])), h1 = Cvt<T>::to_f(Cvt<T>::from_f(sum[1]));
+        ql[nt][k2][0] = Kv4Type<T>::pack(h0 * (-1.f / Kv4Bias<T>::BIAS), h1 * (-1.f / Kv4Bias<T>::BIAS));
+        ql[nt][k2][1] = Kv4Type<T>::pack(h0, h1);
+        sum[0] -= h0;
+        sum[1] -= h1;
+      }
+    }
     float o[NT][D / 16][4];
     float m[NT][2], l[NT][2];
 #pragma unroll
@@ -288,74 +507,95 @@ __global__ void __launch_bounds__(KV4_DEC_THREADS, 2) kv4_decode_kernel(const Kv
 #pragma unroll
       for (int j = 0; j < D / 16; ++j) o[nt][j][0] = o[nt][j][1] = o[nt][j][2] = o[nt][j][3] = 0.f;
     }
-    const int nslots = (d.npg + 1) >> 1;
-    bool ok = true;
-    for (int i = (warp - static_cast<int>(g0 & 3u)) & 3; i < nslots && ok; i += 4) {
+    for (int i = (warp - static_cast<int>(g0 & 3u)) & 3; i < pc.slots && ok; i += 4) {
       const uint32_t g = g0 + static_cast<uint32_t>(i);
       const int s = g % SLOTS;
       ok = mbar_wait(&full[s], (g / SLOTS) & 1, abort_flag, p.status, ERR_WAIT_TMA);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       const uint8_t* slot = smem + s * Shape::SLOT_BYTES;
-      const bool two = 2 * i + 1 < d.npg;
-      const int at[2] = {d.page_index(2 * i) * KV4_PAGE, two ? d.page_index(2 * i + 1) * KV4_PAGE : 0x3fffffff};
       // ---- S^T = K Q^T
       float sc[2][NT][4];
 #pragma unroll
       for (int pg = 0; pg < 2; ++pg) {
         const uint8_t* k0 = slot + pg * 2 * PB + r * ROW;
         const uint8_t* k1 = k0 + 8 * ROW;
-        uint32_t w0[KW], w1[KW];
-        kv4_words<KW>(k0 + t * (D / 8), w0);
-        kv4_words<KW>(k1 + t * (D / 8), w1);
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) sc[pg][nt][0] = sc[pg][nt][1] = sc[pg][nt][2] = sc[pg][nt][3] = 0.f;
-#pragma unroll
-        for (int w = 0; w < KW; ++w) {
-          const int grp = (t * (D / 4) + w * 8) / KV4_GROUP;
-          const uint32_t m0 = *reinterpret_cast<const uint32_t*>(k0 + D / 2 + grp * 4);
-          const uint32_t m1 = *reinterpret_cast<const uint32_t*>(k1 + D / 2 + grp * 4);
-          uint32_t e0[4], e1[4];
-          Kv4Type<T>::expand4(w0[w], __byte_perm(m0, m0, 0x3232), __byte_perm(m0, m0, 0x1010), e0);
-          Kv4Type<T>::expand4(w1[w], __byte_perm(m1, m1, 0x3232), __byte_perm(m1, m1, 0x1010), e1);
+        {
+          // k-slots 2 t, 2 t + 1 are the minima of groups 2 t, 2 t + 1, k-slots + 8 their steps. Where there are fewer
+          // groups than slots ql is 0 and any group's words do.
+          const int go = (2 * t) % GROUPS * 4;
+          const uint2 x = *reinterpret_cast<const uint2*>(k0 + D / 2 + go), y = *reinterpret_cast<const uint2*>(k1 + D / 2 + go);
+          const uint32_t a0 = __byte_perm(x.x, x.y, 0x5410), a1 = __byte_perm(y.x, y.y, 0x5410);
+          const uint32_t a2 = __byte_perm(x.x, x.y, 0x7632), a3 = __byte_perm(y.x, y.y, 0x7632);
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
-            kv4_mma<T>(sc[pg][nt], e0[0], e1[0], e0[1], e1[1], qb[nt][2 * w][0], qb[nt][2 * w][1]);
-            kv4_mma<T>(sc[pg][nt], e0[2], e1[2], e0[3], e1[3], qb[nt][2 * w + 1][0], qb[nt][2 * w + 1][1]);
+            const float zero[4] = {0.f, 0.f, 0.f, 0.f};
+            kv4_mma<T>(sc[pg][nt], a0, a1, a2, a3, ql[nt][0][0], ql[nt][0][1], zero);
+#pragma unroll
+            for (int k2 = 1; k2 < Kv4Bias<T>::TERMS; ++k2)
+              kv4_mma<T>(sc[pg][nt], a0, a1, a2, a3, ql[nt][k2][0], ql[nt][k2][1], sc[pg][nt]);
+          }
+        }
+        uint32_t m0[GROUPS], m1[GROUPS];
+        kv4_words<GROUPS>(k0 + D / 2, m0);
+        kv4_words<GROUPS>(k1 + D / 2, m1);
+#pragma unroll
+        for (int grp = 0; grp < GROUPS; ++grp) {
+          uint32_t e0[4], e1[4];
+          kv4_raw4<T>(*reinterpret_cast<const uint32_t*>(k0 + grp * 16 + t * 4), e0);
+          kv4_raw4<T>(*reinterpret_cast<const uint32_t*>(k1 + grp * 16 + t * 4), e1);
+          const float s0 = kv4_step<T>(m0[grp]), s1 = kv4_step<T>(m1[grp]);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            const float zero[4] = {0.f, 0.f, 0.f, 0.f};
+            float c[4];
+            kv4_mma<T>(c, e0[0], e1[0], e0[1], e1[1], qb[nt][grp][0], qb[nt][grp][1], zero);
+            kv4_mma<T>(c, e0[2], e1[2], e0[3], e1[3], qb[nt][grp][2], qb[nt][grp][3], c);
+            sc[pg][nt][0] = fmaf(s0, c[0], sc[pg][nt][0]);
+            sc[pg][nt][1] = fmaf(s0, c[1], sc[pg][nt][1]);
+            sc[pg][nt][2] = fmaf(s1, c[2], sc[pg][nt][2]);
+            sc[pg][nt][3] = fmaf(s1, c[3], sc[pg][nt][3]);
           }
         }
       }
       // ---- scale, cap, mask. A slot that every row sees in full (all but the ends of a sequence or window) skips
       // the per-element test; the others also drop V of tokens that no row sees, whatever their bytes hold.
-      bool plain = two;
-#pragma unroll
-      for (int pg = 0; pg < 2; ++pg)
-        plain = plain && at[pg] + KV4_PAGE <= d.all_to && (!EXT || at[pg] >= d.all_from || at[pg] + KV4_PAGE <= p.sink);
+      const int pi = (pc.slot0 + i) * 2;
+      const bool two = pi + 1 < npg;
+      const int at0 = (!EXT || pi < pc.sink_pg ? pi : pi + pc.skip) * KV4_PAGE;
+      const int at1 = two ? (!EXT || pi + 1 < pc.sink_pg ? pi + 1 : pi + 1 + pc.skip) * KV4_PAGE : 0x3fffffff;
+      bool plain = at1 + KV4_PAGE <= pc.all_to;
+      if (EXT) plain = plain && (at0 >= pc.all_from || at0 + KV4_PAGE <= p.sink) && (at1 >= pc.all_from || at1 + KV4_PAGE <= p.sink);
       uint32_t seen = 0xffffffffu;
-#pragma unroll
-      for (int pg = 0; pg < 2; ++pg)
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            float v = sc[pg][nt][c];
-            v = EXT && p.cap_log2 != 0.f ? kv4_softcap(v, p.cap_k, p.cap_log2) : v * p.scale_log2;
-            sc[pg][nt][c] = v;
-          }
-      if (!plain) {
+      if (EXT && p.cap_log2 != 0.f) {
 #pragma unroll
         for (int pg = 0; pg < 2; ++pg)
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int c = 0; c < 4; ++c)
-              if (!kv4_visible(at[pg] + r + (c >> 1) * 8, kvlen[nt][c & 1], start[nt][c & 1], p.sink, tm[nt][c & 1]))
-                sc[pg][nt][c] = -INFINITY;
-        const int pos = (lane < 16 ? at[0] : at[1]) + (lane & 15);  // lane = token of the slot
+            for (int c = 0; c < 4; ++c) sc[pg][nt][c] = kv4_softcap(sc[pg][nt][c], cap_k, p.cap_log2);
+      }
+      if (!plain) {
+        auto sees = [&](int pos, int tok) {
+          return kv4_visible(pos, p.q_kvlen[tok], EXT && p.q_kvstart ? p.q_kvstart[tok] : 0, p.sink,
+                             EXT && p.tree_mask ? p.tree_mask[tok] : 0ull);
+        };
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const int row = nt * 8 + 2 * t + c;
+            const bool live = row < rows;
+            const int tok = pc.qstart + (live ? (pc.row0 + row) / p.group : 0);
+#pragma unroll
+            for (int pg = 0; pg < 2; ++pg)
+#pragma unroll
+              for (int h = 0; h < 2; ++h)
+                if (!live || !sees((pg ? at1 : at0) + r + h * 8, tok)) sc[pg][nt][c + 2 * h] = -INFINITY;
+          }
+        const int pos = (lane < 16 ? at0 : at1) + (lane & 15);  // lane = token of the slot
         bool any = false;
-        for (int q = 0; q < d.ntok; ++q)
-          any = any || kv4_visible(pos, p.q_kvlen[d.qstart + q], EXT && p.q_kvstart ? p.q_kvstart[d.qstart + q] : 0, p.sink,
-                                   EXT && p.tree_mask ? p.tree_mask[d.qstart + q] : 0ull);
+        for (int q = 0; q < pc.ntok; ++q) any = any || sees(pos, pc.qstart + q);
         seen = __ballot_sync(0xffffffffu, any);
       }
       // ---- running maximum (raised lazily) and P
@@ -365,7 +605,7 @@ __global__ void __launch_bounds__(KV4_DEC_THREADS, 2) kv4_decode_kernel(const Kv
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          top[nt][c] = fmaxf(fmaxf(sc[0][nt][c], sc[0][nt][c + 2]), fmaxf(sc[1][nt][c], sc[1][nt][c + 2]));
+          top[nt][c] = fmaxf(fmaxf(sc[0][nt][c], sc[0][nt][c + 2]), fmaxf(sc[1][nt][c], sc[1][nt][c + 2])) * scale;
           raise = raise || top[nt][c] > m[nt][c] + 8.f;
         }
       if (__any_sync(0xffffffffu, raise)) {
@@ -391,28 +631,35 @@ __global__ void __launch_bounds__(KV4_DEC_THREADS, 2) kv4_decode_kernel(const Kv
       uint32_t pb[2][NT][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        const float ms0 = m[nt][0] == -INFINITY ? 0.f : m[nt][0], ms1 = m[nt][1] == -INFINITY ? 0.f : m[nt][1];
+        const float2 shift = make_float2(m[nt][0] == -INFINITY ? 0.f : -m[nt][0], m[nt][1] == -INFINITY ? 0.f : -m[nt][1]);
+        float2 ls = make_float2(l[nt][0], l[nt][1]);
 #pragma unroll
-        for (int pg = 0; pg < 2; ++pg) {
-          const float e0 = exp2f(sc[pg][nt][0] - ms0), e1 = exp2f(sc[pg][nt][1] - ms1);
-          const float e2 = exp2f(sc[pg][nt][2] - ms0), e3 = exp2f(sc[pg][nt][3] - ms1);
-          l[nt][0] += e0 + e2;
-          l[nt][1] += e1 + e3;
-          pb[pg][nt][0] = kv4_movmatrix(Kv4Type<T>::pack(e0, e1));
-          pb[pg][nt][1] = kv4_movmatrix(Kv4Type<T>::pack(e2, e3));
-        }
+        for (int pg = 0; pg < 2; ++pg)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const float2 x = kv4_fma2(make_float2(sc[pg][nt][2 * h], sc[pg][nt][2 * h + 1]), make_float2(scale, scale), shift);
+            const float2 w = make_float2(exp2f(x.x), exp2f(x.y));
+            ls = kv4_add2(ls, w);
+            pb[pg][nt][h] = kv4_movmatrix(Kv4Type<T>::pack(w.x, w.y));
+          }
+        l[nt][0] = ls.x;
+        l[nt][1] = ls.y;
       }
       // ---- O^T += V^T P^T: this lane expands channels [r D / 8, (r + 1) D / 8) of tokens 2t, 2t+1, 2t+8, 2t+9
 #pragma unroll
       for (int pg = 0; pg < 2; ++pg) {
-        const uint8_t* vb = slot + (pg * 2 + 1) * PB;
+        const uint8_t* vb = slot + (pg * 2 + 1) * PB + 2 * t * ROW;
         uint32_t w[4][VW], meta[4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int token = 2 * t + (k & 1) + (k >> 1) * 8;
-          kv4_words<VW>(vb + token * ROW + r * (D / 16), w[k]);
-          meta[k] = *reinterpret_cast<const uint32_t*>(vb + token * ROW + D / 2 + (r * (D / 8) / KV4_GROUP) * 4);
-          if (!((seen >> (pg * 16 + token)) & 1u)) meta[k] = 0u;
+        for (int x = 0; x < 4; ++x) {
+          const uint8_t* v = vb + ((x & 1) + (x >> 1) * 8) * ROW;
+          kv4_words<VW>(v + r * (D / 16), w[x]);
+          meta[x] = *reinterpret_cast<const uint32_t*>(v + D / 2 + (r * (D / 8) / KV4_GROUP) * 4);
+        }
+        if (!plain) {
+#pragma unroll
+          for (int x = 0; x < 4; ++x)
+            if (!((seen >> (pg * 16 + 2 * t + (x & 1) + (x >> 1) * 8)) & 1u)) meta[x] = 0u;
         }
         const uint32_t lo_ab = __byte_perm(meta[0], meta[1], 0x5410), s_ab = __byte_perm(meta[0], meta[1], 0x7632);
         const uint32_t lo_cd = __byte_perm(meta[2], meta[3], 0x5410), s_cd = __byte_perm(meta[2], meta[3], 0x7632);
@@ -426,14 +673,16 @@ __global__ void __launch_bounds__(KV4_DEC_THREADS, 2) kv4_decode_kernel(const Kv
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-              kv4_mma<T>(o[nt][i2 * 4 + k], a0[k], a1[k], a2[k], a3[k], pb[pg][nt][0], pb[pg][nt][1]);
+            for (int x = 0; x < 4; ++x)
+              kv4_mma<T>(o[nt][i2 * 4 + x], a0[x], a1[x], a2[x], a3[x], pb[pg][nt][0], pb[pg][nt][1], o[nt][i2 * 4 + x]);
         }
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&empty[s]);
     }
-    g0 += static_cast<uint32_t>(nslots);
+    g0 += static_cast<uint32_t>(max(0, pc.slots));
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&piece_empty[e]);  // descriptor and query rows are in registers
     // ---------------------------------------------------------------- merge the four warps of the unit
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
@@ -473,9 +722,8 @@ __global__ void __launch_bounds__(KV4_DEC_THREADS, 2) kv4_decode_kernel(const Kv
       for (int w = 0; w < 4; ++w)
 #pragma unroll
         for (int c = 0; c < D / 32; ++c) acc[c] = fmaf(sm_o[(w * ROWS + row) * D + c * 32 + lane], wgt[w], acc[c]);
-      const int tok = d.qstart + (row0 + row) / p.group, head = d.hk * p.group + (row0 + row) % p.group;
-      if (p.splits > 1) {
-        const size_t base = ((static_cast<size_t>(d.item) * p.hkv + d.hk) * p.splits + d.split) * 16 + row0 + row;
+      if (pc.part >= 0) {
+        const size_t base = static_cast<size_t>(pc.part) * 16 + row;
 #pragma unroll
         for (int c = 0; c < D / 32; ++c) p.part_o[base * D + c * 32 + lane] = acc[c];
         if (lane == 0) {
@@ -483,91 +731,109 @@ __global__ void __launch_bounds__(KV4_DEC_THREADS, 2) kv4_decode_kernel(const Kv
           p.part_ml[base * 2 + 1] = L;
         }
       } else {
-        const float inv = L == 0.f ? 0.f : 1.f / L;  // a row that sees nothing is 0; NaN stays NaN
-        T* dst = reinterpret_cast<T*>(p.out) + (static_cast<size_t>(tok) * p.hq + head) * D;
-#pragma unroll
-        for (int c = 0; c < D / 32; ++c) dst[c * 32 + lane] = Cvt<T>::from_f(acc[c] * inv);
-        if (p.lse && lane == 0)
-          p.lse[static_cast<size_t>(tok) * p.hq + head] = L == 0.f ? -INFINITY : (M + log2f(L)) * 0.6931471805599453f;
+        kv4_finish_row<T, D>(p, pc.qstart, pc.hk, pc.row0 + row, M, L, acc);
       }
     }
-    // the scratch area is rewritten by the next unit; after the barrier all four warps read the same abort flag,
-    // so they leave together if a wait of any of them ran out
+    // The scratch area is rewritten by the next unit. One thread samples the abort flag between the barriers, so that
+    // all four warps leave together if a wait of any role ran out.
+    if (threadIdx.x == 0) leave_word = *abort_flag;
     asm volatile("bar.sync 1, 128;" ::: "memory");
-    if (*abort_flag) break;
+    if (leave_word || pc.last) break;
   }
 }
 
-// Joins the splits of every (item, kv head): one warp per row.
+// Joins the pieces of the units that were cut: block c has the unit that began in CTA c's share, if any. Its first
+// piece is that CTA's last, the others are the first pieces of the CTAs after it.
 template <typename T, int D>
-__global__ void __launch_bounds__(128) kv4_decode_merge_kernel(const Kv4DecParams p) {
-  const int item = blockIdx.x, hk = blockIdx.y;
+__global__ void __launch_bounds__(128) kv4_decode_merge_kernel(const Kv4DecParams p, int rows_per_block) {
+  pdl_launch_dependents();
+  pdl_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int qstart = p.item_qstart[item], valid_rows = p.item_ntok[item] * p.group;
-  for (int row = warp; row < valid_rows; row += 4) {
-    const size_t first = (static_cast<size_t>(item) * p.hkv + hk) * p.splits * 16 + row;
+  const int4 pu = reinterpret_cast<const int4*>(p.part_unit)[blockIdx.x];
+  const int item = pu.x, pieces = pu.z;
+  if (item < 0) return;
+  const int hk = pu.y / p.row_blocks, row0 = pu.y % p.row_blocks * rows_per_block;
+  const int qstart = p.item_qstart[item];
+  const int rows = min(rows_per_block, p.item_ntok[item] * p.group - row0);
+  for (int row = warp; row < rows; row += 4) {
+    auto block = [&](int i) { return (i == 0 ? blockIdx.x * 2 + 1 : (blockIdx.x + i) * 2) * static_cast<size_t>(16) + row; };
     float M = -INFINITY;
-    for (int s = 0; s < p.splits; ++s) M = fmaxf(M, p.part_ml[(first + s * 16) * 2]);
+    for (int i = lane; i < pieces; i += 32) M = fmaxf(M, p.part_ml[block(i) * 2]);
+    M = warp_max(M);
     float L = 0.f, acc[D / 32];
 #pragma unroll
     for (int c = 0; c < D / 32; ++c) acc[c] = 0.f;
-    for (int s = 0; s < p.splits; ++s) {
-      const float ms = p.part_ml[(first + s * 16) * 2], ls = p.part_ml[(first + s * 16) * 2 + 1];
+    for (int i = 0; i < pieces; ++i) {
+      const size_t b = block(i);
+      const float ms = p.part_ml[b * 2], ls = p.part_ml[b * 2 + 1];
       const float w = ms == -INFINITY ? 0.f : exp2f(ms - M);
       L += ls != ls ? ls : ls * w;
 #pragma unroll
-      for (int c = 0; c < D / 32; ++c) acc[c] = fmaf(p.part_o[(first + s * 16) * D + c * 32 + lane], w, acc[c]);
+      for (int c = 0; c < D / 32; ++c) acc[c] = fmaf(p.part_o[b * D + c * 32 + lane], w, acc[c]);
     }
-    const int tok = qstart + row / p.group, head = hk * p.group + row % p.group;
-    const float inv = L == 0.f ? 0.f : 1.f / L;
-    T* dst = reinterpret_cast<T*>(p.out) + (static_cast<size_t>(tok) * p.hq + head) * D;
-#pragma unroll
-    for (int c = 0; c < D / 32; ++c) dst[c * 32 + lane] = Cvt<T>::from_f(acc[c] * inv);
-    if (p.lse && lane == 0)
-      p.lse[static_cast<size_t>(tok) * p.hq + head] = L == 0.f ? -INFINITY : (M + log2f(L)) * 0.6931471805599453f;
+    kv4_finish_row<T, D>(p, qstart, hk, row0 + row, M, L, acc);
   }
 }
 
 template <typename T, int D, int NT, bool EXT>
-int kv4_decode_launch(const Kv4DecParams& p, int num_items, cudaStream_t stream) {
+int kv4_decode_launch(Kv4DecParams p, int num_items, int max_ctas, cudaStream_t stream) {
   using Shape = Kv4DecShape<D, NT>;
   auto kern = kv4_decode_kernel<T, D, NT, EXT>;
+  const int batch = num_items < KV4_DEC_ITEMS ? num_items : KV4_DEC_ITEMS;
+  const int most = Shape::OFF_SCAN + (KV4_DEC_ITEMS + 1) * 4;
   static int per_sm[64] = {};
   int dev = 0;
   cudaError_t err = cudaGetDevice(&dev);
   if (err != cudaSuccess) return static_cast<int>(err);
   dev &= 63;
   if (!per_sm[dev]) {
-    err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::SMEM);
+    err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
     if (err != cudaSuccess) return static_cast<int>(err);
     int n = 0;
-    err = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, KV4_DEC_THREADS, Shape::SMEM);
+    err = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, KV4_DEC_THREADS, most);
     if (err != cudaSuccess) return static_cast<int>(err);
     per_sm[dev] = n > 0 ? n : 1;
   }
-  const int most = per_sm[dev] * sm_count();
-  kern<<<p.num_units < most ? p.num_units : most, KV4_DEC_THREADS, Shape::SMEM, stream>>>(p);
-  count_launch();
-  if (p.splits > 1) {
-    kv4_decode_merge_kernel<T, D><<<dim3(num_items, p.hkv), 128, 0, stream>>>(p);
+  int ctas = per_sm[dev] * sm_count();
+  if (ctas > max_ctas) ctas = max_ctas;
+  for (int first = 0; first < num_items; first += batch) {
+    Kv4DecParams part = p;
+    part.item_seq += first;
+    part.item_qstart += first;
+    part.item_ntok += first;
+    part.num_items = num_items - first < batch ? num_items - first : batch;
+    kern<<<ctas, KV4_DEC_THREADS, Shape::OFF_SCAN + (part.num_items + 1) * 4, stream>>>(part);
+    count_launch();
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(ctas);
+    cfg.blockDim = dim3(128);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    err = cudaLaunchKernelEx(&cfg, kv4_decode_merge_kernel<T, D>, part, Shape::ROWS);
+    if (err != cudaSuccess) return static_cast<int>(err);
     count_launch();
   }
   return static_cast<int>(cudaGetLastError());
 }
 
 template <typename T, int D>
-int kv4_decode_shape(Kv4DecParams& p, int rows, bool ext, int num_items, cudaStream_t stream) {
-  // Up to 8 query rows need one n-tile. 9 to 16 rows take two, which share the expanded K and V; at D = 256 the
+int kv4_decode_shape(Kv4DecParams& p, int rows, bool ext, int num_items, int max_ctas, cudaStream_t stream) {
+  // Up to 8 query rows need one n-tile. 9 to 16 rows take two, which share the expanded V; at D = 256 the
   // accumulators of two would not fit the register file, and two units read the same pages instead.
-  if (D < 256 && rows > 8) {
-    p.row_blocks = 1;
-    p.num_units = num_items * p.hkv * p.splits;
-    return ext ? kv4_decode_launch<T, D, (D < 256 ? 2 : 1), true>(p, num_items, stream)
-               : kv4_decode_launch<T, D, (D < 256 ? 2 : 1), false>(p, num_items, stream);
+  if constexpr (D < 256) {
+    if (rows > 8) {
+      p.row_blocks = 1;
+      return ext ? kv4_decode_launch<T, D, 2, true>(p, num_items, max_ctas, stream)
+                 : kv4_decode_launch<T, D, 2, false>(p, num_items, max_ctas, stream);
+    }
   }
   p.row_blocks = (rows + 7) / 8;
-  p.num_units = num_items * p.hkv * p.splits * p.row_blocks;
-  return ext ? kv4_decode_launch<T, D, 1, true>(p, num_items, stream) : kv4_decode_launch<T, D, 1, false>(p, num_items, stream);
+  return ext ? kv4_decode_launch<T, D, 1, true>(p, num_items, max_ctas, stream)
+             : kv4_decode_launch<T, D, 1, false>(p, num_items, max_ctas, stream);
 }
 
 }  // namespace mlcb
@@ -575,21 +841,22 @@ int kv4_decode_shape(Kv4DecParams& p, int rows, bool ext, int num_items, cudaStr
 using namespace mlcb;
 
 // One layer's cache [num_pages, 2, hkv, 16, row]. Items are (sequence, query-token range) pairs of at most `rows`
-// <= 16 query rows (tokens * hq / hkv) each. splits > 1 needs fp32 scratch part_o [items, hkv, splits, 16, d] and
-// part_ml [.., 16, 2]. Returns -1 shape, -2 alignment, -3 type, -4 missing scratch, -5 too many units.
+// <= 16 query rows (tokens * hq / hkv) each. Scratch for max_ctas CTAs: part_o [2 max_ctas, 16, d] and part_ml
+// [2 max_ctas, 16, 2] fp32, part_unit [max_ctas, 4] int32; it is written before it is read. Returns -1 shape,
+// -2 alignment, -3 type, -4 missing scratch.
 MLCB_API int mlcb_kv4_decode(const void* q, const void* pages, void* out, float* lse, const int* item_seq,
                              const int* item_qstart, const int* item_ntok, const int* q_kvlen, const int* page_indptr,
                              const int* page_indices, int num_items, int rows, long long q_stride, int hq, int hkv, int d,
-                             long long num_pages, float sm_scale, int dtype, int splits, float* part_o, float* part_ml,
-                             int* status, cudaStream_t stream, const int* q_kvstart, const unsigned long long* tree_mask,
-                             int sink, float softcap) {
+                             long long num_pages, float sm_scale, int dtype, int max_ctas, float* part_o, float* part_ml,
+                             int* part_unit, int* status, cudaStream_t stream, const int* q_kvstart,
+                             const unsigned long long* tree_mask, int sink, float softcap) {
   if (num_items <= 0) return 0;
   if (hkv <= 0 || hq <= 0 || hq % hkv || rows < 1 || rows > 16 || (d != 64 && d != 128 && d != 256)) return -1;
-  if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(pages)) & 15) return -2;
+  if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(pages) | reinterpret_cast<uintptr_t>(part_unit)) & 15)
+    return -2;
   if (q_stride % 8) return -2;
   if (dtype != 0 && dtype != 1) return -3;
-  if (splits < 1 || (splits > 1 && (!part_o || !part_ml))) return -4;
-  if (static_cast<long long>(num_items) * hkv * splits * 2 > 0x7fffffffLL || hkv > 65535) return -5;
+  if (max_ctas < 1 || !part_o || !part_ml || !part_unit) return -4;
   Kv4DecParams p;
   p.q = q;
   p.pages = static_cast<const uint8_t*>(pages);
@@ -597,6 +864,7 @@ MLCB_API int mlcb_kv4_decode(const void* q, const void* pages, void* out, float*
   p.lse = lse;
   p.part_o = part_o;
   p.part_ml = part_ml;
+  p.part_unit = part_unit;
   p.item_seq = item_seq;
   p.item_qstart = item_qstart;
   p.item_ntok = item_ntok;
@@ -611,18 +879,20 @@ MLCB_API int mlcb_kv4_decode(const void* q, const void* pages, void* out, float*
   p.hq = hq;
   p.hkv = hkv;
   p.group = hq / hkv;
-  p.splits = splits;
+  p.row_blocks = 1;
+  p.num_items = num_items;
   p.sink = q_kvstart ? sink : 0;
-  p.scale_log2 = sm_scale * 1.4426950408889634f;
-  p.cap_k = softcap > 0.f ? 2.f * 1.4426950408889634f * sm_scale / softcap : 0.f;
+  p.q_flip = sm_scale < 0.f ? 0x80008000u : 0u;
+  p.scale_log2 = fmaxf(fabsf(sm_scale) * 1.4426950408889634f, 1e-30f);  // a hidden score is -inf * scale: not 0
+  p.cap_k = softcap > 0.f ? 2.f * 1.4426950408889634f * fabsf(sm_scale) / softcap : 0.f;
   p.cap_log2 = softcap > 0.f ? softcap * 1.4426950408889634f : 0.f;
   const bool ext = q_kvstart || tree_mask || softcap > 0.f;
   if (dtype == 0) {
-    if (d == 64) return kv4_decode_shape<__half, 64>(p, rows, ext, num_items, stream);
-    if (d == 128) return kv4_decode_shape<__half, 128>(p, rows, ext, num_items, stream);
-    return kv4_decode_shape<__half, 256>(p, rows, ext, num_items, stream);
+    if (d == 64) return kv4_decode_shape<__half, 64>(p, rows, ext, num_items, max_ctas, stream);
+    if (d == 128) return kv4_decode_shape<__half, 128>(p, rows, ext, num_items, max_ctas, stream);
+    return kv4_decode_shape<__half, 256>(p, rows, ext, num_items, max_ctas, stream);
   }
-  if (d == 64) return kv4_decode_shape<__nv_bfloat16, 64>(p, rows, ext, num_items, stream);
-  if (d == 128) return kv4_decode_shape<__nv_bfloat16, 128>(p, rows, ext, num_items, stream);
-  return kv4_decode_shape<__nv_bfloat16, 256>(p, rows, ext, num_items, stream);
+  if (d == 64) return kv4_decode_shape<__nv_bfloat16, 64>(p, rows, ext, num_items, max_ctas, stream);
+  if (d == 128) return kv4_decode_shape<__nv_bfloat16, 128>(p, rows, ext, num_items, max_ctas, stream);
+  return kv4_decode_shape<__nv_bfloat16, 256>(p, rows, ext, num_items, max_ctas, stream);
 }

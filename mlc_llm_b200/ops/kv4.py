@@ -138,12 +138,10 @@ def kv4_plan(q_indptr, q_kvlen: torch.Tensor, page_indptr: torch.Tensor, page_in
                          dec_rows=int(tiles["dec_ntok"].max()) * (hq // hkv) if num_dec else 16)
 
 
-def _splits(units: int, max_pages: int, device: torch.device) -> int:
-    """KV splits of the decode kernel: enough units for three persistent CTAs per SM, at least 8 pages each."""
-    target = 3 * sm_count(device)
-    if units >= target or max_pages < 16:
-        return 1
-    return int(max(1, min(32, target // max(1, units), max_pages // 8)))
+def _decode_ctas(num_items: int, rows: int, hkv: int, max_pages: int, device: torch.device) -> int:
+    """CTAs of the decode kernel: as many as stay resident, but no more than one per four 32-token slots."""
+    slots = num_items * hkv * ((rows + 7) // 8) * max(1, (max_pages + 1) // 2)
+    return max(1, min(4 * sm_count(device), (slots + 3) // 4))
 
 
 def attend(q: torch.Tensor, kv_pages: torch.Tensor, q_seq: torch.Tensor, q_kvlen: torch.Tensor, page_indptr: torch.Tensor,
@@ -187,16 +185,14 @@ def _launch(q, kv_pages, out, lse, q_seq, q_kvlen, page_indptr, page_indices, hq
         if plan.num_dec:
             # with one token per item the rows are the group's heads, whatever the plan was made for
             rows = group if t == plan.num_dec else min(16, plan.dec_rows)
-            splits = _splits(plan.num_dec * hkv, plan.max_pages, q.device)
-            part_o = part_ml = None
-            if splits > 1:
-                part_o = torch.empty(plan.num_dec * hkv * splits * 16 * d, dtype=torch.float32, device=q.device)
-                part_ml = torch.empty(plan.num_dec * hkv * splits * 16 * 2, dtype=torch.float32, device=q.device)
+            ctas = _decode_ctas(plan.num_dec, rows, hkv, plan.max_pages, q.device)
+            part = torch.empty(ctas * (2 * 16 * (d + 2) + 4), dtype=torch.float32, device=q.device)
+            part_unit, part_ml, part_o = part[: 4 * ctas], part[4 * ctas: 68 * ctas], part[68 * ctas:]
             rc = lib().mlcb_kv4_decode(ptr(q), ptr(kv_pages), ptr(out), ptr(lse), ptr(plan.dec_seq), ptr(plan.dec_qstart),
                                        ptr(plan.dec_ntok), ptr(q_kvlen), ptr(page_indptr), ptr(page_indices),
                                        c_int(plan.num_dec), c_int(rows), c_ll(q.stride(0)), c_int(hq), c_int(hkv), c_int(d),
-                                       c_ll(kv_pages.shape[0]), c_float(sm_scale), dtype, c_int(splits), ptr(part_o),
-                                       ptr(part_ml), status, stream_ptr(), ptr(q_kvstart), ptr(tree_mask), c_int(sink),
+                                       c_ll(kv_pages.shape[0]), c_float(sm_scale), dtype, c_int(ctas), ptr(part_o),
+                                       ptr(part_ml), ptr(part_unit), status, stream_ptr(), ptr(q_kvstart), ptr(tree_mask), c_int(sink),
                                        c_float(softcap))
             check(rc, "mlcb_kv4_decode")
         return

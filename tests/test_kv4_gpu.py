@@ -120,7 +120,7 @@ class Step:
     last pages behind the sequence, pages of nobody) holds NaN."""
 
     def __init__(self, dtype, lens, new, hq, hkv, d, page=16, window=0, sink=0, cap=0.0, tree=False, seed=0,
-                 first_page=0, kvlen=None):
+                 first_page=0, kvlen=None, q_by=1.0, k_by=1.0):
         g = torch.Generator().manual_seed(seed)
         self.hq, self.hkv, self.d, self.page, self.sink, self.cap, self.dtype = hq, hkv, d, page, sink, cap, dtype
         held = [(n + page - 1) // page for n in lens]
@@ -130,6 +130,7 @@ class Step:
         slots = torch.tensor([int(perm[indptr[i] + j // page]) * page + j % page for i, n in enumerate(lens) for j in range(n)],
                              dtype=torch.int64)
         kv = _kv(g, len(slots), hkv, d, dtype)
+        kv[:, : hkv * d] *= k_by
         self.cache = torch.full((pages + first_page, 2, hkv, page, ops.kv4_row(d, dtype)), math.nan, dtype=dtype, device=DEV)
         if len(slots):
             at = (slots + first_page * page).to(torch.int32).to(DEV)
@@ -138,7 +139,7 @@ class Step:
         cut = np.concatenate([[0], np.cumsum(lens)])
         self.vals = [vals[cut[i]:cut[i + 1]] for i in range(len(lens))]
         t = sum(new)
-        qkv = torch.randn(t, (hq + 2 * hkv) * d, generator=g).to(dtype)
+        qkv = (torch.randn(t, (hq + 2 * hkv) * d, generator=g) * q_by).to(dtype)
         self.qkv = qkv.to(DEV)
         self.q = self.qkv[:, : hq * d]
         self.q_indptr = np.concatenate([[0], np.cumsum(new)]).astype(np.int64)
@@ -231,6 +232,8 @@ DECODE = [
     ([1000, 20, 129], [2, 1, 3], 8, 2, 64, {"window": 100, "sink": 20}),
     ([1000, 77], [1, 1], 8, 4, 256, {"window": 500, "cap": 50.0}),
     ([400, 77], [1, 1], 32, 8, 128, {"cap": 30.0}),
+    ([300, 77], [1, 2], 8, 2, 128, {"q_by": 3000.0, "k_by": 2.0 ** -11}),  # sums of q beyond fp16
+    ([300, 77], [1, 2], 8, 2, 128, {"q_by": 1e-3, "k_by": 500.0}),
     ([2000] * 40, [1] * 40, 32, 8, 128, {}),                       # more units than CTAs
 ]
 
