@@ -16,6 +16,7 @@
 namespace mlcb {
 
 constexpr int KV4_GROUP = 32;
+constexpr int KV4_PAGE = 16;  // tokens per page of the tensor-core kernels
 __host__ __device__ constexpr int kv4_row_bytes(int d) { return d / 2 + d / KV4_GROUP * 4; }
 
 // (w & mask) | bits in one instruction.
@@ -31,7 +32,7 @@ template <typename T>
 struct Kv4Type;
 template <>
 struct Kv4Type<__half> {
-  using Pair = __half2;
+  static constexpr bool IS_BF16 = false;
   static constexpr float BOUND = 65440.f;
   // out[i] = pair of s * c_i + lo for the nibbles at bits 4 i of both halves. A nibble under the exponent of
   // 1024 (bits 0-3) or of 64 (bits 4-7) is the exact number 1024 + c or 64 + c: no int-to-float conversion, one
@@ -56,7 +57,7 @@ struct Kv4Type<__half> {
 };
 template <>
 struct Kv4Type<__nv_bfloat16> {
-  using Pair = __nv_bfloat162;
+  static constexpr bool IS_BF16 = true;
   static constexpr float BOUND = 8.507059173023461586e37f;  // 2^126
   // as above; bf16 has 7 mantissa bits, so only the nibble at bits 0-3 fits (under the exponent of 128)
   static __device__ __forceinline__ void expand4(uint32_t w, uint32_t s2, uint32_t lo2, uint32_t (&out)[4]) {
@@ -85,6 +86,52 @@ __device__ __forceinline__ int kv4_code(uint32_t w, int ch) { return (w >> ((ch 
 // tanh approximation is off by 5e-4 of the value. `k` = 2 log2(e) * scale / cap. (e^2y = inf gives cap; NaN stays.)
 __device__ __forceinline__ float kv4_softcap(float raw, float k, float cap) {
   return cap - __fdividef(2.f * cap, 1.f + exp2f(raw * k));
+}
+
+// Visibility of position `pos` to a query token (the rule of the 16-bit kernels): below kvlen all positions from
+// `start` on and the first `sink`; from kvlen on the set bits of the tree mask.
+__device__ __forceinline__ bool kv4_visible(int pos, int kvlen, int start, int sink, unsigned long long tm) {
+  if (pos < kvlen) return pos >= start || pos < sink;
+  const int r = pos - kvlen;
+  return r < 64 && ((tm >> r) & 1ull);
+}
+
+// (a.x, a.y) * (b.x, b.y) + (c.x, c.y), and a sum of pairs, in one instruction each.
+__device__ __forceinline__ float2 kv4_fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("fma.rn.ftz.f32x2 %0, %1, %2, %3;"
+      : "=l"(reinterpret_cast<unsigned long long&>(d))
+      : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)),
+        "l"(reinterpret_cast<unsigned long long&>(c)));
+  return d;
+}
+__device__ __forceinline__ float2 kv4_add2(float2 a, float2 b) {
+  float2 d;
+  asm("add.rn.ftz.f32x2 %0, %1, %2;"
+      : "=l"(reinterpret_cast<unsigned long long&>(d))
+      : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)));
+  return d;
+}
+
+// N words from shared memory (the address is aligned to 16, 8 or 4 bytes for N = 4, 2, 1).
+template <int N>
+__device__ __forceinline__ void kv4_words(const uint8_t* p, uint32_t (&w)[N]) {
+  if constexpr (N % 4 == 0) {
+#pragma unroll
+    for (int i = 0; i < N / 4; ++i) {
+      const uint4 v = reinterpret_cast<const uint4*>(p)[i];
+      w[4 * i] = v.x;
+      w[4 * i + 1] = v.y;
+      w[4 * i + 2] = v.z;
+      w[4 * i + 3] = v.w;
+    }
+  } else if constexpr (N == 2) {
+    const uint2 v = *reinterpret_cast<const uint2*>(p);
+    w[0] = v.x;
+    w[1] = v.y;
+  } else {
+    w[0] = *reinterpret_cast<const uint32_t*>(p);
+  }
 }
 
 }  // namespace mlcb

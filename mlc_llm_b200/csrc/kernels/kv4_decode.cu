@@ -32,7 +32,6 @@
 
 namespace mlcb {
 
-constexpr int KV4_PAGE = 16;
 constexpr int KV4_DEC_THREADS = 160;
 
 
@@ -57,14 +56,6 @@ struct Kv4DecParams {
   float scale_log2;          // sm_scale * log2(e)
   float cap_k, cap_log2;     // soft cap: scores are kv4_softcap(raw, cap_k, cap_log2); 0 = none
 };
-
-// Visibility of position `pos` to a query token (the rule of the 16-bit kernels): below kvlen all positions from
-// `start` on and the first `sink`; from kvlen on the set bits of the tree mask.
-__device__ __forceinline__ bool kv4_visible(int pos, int kvlen, int start, int sink, unsigned long long tm) {
-  if (pos < kvlen) return pos >= start || pos < sink;
-  const int r = pos - kvlen;
-  return r < 64 && ((tm >> r) & 1ull);
-}
 
 // What one item visits: pages [0, npg) of its list, less those that lie outside every row's window.
 struct Kv4Item {
@@ -102,7 +93,7 @@ __device__ __forceinline__ Kv4Item kv4_item(const Kv4DecParams& p, int item) {
   d.skip = 0;
   if (EXT && p.q_kvstart) {
     d.sink_pg = (p.sink + KV4_PAGE - 1) / KV4_PAGE;
-    d.skip = max(0, first / KV4_PAGE - d.sink_pg);
+    d.skip = max(0, min(first, reach) / KV4_PAGE - d.sink_pg);
   }
   const int p0 = p.page_indptr[b];
   const int held = p.page_indptr[b + 1] - p0;
@@ -190,44 +181,6 @@ __device__ __forceinline__ float kv4_step<__half>(uint32_t meta) {
 template <>
 __device__ __forceinline__ float kv4_step<__nv_bfloat16>(uint32_t meta) {
   return __uint_as_float(meta & 0xffff0000u);
-}
-
-// (a.x, a.y) * (b.x, b.y) + (c.x, c.y), and a sum of pairs, in one instruction each.
-__device__ __forceinline__ float2 kv4_fma2(float2 a, float2 b, float2 c) {
-  float2 d;
-  asm("fma.rn.ftz.f32x2 %0, %1, %2, %3;"
-      : "=l"(reinterpret_cast<unsigned long long&>(d))
-      : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)),
-        "l"(reinterpret_cast<unsigned long long&>(c)));
-  return d;
-}
-__device__ __forceinline__ float2 kv4_add2(float2 a, float2 b) {
-  float2 d;
-  asm("add.rn.ftz.f32x2 %0, %1, %2;"
-      : "=l"(reinterpret_cast<unsigned long long&>(d))
-      : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)));
-  return d;
-}
-
-// N words from shared memory (the address is aligned to 16, 8 or 4 bytes for N = 4, 2, 1).
-template <int N>
-__device__ __forceinline__ void kv4_words(const uint8_t* p, uint32_t (&w)[N]) {
-  if constexpr (N % 4 == 0) {
-#pragma unroll
-    for (int i = 0; i < N / 4; ++i) {
-      const uint4 v = reinterpret_cast<const uint4*>(p)[i];
-      w[4 * i] = v.x;
-      w[4 * i + 1] = v.y;
-      w[4 * i + 2] = v.z;
-      w[4 * i + 3] = v.w;
-    }
-  } else if constexpr (N == 2) {
-    const uint2 v = *reinterpret_cast<const uint2*>(p);
-    w[0] = v.x;
-    w[1] = v.y;
-  } else {
-    w[0] = *reinterpret_cast<const uint32_t*>(p);
-  }
 }
 
 // Row `row` (of the item's rows) of the output: acc[c] = channel 32 c + lane, scaled by 1 / L. A row that sees nothing
@@ -444,14 +397,14 @@ __global__ void __launch_bounds__(KV4_DEC_THREADS, Kv4DecShape<D, NT>::CTAS) kv4
         qb[nt][grp][1] = v.y ^ p.q_flip;
         qb[nt][grp][2] = v.z ^ p.q_flip;
         qb[nt][grp][3] = v.w ^ p.q_flip;
-        if constexpr (Kv4Bias<T>::TERMS == 2) {
+        if constexpr (!Kv4Type<T>::IS_BF16) {
           const uint32_t mag = 0x7fff7fffu;
           top_bits = __vmaxu2(top_bits, __vmaxu2(__vmaxu2(v.x & mag, v.y & mag), __vmaxu2(v.z & mag, v.w & mag)));
         }
       }
     }
     float unit_scale = 1.f;
-    if constexpr (Kv4Bias<T>::TERMS == 2) {
+    if constexpr (!Kv4Type<T>::IS_BF16) {
       // fp16: the largest magnitude's exponent field is 20 for 32 <= |q| < 64; below 32, 64 sum|q| stays finite
       const uint32_t all = __reduce_max_sync(0xffffffffu, max(top_bits & 0xffffu, top_bits >> 16));
       const int over = static_cast<int>(all >> 10) - 19;

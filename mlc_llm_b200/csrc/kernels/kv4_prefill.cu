@@ -1,0 +1,675 @@
+// Prefill attention over the 4-bit paged KV cache (format: kv4.cuh) on the 5th-gen tensor cores: head sizes 64, 96,
+// 128 and 256, 16-token pages, any mask of the 16-bit kernels.
+//
+// A CTA owns up to 256 query rows of one kv head -- (token, q head) pairs, the G = hq / hkv heads of the group side
+// by side -- as two accumulator tiles of 128 rows, and walks the cached positions in blocks of 128:
+//
+//   raw       a warp copies the blocks' packed rows (80 bytes per token at D = 128) into a ring of shared memory
+//   expand    four warps turn them into 16-bit K and V tiles in the layout the tensor core reads (128-byte
+//             swizzle; V MN-major), lo + s c rounded once. One expansion feeds both query tiles: at 600 issue
+//             slots per scheduler and block it hides under the 2048 clocks of the block's products.
+//   S = Q K^T    tcgen05.mma, both operands in shared memory, D in TMEM (128 columns per tile)
+//   softmax      one thread per row, 32 columns of TMEM at a time. Weights are taken against the running reference
+//                maximum of the blocks before; only if a score exceeds it by more than 8 (log2) is the block redone
+//                with a raised one and O rescaled. P (16 bits) overwrites S in TMEM.
+//   O += P V     tcgen05.mma, A = P in TMEM, B = V in shared memory, D accumulates in TMEM for the whole loop
+//
+// While the softmax of one tile runs, the tensor core works on the other tile. With D = 256 one tile fills TMEM (O
+// takes 256 columns): blocks are 64 positions, S has two buffers, and the scores of block j + 1 are computed before
+// the softmax of block j ends.
+//
+// Few long rows (a short chunk behind a long prefix) are split over the cached positions; fp32 partial rows are
+// joined by a second kernel. Bounds: the tensor core (4 D flops per query row and position), then the exponentials
+// (one per row and position; 16 per clock and SM against 8 K flops per clock).
+//
+// Roles: 4 warps per query tile (softmax, epilogue), 4 expanding warps, 1 copying warp, 1 issuing warp. Every wait is
+// bounded (common.cuh).
+#include "kv4.cuh"
+
+namespace mlcb {
+
+struct Kv4PreParams {
+  const void* q;
+  const uint8_t* pages;
+  void* out;
+  float* lse;
+  float* part_o;   // [tiles, hkv, splits, rows, D] fp32 (splits > 1)
+  float* part_ml;  // [tiles, hkv, splits, rows, 2]
+  const int *tile_seq, *tile_qstart, *tile_ntok, *q_kvlen, *page_indptr, *page_indices;
+  const int* q_kvstart;
+  const unsigned long long* tree_mask;
+  int* status;
+  long long q_stride, num_pages;
+  int hq, hkv, group, sink, splits, num_tiles;
+  int parts;               // CTAs per tile: 2 where a tile has more than the 128 rows of a D = 256 CTA
+  uint32_t q_flip;         // sign bits of a pair where sm_scale is negative: scale_log2 is its magnitude
+  float scale_log2;        // sm_scale * log2(e)
+  float cap_k, cap_log2;   // soft cap: scores are kv4_softcap(raw, cap_k, cap_log2); 0 = none
+};
+
+template <int D>
+struct Kv4PreShape {
+  static constexpr int SUB = D == 256 ? 1 : 2;           // query tiles of 128 rows
+  static constexpr int BLK = D == 256 ? 64 : 128;        // cached positions per block
+  static constexpr int HALVES = (D + 63) / 64;           // 64-channel atoms of a row
+  static constexpr int ROW = kv4_row_bytes(D);
+  static constexpr int PAGE_BYTES = KV4_PAGE * ROW;
+  static constexpr int TILE_BYTES = BLK * HALVES * 128;  // one expanded K or V tile
+  static constexpr int TILES = 4;                        // K, V, K, V
+  static constexpr int Q_BYTES = 128 * HALVES * 128;     // one query tile
+  static constexpr int RAW_TOKENS = 64;                  // a raw slot: packed K or V rows of 64 positions
+  static constexpr int RAW_BYTES = RAW_TOKENS * ROW;
+  static constexpr int RAW_PER_TILE = BLK / RAW_TOKENS;
+  static constexpr int RAW_SLOTS = D == 256 ? 3 : 6;
+  static constexpr int OFF_TILE = SUB * Q_BYTES;
+  static constexpr int OFF_RAW = OFF_TILE + TILES * TILE_BYTES;
+  static constexpr int SMEM = OFF_RAW + RAW_SLOTS * RAW_BYTES + 1024;
+  static constexpr int THREADS = SUB * 128 + 128 + 64;
+  static constexpr int O_COL = SUB == 2 ? 256 : 128;     // TMEM: S tiles first, then O
+  static constexpr int O_STEP = 128;
+};
+
+// D[tmem] (+)= A[tmem] * B[smem]; 16-bit inputs, fp32 accumulate. A holds two K-adjacent values per 32-bit column.
+__device__ __forceinline__ void kv4_umma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc,
+                                            uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+__device__ __forceinline__ void kv4_tmem_st32(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+      "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]),
+      "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]),
+      "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+__device__ __forceinline__ void kv4_tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// What a CTA needs to know of its tile, found by all threads together.
+struct Kv4Tile {
+  int reach[2];     // per query tile: positions any of its rows sees end here
+  int all_to[2];    // per query tile: every row sees [all_from, all_to)
+  int all_from[2];
+  int first;        // no row sees a position in [sink, first)
+};
+
+template <typename T, int D, bool EXT>
+__global__ void __launch_bounds__(Kv4PreShape<D>::THREADS, 1) kv4_prefill_kernel(const Kv4PreParams p) {
+  using Shape = Kv4PreShape<D>;
+  constexpr int SUB = Shape::SUB, BLK = Shape::BLK, ROW = Shape::ROW;
+  constexpr int GROUPS = D / KV4_GROUP;
+  pdl_launch_dependents();
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  __shared__ uint64_t bars[2 * Shape::RAW_SLOTS + 2 * Shape::TILES + 8];
+  __shared__ uint32_t tmem_slot;
+  __shared__ int abort_word;
+  __shared__ Kv4Tile info;
+  uint64_t* raw_full = bars;
+  uint64_t* raw_empty = raw_full + Shape::RAW_SLOTS;
+  uint64_t* tile_full = raw_empty + Shape::RAW_SLOTS;
+  uint64_t* tile_empty = tile_full + Shape::TILES;
+  // per query tile; with D = 256 per S buffer, because a fast warp may finish block j + 1 before a slow one block j
+  uint64_t* s_full = tile_empty + Shape::TILES;  // [2]
+  uint64_t* p_full = s_full + 2;                 // [2]
+  uint64_t* o_done = p_full + 2;                 // [SUB]
+  uint64_t* pv_done = o_done + 2;                // D = 256 only
+  uint64_t* q_ready = pv_done + 1;
+  volatile int* abort_flag = &abort_word;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int G = p.group;
+  // long tiles first: the last tiles of a sequence see the most positions
+  const int split = blockIdx.x % p.splits;
+  const int work = p.num_tiles * p.parts - 1 - static_cast<int>(blockIdx.x) / p.splits, hk = blockIdx.y;
+  const int tile = work / p.parts, row0 = work % p.parts * 128;  // first row of the tile that is this CTA's
+  const int seq = p.tile_seq[tile], qstart = p.tile_qstart[tile], ntok = p.tile_ntok[tile];
+  const int valid_rows = max(0, min(ntok * G - row0, SUB * 128));
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < Shape::RAW_SLOTS; ++i) {
+      mbar_init(&raw_full[i], 1);
+      mbar_init(&raw_empty[i], 4);
+    }
+    for (int i = 0; i < Shape::TILES; ++i) {
+      mbar_init(&tile_full[i], 4);
+      mbar_init(&tile_empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], 4);
+      mbar_init(&o_done[i], 1);
+    }
+    mbar_init(pv_done, 1);
+    mbar_init(q_ready, 4 * SUB);
+    abort_word = 0;
+    mbar_fence_init();
+    for (int i = 0; i < 2; ++i) {
+      info.reach[i] = 0;
+      info.all_to[i] = 0x7fffffff;
+      info.all_from[i] = 0;
+    }
+    info.first = 0x7fffffff;
+  }
+  constexpr int ISSUER = SUB * 4 + 5, COPIER = SUB * 4 + 4;
+  if (warp == ISSUER) {
+    tmem_alloc(&tmem_slot, 512);
+    tmem_relinquish();
+  }
+  __syncthreads();
+  for (int i = row0 / G + threadIdx.x; i * G < row0 + valid_rows; i += Shape::THREADS) {
+    const int n = p.q_kvlen[qstart + i];
+    int end = n, from = 0;
+    if (EXT && p.tree_mask) {
+      const unsigned long long tm = p.tree_mask[qstart + i];
+      if (tm) end += 64 - __clzll(tm);
+    }
+    if (EXT && p.q_kvstart) from = p.q_kvstart[qstart + i];
+#pragma unroll
+    for (int s = 0; s < SUB; ++s)
+      if (i * G < row0 + (s + 1) * 128 && (i + 1) * G > row0 + s * 128) {  // a token's heads may straddle the two tiles
+        atomicMax(&info.reach[s], end);
+        atomicMin(&info.all_to[s], n);
+        atomicMax(&info.all_from[s], from);
+      }
+    atomicMin(&info.first, from);
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_slot;
+  const int p0 = p.page_indptr[seq];
+  const int held = p.page_indptr[seq + 1] - p0;
+  const int* list = p.page_indices + p0;
+  const long long room = static_cast<long long>(held) * KV4_PAGE;
+  if (threadIdx.x == 0 && p.status && max(info.reach[0], info.reach[1]) > room) atomicCAS(p.status, 0, ERR_BAD_INDEX);
+  // Blocks a tile visits: all up to its reach, less the run of whole blocks between the sink and the first position
+  // that any row sees; of those, this split's share.
+  int sink_blks = 0, skip = 0, most = 0, nblk[2] = {0, 0};
+  {
+    int low = 0x7fffffff;
+#pragma unroll
+    for (int s = 0; s < SUB; ++s) {
+      nblk[s] = static_cast<int>((min(static_cast<long long>(info.reach[s]), room) + BLK - 1) / BLK);
+      if (s * 128 < valid_rows) low = min(low, info.reach[s]);
+    }
+    if (EXT && p.q_kvstart) {
+      sink_blks = (p.sink + BLK - 1) / BLK;
+      skip = max(0, min(info.first, low) / BLK - sink_blks);
+    }
+#pragma unroll
+    for (int s = 0; s < SUB; ++s) {
+      nblk[s] = max(0, nblk[s] - skip);
+      most = max(most, nblk[s]);
+    }
+  }
+  const int per = (most + p.splits - 1) / p.splits, j0 = split * per;
+#pragma unroll
+  for (int s = 0; s < SUB; ++s) nblk[s] = max(0, min(nblk[s] - j0, per));
+  const int nmax = SUB == 2 ? max(nblk[0], nblk[1]) : nblk[0];
+  auto base_of = [&](int j) { return (!EXT || j0 + j < sink_blks ? j0 + j : j0 + j + skip) * BLK; };
+
+  if (warp == COPIER) {
+    // ---------------------------------------------------------------- packed rows -> raw ring
+    bool ok = true;
+    int m = 0;  // raw slots so far
+    for (int j = 0; j < nmax && ok; ++j) {
+      const int pg0 = base_of(j) / KV4_PAGE;
+      int mine = 0;  // lane i: page number of the block's page i
+      if (lane < BLK / KV4_PAGE && pg0 + lane < held) {
+        mine = list[pg0 + lane];
+        if (mine >= p.num_pages) {
+          if (p.status) atomicCAS(p.status, 0, ERR_BAD_INDEX);
+          mine = 0;
+        }
+        if (mine < 0) mine = 0;  // released by a sliding window: every position of it is masked
+      }
+      for (int n = 0; n < 2 * Shape::RAW_PER_TILE && ok; ++n, ++m) {
+        const int kv = n / Shape::RAW_PER_TILE, part = n % Shape::RAW_PER_TILE;
+        const int s = m % Shape::RAW_SLOTS;
+        if (m >= Shape::RAW_SLOTS) {
+          ok = mbar_wait(&raw_empty[s], ((m / Shape::RAW_SLOTS) & 1) ^ 1, abort_flag, p.status, ERR_WAIT_PRODUCER);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+        }
+        const int first = part * 4, here = max(0, min(4, held - pg0 - first));  // pages of this slot that exist
+        if (lane == 0) mbar_expect_tx(&raw_full[s], here * Shape::PAGE_BYTES);
+        __syncwarp();
+        const int pg = __shfl_sync(0xffffffffu, mine, first + (lane & 3));
+        if (lane < here) {
+          const size_t block = (static_cast<size_t>(pg) * 2 + kv) * p.hkv + hk;
+          bulk_load(smem + Shape::OFF_RAW + s * Shape::RAW_BYTES + lane * Shape::PAGE_BYTES,
+                    p.pages + block * Shape::PAGE_BYTES, Shape::PAGE_BYTES, &raw_full[s]);
+        }
+      }
+    }
+  } else if (warp == ISSUER) {
+    // ---------------------------------------------------------------- tensor core
+    if (lane == 0 && nmax > 0) {
+      const uint32_t idesc_qk = umma_idesc(Kv4Type<T>::IS_BF16 ? 1 : 0, 128, BLK, 0, 0);
+      const uint32_t idesc_pv = umma_idesc(Kv4Type<T>::IS_BF16 ? 1 : 0, 128, D, 0, 1);
+      bool ok = mbar_wait(q_ready, 0, abort_flag, p.status, ERR_WAIT_PRODUCER);
+      auto tile_wait = [&](int n) {
+        return mbar_wait(&tile_full[n % Shape::TILES], (n / Shape::TILES) & 1, abort_flag, p.status, ERR_WAIT_DEQUANT);
+      };
+      auto s_col = [&](int i, int j) { return tmem + (SUB == 2 ? i * 128 : (j & 1) * BLK); };
+      auto qk = [&](int i, int j) {
+        const uint32_t sq = smem_u32(smem + i * Shape::Q_BYTES);
+        const uint32_t sk = smem_u32(smem + Shape::OFF_TILE + (2 * j) % Shape::TILES * Shape::TILE_BYTES);
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+          const uint64_t a = umma_smem_desc(sq + (kk >> 2) * (128 * 128) + (kk & 3) * 32, 16, 1024);
+          const uint64_t b = umma_smem_desc(sk + (kk >> 2) * (BLK * 128) + (kk & 3) * 32, 16, 1024);
+          umma_f16(s_col(i, j), a, b, idesc_qk, kk ? 1u : 0u);
+        }
+        umma_commit(&s_full[SUB == 2 ? i : j & 1]);
+      };
+      auto pv = [&](int i, int j) {
+        const uint32_t sv = smem_u32(smem + Shape::OFF_TILE + (2 * j + 1) % Shape::TILES * Shape::TILE_BYTES);
+#pragma unroll
+        for (int kk = 0; kk < BLK / 16; ++kk) {
+          // V: MN-major, 64-wide atoms along channels (LBO), 8-position groups (SBO)
+          const uint64_t b = umma_smem_desc(sv + kk * 2048, BLK * 128, 1024);
+          kv4_umma_ts(tmem + Shape::O_COL + i * Shape::O_STEP, s_col(i, j) + kk * 8, b, idesc_pv, (j | kk) ? 1u : 0u);
+        }
+        if (SUB == 1) umma_commit(pv_done);
+      };
+      ok = ok && tile_wait(0);
+      if (ok) {
+        tc_fence_after();
+#pragma unroll
+        for (int i = 0; i < SUB; ++i)
+          if (nblk[i] > 0) qk(i, 0);
+        umma_commit(&tile_empty[0]);
+      }
+      for (int j = 0; j < nmax && ok; ++j) {
+        if (SUB == 1 && j + 1 < nmax) {
+          ok = tile_wait(2 * j + 2);
+          if (!ok) break;
+          tc_fence_after();
+          qk(0, j + 1);
+          umma_commit(&tile_empty[(2 * j + 2) % Shape::TILES]);
+        }
+        ok = tile_wait(2 * j + 1);
+#pragma unroll
+        for (int i = 0; i < SUB; ++i) {
+          if (!ok || j >= nblk[i]) continue;
+          ok = SUB == 2 ? mbar_wait(&p_full[i], j & 1, abort_flag, p.status, ERR_WAIT_EPILOGUE)
+                        : mbar_wait(&p_full[j & 1], (j >> 1) & 1, abort_flag, p.status, ERR_WAIT_EPILOGUE);
+          if (!ok) continue;
+          tc_fence_after();
+          pv(i, j);
+          if (j + 1 == nblk[i]) umma_commit(&o_done[i]);
+          if (SUB == 2 && j + 1 < nblk[i]) {
+            ok = tile_wait(2 * j + 2);
+            if (!ok) continue;
+            tc_fence_after();
+            qk(i, j + 1);
+          }
+        }
+        if (!ok) break;
+        umma_commit(&tile_empty[(2 * j + 1) % Shape::TILES]);
+        if (SUB == 2 && j + 1 < nmax) umma_commit(&tile_empty[(2 * j + 2) % Shape::TILES]);
+      }
+    }
+  } else if (warp >= SUB * 4) {
+    // ---------------------------------------------------------------- expanding warps
+    // A warp takes 32 of a raw slot's 64 positions and half of the groups; lane = position, so the 16-byte loads
+    // (row pitch 5/8 D bytes) and the swizzled 16-byte stores are free of bank conflicts.
+    const int w = warp - SUB * 4;
+    const int token = (w & 1) * 32 + lane;
+    const int reach = max(info.reach[0], SUB == 2 ? info.reach[1] : 0);
+    const int first = EXT && p.q_kvstart ? info.first : 0;
+    bool ok = true;
+    int m = 0;
+    for (int n = 0; n < 2 * nmax && ok; ++n) {
+      const int b = n % Shape::TILES;
+      if (n >= Shape::TILES) {
+        ok = mbar_wait(&tile_empty[b], ((n / Shape::TILES) & 1) ^ 1, abort_flag, p.status, ERR_WAIT_MMA);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+      }
+      uint8_t* dst = smem + Shape::OFF_TILE + b * Shape::TILE_BYTES;
+      const int base = base_of(n >> 1);
+      for (int part = 0; part < Shape::RAW_PER_TILE; ++part, ++m) {
+        const int s = m % Shape::RAW_SLOTS;
+        ok = mbar_wait(&raw_full[s], (m / Shape::RAW_SLOTS) & 1, abort_flag, p.status, ERR_WAIT_TMA);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        const uint8_t* src = smem + Shape::OFF_RAW + s * Shape::RAW_BYTES + token * ROW;
+        const int at = part * Shape::RAW_TOKENS + token;  // position in the block
+        // V of a position that no row sees counts as 0 whatever its bytes hold (P is 0 there; 0 * NaN is not)
+        const bool live = !(n & 1) || (base + at < reach && base + at < room && (base + at >= first || base + at < p.sink));
+        uint8_t* row = dst + at * 128;
+#pragma unroll
+        for (int gi = 0; gi < (GROUPS + 1) / 2; ++gi) {
+          const int g = gi * 2 + (w >> 1);
+          if (GROUPS % 2 && g >= GROUPS) break;
+          uint32_t c[4];
+          if constexpr (ROW % 16 == 0) {
+            kv4_words<4>(src + g * 16, c);
+          } else {
+#pragma unroll
+            for (int x = 0; x < 4; ++x) c[x] = reinterpret_cast<const uint32_t*>(src)[g * 4 + x];
+          }
+          uint32_t meta = reinterpret_cast<const uint32_t*>(src + D / 2)[g];
+          if (!live) meta = 0u;
+          const uint32_t lo2 = __byte_perm(meta, meta, 0x1010), s2 = __byte_perm(meta, meta, 0x3232);
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            uint32_t v[4];
+            Kv4Type<T>::expand4(c[x], s2, lo2, v);
+            const int chunk = (g & 1) * 4 + x;  // 16-byte chunk of the 64-channel atom
+            *reinterpret_cast<uint4*>(row + (g >> 1) * (BLK * 128) + ((chunk ^ (at & 7)) << 4)) =
+                make_uint4(v[0], v[1], v[2], v[3]);
+          }
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&raw_empty[s]);
+      }
+      if (!ok) break;
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&tile_full[b]);
+    }
+  } else {
+    // ---------------------------------------------------------------- softmax / epilogue
+    const int sub = warp >> 2;
+    const int row = threadIdx.x & 127;                 // row of the tile
+    const int grow = sub * 128 + row;                  // row of the CTA
+    const bool row_valid = grow < valid_rows;
+    const bool warp_active = sub * 128 + (warp & 3) * 32 < valid_rows;
+    const int tok = qstart + (row_valid ? (row0 + grow) / G : 0), head = hk * G + (row_valid ? (row0 + grow) % G : 0);
+    {
+      const uint4* src = reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(p.q) +
+                                                        (static_cast<size_t>(tok) * p.q_stride + static_cast<size_t>(head) * D) * 2);
+      uint8_t* dst = smem + sub * Shape::Q_BYTES + row * 128;
+#pragma unroll
+      for (int c = 0; c < D / 8; ++c) {
+        uint4 v = row_valid ? src[c] : make_uint4(0, 0, 0, 0);
+        if (row_valid) {
+          v.x ^= p.q_flip;
+          v.y ^= p.q_flip;
+          v.z ^= p.q_flip;
+          v.w ^= p.q_flip;
+        }
+        *reinterpret_cast<uint4*>(dst + (c >> 3) * (128 * 128) + (((c & 7) ^ (row & 7)) << 4)) = v;
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(q_ready);
+    }
+    const int kvlen = row_valid ? p.q_kvlen[tok] : 0;
+    int start = 0;
+    unsigned long long tm = 0ull;
+    if (EXT && row_valid) {
+      if (p.q_kvstart) start = p.q_kvstart[tok];
+      if (p.tree_mask) tm = p.tree_mask[tok];
+    }
+    const float scale = EXT && p.cap_log2 != 0.f ? 1.f : p.scale_log2;
+    const int mine = sub ? nblk[1] : nblk[0], all_to = info.all_to[sub], all_from = info.all_from[sub];
+    const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t t_o = tmem + lanes + Shape::O_COL + sub * Shape::O_STEP;
+    float m_ref = -INFINITY, l = 0.f;
+    bool ok = true;
+    for (int j = 0; j < mine && ok; ++j) {
+      ok = SUB == 2 ? mbar_wait(&s_full[sub], j & 1, abort_flag, p.status, ERR_WAIT_MMA)
+                    : mbar_wait(&s_full[j & 1], (j >> 1) & 1, abort_flag, p.status, ERR_WAIT_MMA);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      tc_fence_after();
+      const uint32_t t_s = tmem + lanes + (SUB == 2 ? sub * 128 : (j & 1) * BLK);
+      if (warp_active) {
+        const int base = base_of(j);
+        const bool plain = base + BLK <= all_to && (!EXT || base >= all_from || base + BLK <= p.sink);
+        uint32_t pk[BLK / 2];
+        float sum = 0.f, mx = -INFINITY;
+        // 32 columns: scores, their maximum, weights against the reference `shift` = -m
+        auto columns = [&](int c, float shift, bool weights) {
+          uint32_t r[32];
+          __syncwarp();
+          tmem_ld32(t_s + c * 32, r);
+          tmem_ld_wait();
+          if (EXT && p.cap_log2 != 0.f) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(kv4_softcap(__uint_as_float(r[i]), p.cap_k, p.cap_log2));
+          }
+          if (!plain) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (!kv4_visible(base + c * 32 + i, kvlen, start, EXT ? p.sink : 0, tm)) r[i] = 0xff800000u;
+          }
+          if (!weights) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) mx = fmaxf(mx, __uint_as_float(r[i]));
+            return;
+          }
+          float2 acc = make_float2(0.f, 0.f);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const float2 v = make_float2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
+            mx = fmaxf(mx, fmaxf(v.x, v.y));
+            const float2 x = kv4_fma2(v, make_float2(scale, scale), make_float2(shift, shift));
+            const float2 e = make_float2(exp2f(x.x), exp2f(x.y));
+            acc = kv4_add2(acc, e);
+            pk[c * 16 + i] = Kv4Type<T>::pack(e.x, e.y);
+          }
+          sum += acc.x + acc.y;
+        };
+        bool redo = j == 0;
+        if (j > 0) {
+          const float shift = m_ref == -INFINITY ? 0.f : -m_ref;
+#pragma unroll
+          for (int c = 0; c < BLK / 32; ++c) columns(c, shift, true);
+          redo = mx * scale > m_ref + 8.f;
+        } else {
+#pragma unroll
+          for (int c = 0; c < BLK / 32; ++c) columns(c, 0.f, false);
+        }
+        if (__any_sync(0xffffffffu, redo)) {
+          const float m_new = fmaxf(m_ref, mx * scale);
+          const float alpha = m_ref == -INFINITY ? 0.f : exp2f(m_ref - m_new);
+          if (j > 0) {
+            if (SUB == 1) {  // the scores of this block were computed before the last P V ended
+              ok = mbar_wait(pv_done, (j - 1) & 1, abort_flag, p.status, ERR_WAIT_MMA);
+              ok = __all_sync(0xffffffffu, ok);
+              if (!ok) break;
+              tc_fence_after();
+            }
+#pragma unroll 1
+            for (int c = 0; c < D; c += 32) {
+              uint32_t o[32];
+              tmem_ld32(t_o + c, o);
+              tmem_ld_wait();
+#pragma unroll
+              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+              kv4_tmem_st32(t_o + c, o);
+            }
+          }
+          l *= m_ref == -INFINITY ? 1.f : alpha;
+          m_ref = m_new;
+          sum = 0.f;
+          const float shift = m_ref == -INFINITY ? 0.f : -m_ref;
+#pragma unroll
+          for (int c = 0; c < BLK / 32; ++c) columns(c, shift, true);
+        }
+        l += sum;
+#pragma unroll
+        for (int c = 0; c < BLK / 64; ++c) kv4_tmem_st32(t_s + c * 32, pk + c * 32);
+        kv4_tmem_st_wait();
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&p_full[SUB == 2 ? sub : j & 1]);
+    }
+    // ---- epilogue: O / l, or the partial row
+    if (ok && mine > 0) {
+      ok = mbar_wait(&o_done[sub], 0, abort_flag, p.status, ERR_WAIT_MMA);
+      ok = __all_sync(0xffffffffu, ok);
+    }
+    if (ok && warp_active) {
+      tc_fence_after();
+      const float inv = l == 0.f ? 0.f : 1.f / l;  // a row that sees nothing is 0; NaN stays NaN
+      const size_t prow = ((static_cast<size_t>(work) * p.hkv + hk) * p.splits + split) * (SUB * 128) + grow;
+#pragma unroll 1
+      for (int c = 0; c < D; c += 32) {
+        uint32_t o[32];
+        __syncwarp();
+        if (mine > 0) {
+          tmem_ld32(t_o + c, o);
+          tmem_ld_wait();
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i] = 0;
+        }
+        if (row_valid && p.splits > 1) {
+          float* dst = p.part_o + prow * D + c;
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            reinterpret_cast<uint4*>(dst)[i] = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+        } else if (row_valid) {
+          uint8_t* dst = reinterpret_cast<uint8_t*>(p.out) + ((static_cast<size_t>(tok) * p.hq + head) * D + c) * 2;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            uint32_t v[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              v[k] = Kv4Type<T>::pack(__uint_as_float(o[i * 8 + 2 * k]) * inv, __uint_as_float(o[i * 8 + 2 * k + 1]) * inv);
+            reinterpret_cast<uint4*>(dst)[i] = make_uint4(v[0], v[1], v[2], v[3]);
+          }
+        }
+      }
+      if (row_valid) {
+        if (p.splits > 1) {
+          p.part_ml[prow * 2] = m_ref;
+          p.part_ml[prow * 2 + 1] = l;
+        } else if (p.lse) {
+          p.lse[static_cast<size_t>(tok) * p.hq + head] = l == 0.f ? -INFINITY : (m_ref + log2f(l)) * 0.6931471805599453f;
+        }
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == ISSUER) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// Joins the splits: one warp per row, grid (tiles, hkv).
+template <typename T, int D>
+__global__ void __launch_bounds__(256) kv4_prefill_merge_kernel(const Kv4PreParams p) {
+  constexpr int ROWS = Kv4PreShape<D>::SUB * 128;
+  const int tile = blockIdx.x / p.parts, row0 = blockIdx.x % p.parts * 128;
+  const int hk = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int qstart = p.tile_qstart[tile], rows = min(ROWS, p.tile_ntok[tile] * p.group - row0);
+  for (int row = blockIdx.z * 8 + warp; row < rows; row += 8 * gridDim.z) {
+    const size_t first = (static_cast<size_t>(blockIdx.x) * p.hkv + hk) * p.splits * ROWS + row;
+    float M = -INFINITY, L = 0.f, acc[D / 32];
+    for (int s = 0; s < p.splits; ++s) M = fmaxf(M, p.part_ml[(first + s * ROWS) * 2]);
+#pragma unroll
+    for (int c = 0; c < D / 32; ++c) acc[c] = 0.f;
+    for (int s = 0; s < p.splits; ++s) {
+      const size_t b = first + s * ROWS;
+      const float ms = p.part_ml[b * 2], ls = p.part_ml[b * 2 + 1];
+      const float w = ms == -INFINITY ? 0.f : exp2f(ms - M);
+      L += ls != ls ? ls : ls * w;
+#pragma unroll
+      for (int c = 0; c < D / 32; ++c) acc[c] = fmaf(p.part_o[b * D + c * 32 + lane], w, acc[c]);
+    }
+    const size_t at = static_cast<size_t>(qstart + (row0 + row) / p.group) * p.hq + hk * p.group + (row0 + row) % p.group;
+    const float inv = L == 0.f ? 0.f : 1.f / L;
+    T* dst = reinterpret_cast<T*>(p.out) + at * D;
+#pragma unroll
+    for (int c = 0; c < D / 32; ++c) dst[c * 32 + lane] = Cvt<T>::from_f(acc[c] * inv);
+    if (p.lse && lane == 0) p.lse[at] = L == 0.f ? -INFINITY : (M + log2f(L)) * 0.6931471805599453f;
+  }
+}
+
+template <typename T, int D, bool EXT>
+int kv4_prefill_launch(const Kv4PreParams& p, cudaStream_t stream) {
+  using Shape = Kv4PreShape<D>;
+  auto kern = kv4_prefill_kernel<T, D, EXT>;
+  static bool attr_set[64] = {};
+  if (first_use_on_device(attr_set)) {
+    const cudaError_t err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::SMEM);
+    if (err != cudaSuccess) return static_cast<int>(err);
+  }
+  kern<<<dim3(p.num_tiles * p.parts * p.splits, p.hkv), Shape::THREADS, Shape::SMEM, stream>>>(p);
+  count_launch();
+  if (p.splits > 1) {
+    kv4_prefill_merge_kernel<T, D><<<dim3(p.num_tiles * p.parts, p.hkv, 8), 256, 0, stream>>>(p);
+    count_launch();
+  }
+  return static_cast<int>(cudaGetLastError());
+}
+
+template <typename T>
+int kv4_prefill_shape(const Kv4PreParams& p, int d, bool ext, cudaStream_t stream) {
+  if (d == 64) return ext ? kv4_prefill_launch<T, 64, true>(p, stream) : kv4_prefill_launch<T, 64, false>(p, stream);
+  if (d == 96) return ext ? kv4_prefill_launch<T, 96, true>(p, stream) : kv4_prefill_launch<T, 96, false>(p, stream);
+  if (d == 128) return ext ? kv4_prefill_launch<T, 128, true>(p, stream) : kv4_prefill_launch<T, 128, false>(p, stream);
+  return ext ? kv4_prefill_launch<T, 256, true>(p, stream) : kv4_prefill_launch<T, 256, false>(p, stream);
+}
+
+}  // namespace mlcb
+
+using namespace mlcb;
+
+// One layer's cache [num_pages, 2, hkv, 16, row]. Tiles are (sequence, query-token range) pairs with tokens * hq / hkv
+// <= tile_rows <= 256. splits > 1 needs fp32 scratch for 256 rows per (tile, kv head, split): part_o [.., 256, d] and
+// part_ml [.., 256, 2]. Returns -1 shape, -2 alignment, -3 type, -4 missing scratch.
+MLCB_API int mlcb_kv4_prefill(const void* q, const void* pages, void* out, float* lse, const int* tile_seq,
+                              const int* tile_qstart, const int* tile_ntok, const int* q_kvlen, const int* page_indptr,
+                              const int* page_indices, int num_tiles, int tile_rows, long long q_stride, int hq, int hkv,
+                              int d, long long num_pages, float sm_scale, int dtype, int splits, float* part_o,
+                              float* part_ml, int* status, cudaStream_t stream, const int* q_kvstart,
+                              const unsigned long long* tree_mask, int sink, float softcap) {
+  if (num_tiles <= 0) return 0;
+  if (hkv <= 0 || hkv > 65535 || hq <= 0 || hq % hkv || (d != 64 && d != 96 && d != 128 && d != 256)) return -1;
+  if (tile_rows < 1 || tile_rows > 256) return -1;
+  if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(pages)) & 15) return -2;
+  if (q_stride % 8) return -2;
+  if (dtype != 0 && dtype != 1) return -3;
+  if (splits < 1 || (splits > 1 && (!part_o || !part_ml)) || static_cast<long long>(num_tiles) * splits * 2 > 0x7fffffffLL) return -4;
+  Kv4PreParams p;
+  p.q = q;
+  p.pages = static_cast<const uint8_t*>(pages);
+  p.out = out;
+  p.lse = lse;
+  p.part_o = part_o;
+  p.part_ml = part_ml;
+  p.tile_seq = tile_seq;
+  p.tile_qstart = tile_qstart;
+  p.tile_ntok = tile_ntok;
+  p.q_kvlen = q_kvlen;
+  p.page_indptr = page_indptr;
+  p.page_indices = page_indices;
+  p.q_kvstart = q_kvstart;
+  p.tree_mask = tree_mask;
+  p.status = status;
+  p.q_stride = q_stride;
+  p.num_pages = num_pages;
+  p.hq = hq;
+  p.hkv = hkv;
+  p.group = hq / hkv;
+  p.sink = q_kvstart ? sink : 0;
+  p.splits = splits;
+  p.num_tiles = num_tiles;
+  p.parts = d == 256 && tile_rows > 128 ? 2 : 1;
+  p.q_flip = sm_scale < 0.f ? 0x80008000u : 0u;
+  p.scale_log2 = fmaxf(fabsf(sm_scale) * 1.4426950408889634f, 1e-30f);  // a hidden score is -inf * scale: not 0
+  p.cap_k = softcap > 0.f ? 2.f * 1.4426950408889634f * fabsf(sm_scale) / softcap : 0.f;
+  p.cap_log2 = softcap > 0.f ? softcap * 1.4426950408889634f : 0.f;
+  const bool ext = q_kvstart || tree_mask || softcap > 0.f;
+  return dtype == 0 ? kv4_prefill_shape<__half>(p, d, ext, stream) : kv4_prefill_shape<__nv_bfloat16>(p, d, ext, stream);
+}

@@ -12,16 +12,16 @@ import torch
 from ._lib import DTYPE_CODE, check, lib, ptr, status_word, stream_ptr
 
 
-def build_tiles(q_indptr: np.ndarray, group: int, decode_items: bool = True) -> Dict[str, np.ndarray]:
+def build_tiles(q_indptr: np.ndarray, group: int, decode_items: bool = True, tile_rows: int = 128) -> Dict[str, np.ndarray]:
     """Split the appended tokens of a batch into work items for the two attention kernels.
 
     Sequences whose chunk fits 16 query rows (``tokens * group <= 16``: decode and short verify
     chunks) become one item each for the decode kernel (``dec_seq``, ``dec_qstart``, ``dec_ntok``).
-    The others are cut into tiles of ``128 // group`` tokens for the tcgen05 kernel (``tile_seq``,
-    ``tile_qstart``, ``tile_ntok``). All arrays are int32; ``*_qstart`` are global token indices.
+    The others are cut into tiles of ``tile_rows // group`` tokens for the tcgen05 kernel (``tile_seq``,
+    ``tile_qstart``, ``tile_ntok``; 128 rows over a 16-bit cache, up to 256 over a 4-bit one). All arrays are int32; ``*_qstart`` are global token indices.
     ``decode_items=False`` sends every sequence to the tcgen05 kernel.
     """
-    tpt = max(1, 128 // group)
+    tpt = max(1, tile_rows // group)
     q_indptr = np.asarray(q_indptr, dtype=np.int64)
     lens_all = np.diff(q_indptr)
     small = (lens_all * group <= 16) & (lens_all > 0) if group <= 16 and decode_items \
@@ -60,6 +60,7 @@ class AttentionPlan:
     num_dec: int = 0
     dec_splits: int = 1
     max_pages: int = 0
+    tile_rows: int = 128  # most query rows of any tile
     dec_rows: int = 16  # most query rows (tokens x heads of a group) of any decode item
 
 

@@ -123,18 +123,21 @@ def kv4_read(kv_pages: torch.Tensor, slot: torch.Tensor, d: int) -> Tuple[torch.
 
 
 # --------------------------------------------------------------------------- attention
+KV4_TILE_ROWS = 256  # query rows that share one expansion of the cached blocks
+
+
 def kv4_plan(q_indptr, q_kvlen: torch.Tensor, page_indptr: torch.Tensor, page_indices: torch.Tensor, hq: int, hkv: int,
              max_len: int) -> AttentionPlan:
     """The tiling of one step for ``ops.paged_attention`` over a packed cache (shared by all layers). ``q_indptr``:
     host array, first token of every sequence's chunk; ``max_len``: the longest sequence, appended tokens included."""
     q_indptr = np.asarray(q_indptr, dtype=np.int64)
-    tiles = build_tiles(q_indptr, hq // hkv)
+    tiles = build_tiles(q_indptr, hq // hkv, tile_rows=KV4_TILE_ROWS)
     dev = q_kvlen.device
     on = {k: torch.from_numpy(a).to(dev) for k, a in tiles.items()}
     num_dec = len(tiles["dec_seq"])
     return AttentionPlan(on["tile_seq"], on["tile_qstart"], on["tile_ntok"], q_kvlen, page_indptr, page_indices,
                          len(tiles["tile_seq"]), dec_seq=on["dec_seq"], dec_qstart=on["dec_qstart"], dec_ntok=on["dec_ntok"],
-                         num_dec=num_dec, dec_splits=1, max_pages=(int(max_len) + 15) // 16,
+                         num_dec=num_dec, dec_splits=1, max_pages=(int(max_len) + 15) // 16, tile_rows=KV4_TILE_ROWS,
                          dec_rows=int(tiles["dec_ntok"].max()) * (hq // hkv) if num_dec else 16)
 
 
@@ -176,30 +179,70 @@ def attend(q: torch.Tensor, kv_pages: torch.Tensor, q_seq: torch.Tensor, q_kvlen
     return (out, lse) if return_lse else out
 
 
+def _decode(q, kv_pages, out, lse, q_kvlen, page_indptr, page_indices, hq, hkv, d, sm_scale, q_kvstart, sink, tree_mask,
+            softcap, plan) -> None:
+    # with one token per item the rows are the group's heads, whatever the plan was made for
+    rows = hq // hkv if q.shape[0] == plan.num_dec else min(16, plan.dec_rows)
+    ctas = _decode_ctas(plan.num_dec, rows, hkv, plan.max_pages, q.device)
+    part = torch.empty(ctas * (2 * 16 * (d + 2) + 4), dtype=torch.float32, device=q.device)
+    part_unit, part_ml, part_o = part[: 4 * ctas], part[4 * ctas: 68 * ctas], part[68 * ctas:]
+    rc = lib().mlcb_kv4_decode(ptr(q), ptr(kv_pages), ptr(out), ptr(lse), ptr(plan.dec_seq), ptr(plan.dec_qstart),
+                               ptr(plan.dec_ntok), ptr(q_kvlen), ptr(page_indptr), ptr(page_indices), c_int(plan.num_dec),
+                               c_int(rows), c_ll(q.stride(0)), c_int(hq), c_int(hkv), c_int(d), c_ll(kv_pages.shape[0]),
+                               c_float(sm_scale), c_int(DTYPE_CODE[q.dtype]), c_int(ctas), ptr(part_o), ptr(part_ml),
+                               ptr(part_unit), ptr(status_word(q.device)), stream_ptr(), ptr(q_kvstart), ptr(tree_mask),
+                               c_int(sink), c_float(softcap))
+    check(rc, "mlcb_kv4_decode")
+
+
+def _prefill_splits(ctas: int, blocks: int, device: torch.device) -> int:
+    """KV splits of the prefill kernel (one CTA per SM): few tiles are cut so that they cover the SMs, two blocks of
+    cached positions per split at least."""
+    return max(1, min(sm_count(device) // max(1, ctas), blocks // 2, 64))
+
+
+def _prefill(q, kv_pages, out, lse, q_kvlen, page_indptr, page_indices, hq, hkv, d, sm_scale, q_kvstart, sink, tree_mask,
+             softcap, plan, decode_items: bool) -> None:
+    if decode_items:
+        seq, qstart, ntok, num, rows = plan.dec_seq, plan.dec_qstart, plan.dec_ntok, plan.num_dec, min(16, plan.dec_rows)
+    else:
+        seq, qstart, ntok, num, rows = plan.tile_seq, plan.tile_qstart, plan.tile_ntok, plan.num_tiles, plan.tile_rows
+    ctas = num * hkv * (2 if d == 256 and rows > 128 else 1)
+    splits = _prefill_splits(ctas, plan.max_pages // (4 if d == 256 else 8), q.device)
+    part_o = part_ml = None
+    if splits > 1:
+        part = torch.empty(num * hkv * splits * 256 * (d + 2), dtype=torch.float32, device=q.device)
+        part_ml, part_o = part[: num * hkv * splits * 512], part[num * hkv * splits * 512:]
+    rc = lib().mlcb_kv4_prefill(ptr(q), ptr(kv_pages), ptr(out), ptr(lse), ptr(seq), ptr(qstart), ptr(ntok), ptr(q_kvlen),
+                                ptr(page_indptr), ptr(page_indices), c_int(num), c_int(rows), c_ll(q.stride(0)), c_int(hq),
+                                c_int(hkv), c_int(d), c_ll(kv_pages.shape[0]), c_float(sm_scale),
+                                c_int(DTYPE_CODE[q.dtype]), c_int(splits), ptr(part_o), ptr(part_ml),
+                                ptr(status_word(q.device)), stream_ptr(), ptr(q_kvstart), ptr(tree_mask), c_int(sink),
+                                c_float(softcap))
+    check(rc, "mlcb_kv4_prefill")
+
+
 def _launch(q, kv_pages, out, lse, q_seq, q_kvlen, page_indptr, page_indices, hq, hkv, d, page, sm_scale, q_kvstart, sink,
             tree_mask, softcap, plan) -> None:
-    t, group = q.shape[0], hq // hkv
-    dtype, status = c_int(DTYPE_CODE[q.dtype]), ptr(status_word(q.device))
+    t = q.shape[0]
     aligned = q.data_ptr() % 16 == 0 and (q.stride(0) % 8 == 0 or t == 1)
-    if plan is not None and plan.use_tensor_core and page == 16 and d in (64, 128, 256) and aligned and not plan.num_tiles:
+    if plan is not None and plan.use_tensor_core and page == 16 and d in (64, 96, 128, 256) and aligned \
+            and hq // hkv <= plan.tile_rows:
+        args = (q, kv_pages, out, lse, q_kvlen, page_indptr, page_indices, hq, hkv, d, sm_scale, q_kvstart, sink, tree_mask,
+                softcap, plan)
         if plan.num_dec:
-            # with one token per item the rows are the group's heads, whatever the plan was made for
-            rows = group if t == plan.num_dec else min(16, plan.dec_rows)
-            ctas = _decode_ctas(plan.num_dec, rows, hkv, plan.max_pages, q.device)
-            part = torch.empty(ctas * (2 * 16 * (d + 2) + 4), dtype=torch.float32, device=q.device)
-            part_unit, part_ml, part_o = part[: 4 * ctas], part[4 * ctas: 68 * ctas], part[68 * ctas:]
-            rc = lib().mlcb_kv4_decode(ptr(q), ptr(kv_pages), ptr(out), ptr(lse), ptr(plan.dec_seq), ptr(plan.dec_qstart),
-                                       ptr(plan.dec_ntok), ptr(q_kvlen), ptr(page_indptr), ptr(page_indices),
-                                       c_int(plan.num_dec), c_int(rows), c_ll(q.stride(0)), c_int(hq), c_int(hkv), c_int(d),
-                                       c_ll(kv_pages.shape[0]), c_float(sm_scale), dtype, c_int(ctas), ptr(part_o),
-                                       ptr(part_ml), ptr(part_unit), status, stream_ptr(), ptr(q_kvstart), ptr(tree_mask), c_int(sink),
-                                       c_float(softcap))
-            check(rc, "mlcb_kv4_decode")
+            if d == 96:  # no decode kernel: its lanes own powers of two of channels
+                _prefill(*args, decode_items=True)
+            else:
+                _decode(*args)
+        if plan.num_tiles:
+            _prefill(*args, decode_items=False)
         return
     rc = lib().mlcb_kv4_attn_simt(ptr(q), ptr(kv_pages), ptr(out), ptr(lse), ptr(q_seq), ptr(q_kvlen), ptr(q_kvstart),
                                   ptr(tree_mask), ptr(page_indptr), ptr(page_indices), c_int(t), c_ll(q.stride(0)),
                                   c_int(hq), c_int(hkv), c_int(d), c_int(page), c_ll(kv_pages.shape[0]), c_int(sink),
-                                  c_float(sm_scale), c_float(softcap), dtype, status, stream_ptr())
+                                  c_float(sm_scale), c_float(softcap), c_int(DTYPE_CODE[q.dtype]),
+                                  ptr(status_word(q.device)), stream_ptr())
     check(rc, "mlcb_kv4_attn_simt")
 
 

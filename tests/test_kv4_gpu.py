@@ -176,6 +176,7 @@ class Step:
         hq, hkv, d, g = self.hq, self.hkv, self.d, self.hq // self.hkv
         u, scale = torch.finfo(self.dtype).eps / 2, d ** -0.5
         q = self.q.cpu().double().view(-1, hkv, g, d)
+        assert out.shape == (q.shape[0], hq * d)
         got = out.cpu().double().view(-1, hkv, g, d)
         for t in range(q.shape[0]):
             n = int(self.kvlen[t])
@@ -251,6 +252,39 @@ def test_decode(dtype, case):
     assert _same_bytes(out, again)   # no atomics: the same call gives the same bits
 
 
+PREFILL = [
+    ([100], [100], 8, 2, 128, {}),
+    ([300, 17, 64, 1], [300, 17, 64, 1], 8, 2, 128, {}),           # two query tiles, one, and decode items next to them
+    ([700, 260], [200, 129], 32, 8, 128, {}),                      # chunks behind a cached prefix
+    ([3000], [40], 8, 2, 128, {}),                                 # few rows, long prefix: split and joined
+    ([2500, 700], [33, 70], 14, 2, 64, {}),                        # 7 heads: rows of a token straddle the tiles
+    ([150, 129], [150, 64], 4, 4, 64, {}),
+    ([400, 90], [300, 90], 8, 4, 256, {}),
+    ([1500], [45], 16, 1, 256, {}),                                # more than 128 rows per tile at d = 256, split
+    ([200, 500, 31], [130, 60, 1], 4, 4, 96, {}),
+    ([70, 129], [1, 1], 6, 2, 96, {}),                             # d = 96 decodes through this kernel too
+    ([600, 300], [300, 100], 8, 2, 128, {"window": 100, "sink": 20}),
+    ([2000], [60], 8, 2, 128, {"window": 300, "sink": 4}),
+    ([300, 140], [300, 40], 8, 2, 64, {"window": 64}),
+    ([300, 150], [150, 150], 8, 4, 256, {"window": 128, "sink": 4, "cap": 50.0}),
+    ([200, 90], [200, 30], 8, 2, 128, {"cap": 30.0}),
+    ([400, 1000, 60], [60, 31, 25], 8, 2, 128, {"tree": True}),
+    ([400, 100], [20, 50], 8, 4, 256, {"tree": True}),
+    ([300, 77], [200, 20], 8, 2, 128, {"q_by": 3000.0, "k_by": 2.0 ** -11}),
+]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("case", range(len(PREFILL)))
+def test_prefill(dtype, case):
+    lens, new, hq, hkv, d, extra = PREFILL[case]
+    st = Step(dtype, lens, new, hq, hkv, d, seed=case, **extra)
+    out, lse = st.run()
+    ops.check_status(out.device)
+    st.check(out, lse)
+    assert _same_bytes(out, st.run(lse=False))
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("lens,new,hq,hkv,d,page,extra", [
     ([60, 5], [3, 5], 4, 4, 96, 16, {}), ([60, 5], [1, 2], 4, 2, 32, 16, {"cap": 20.0}),
@@ -277,19 +311,28 @@ def test_rows_that_see_nothing(d):
         out, lse = st.run(plan=plan)
         ops.check_status(out.device)
         st.check(out, lse)
+    # the same among the rows of a prefill tile
+    st = Step(torch.float16, [200, 60], [150, 50], 8, 2, d, window=64, sink=2)
+    st.kvlen[10], st.kvlen[151], st.kvstart[20], st.kvstart[160] = 0, 0, 5000, 200
+    for plan in (True, False):
+        out, lse = st.run(plan=plan)
+        ops.check_status(out.device)
+        st.check(out, lse)
 
 
 def test_page_numbers_outside_the_cache_are_reported():
     for plan in (True, False):
-        st = Step(torch.float16, [40, 40], [1, 1], 8, 2, 128)
-        st.indices[1] = st.cache.shape[0]
-        st.run(plan=plan)
-        with pytest.raises(ops.KernelError):
-            ops.check_status(st.cache.device)
-        st = Step(torch.float16, [40, 40], [1, 1], 8, 2, 128, kvlen=[40, 60])  # three pages hold 48 tokens
-        st.run(plan=plan)
-        with pytest.raises(ops.KernelError):
-            ops.check_status(st.cache.device)
+        for new in ([1, 1], [20, 20]):
+            st = Step(torch.float16, [40, 40], new, 8, 2, 128)
+            st.indices[1] = st.cache.shape[0]
+            st.run(plan=plan)
+            with pytest.raises(ops.KernelError):
+                ops.check_status(st.cache.device)
+            st = Step(torch.float16, [40, 40], new, 8, 2, 128)
+            st.kvlen[-1] = 60  # three pages hold 48 tokens
+            st.run(plan=plan)
+            with pytest.raises(ops.KernelError):
+                ops.check_status(st.cache.device)
 
 
 def test_offsets_beyond_32_bits():
