@@ -4,6 +4,8 @@
 // pages hold 16-bit values only.
 #include "kv4.cuh"
 
+#include <type_traits>
+
 namespace mlcb {
 
 // ------------------------------------------------------------------ append
@@ -27,34 +29,70 @@ __device__ __forceinline__ float kv4_sane(float v) {
   return v != v ? 0.f : fminf(fmaxf(v, -Kv4Type<T>::BOUND), Kv4Type<T>::BOUND);
 }
 
-// Quantises the 8 values of `val` (lanes 4 i .. 4 i + 3 hold one group) and stores code word and step / minimum.
+// Magnitude bits of KV4 bounds: larger ones (infinity and NaN among them) are clamped before quantisation.
+template <typename T>
+constexpr uint32_t KV4_BOUND_BITS = 0;
+template <>
+constexpr uint32_t KV4_BOUND_BITS<__half> = 0x7bfdu;          // 65440
+template <>
+constexpr uint32_t KV4_BOUND_BITS<__nv_bfloat16> = 0x7e80u;   // 2^126
+
+// The codes by the letter of the format: correctly rounded divisions.
+__device__ __noinline__ uint32_t kv4_codes_exact(const float (&f)[8], float lo, float s) {
+  uint32_t w = 0;
+  for (int j = 0; j < 8; ++j) {
+    const int c = min(15, __float2int_rn(__fdiv_rn(__fsub_rn(f[j], lo), s)));  // f >= lo: never negative
+    w |= static_cast<uint32_t>(c) << ((j & 1) * 16 + (j >> 1) * 4);
+  }
+  return w;
+}
+
+// Quantises the 8 values of `val` (lanes 4 i .. 4 i + 3 hold one group) and stores code word and minimum / step.
+// A code is rint of a quotient in [0, 15.1]. The reciprocal gives that quotient to 4e-6, so that only one within 6e-5
+// of a half-way point could round elsewhere: those words, and ones whose step is too coarse for the range (subnormal),
+// take the exact path. A division per value cost 3 200 of a token's 7 400 warp instructions.
 template <typename T>
 __device__ __forceinline__ void kv4_store8(const uint4& val, uint8_t* row, int chunk, int code_bytes) {
-  const T* e = reinterpret_cast<const T*>(&val);
+  const uint32_t bits[4] = {val.x, val.y, val.z, val.w};
+  const T* e = reinterpret_cast<const T*>(bits);
+  uint32_t mag = 0;
   float f[8];
-  float lo = INFINITY, hi = -INFINITY;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    f[j] = kv4_sane<T>(Cvt<T>::to_f(e[j]));
-    lo = fminf(lo, f[j]);
-    hi = fmaxf(hi, f[j]);
+  for (int j = 0; j < 4; ++j) mag = __vmaxu2(mag, bits[j] & 0x7fff7fffu);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) f[j] = Cvt<T>::to_f(e[j]);
+  if (max(mag & 0xffffu, mag >> 16) > KV4_BOUND_BITS<T>) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f[j] = kv4_sane<T>(f[j]);
   }
+  float lo = fminf(fminf(fminf(f[0], f[1]), fminf(f[2], f[3])), fminf(fminf(f[4], f[5]), fminf(f[6], f[7])));
+  float hi = fmaxf(fmaxf(fmaxf(f[0], f[1]), fmaxf(f[2], f[3])), fmaxf(fmaxf(f[4], f[5]), fmaxf(f[6], f[7])));
   const unsigned quad = 0xfu << (threadIdx.x & 28);
 #pragma unroll
   for (int o = 1; o < 4; o <<= 1) {
     lo = fminf(lo, __shfl_xor_sync(quad, lo, o));
     hi = fmaxf(hi, __shfl_xor_sync(quad, hi, o));
   }
-  // correctly rounded divisions, whatever the library is compiled with: the codes are the format's definition
-  const T st = Cvt<T>::from_f(__fdiv_rn(__fsub_rn(hi, lo), 15.f));
+  const float range = __fsub_rn(hi, lo);
+  const T st = Cvt<T>::from_f(__fdiv_rn(range, 15.f));
   const float s = Cvt<T>::to_f(st);
   uint32_t w = 0;
   if (s > 0.f) {
+    const float inv = __fdividef(1.f, s);
+    const float magic = 12582912.f;  // 1.5 * 2^23: a sum with it is rounded to a whole number, held in its low bits
+    float far = 0.f;
+    uint32_t sum = 0;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const int c = min(15, __float2int_rn(__fdiv_rn(__fsub_rn(f[j], lo), s)));  // f >= lo: never negative
-      w |= static_cast<uint32_t>(c) << ((j & 1) * 16 + (j >> 1) * 4);
+      const float t = __fmul_rn(__fsub_rn(f[j], lo), inv);
+      const float y = __fadd_rn(t, magic);
+      far = fmaxf(far, fabsf(__fsub_rn(t, __fsub_rn(y, magic))));
+      sum += __float_as_uint(y) << ((j & 1) * 16 + (j >> 1) * 4);
     }
+    // the magic number's own bits, 0x4b400000 << 0, 4, 8, 12 (16 and more shift them out): 0x4b400000 * 0x1111 mod 2^32
+    w = sum - 0x4b400000u * 0x1111u;
+    const bool sure = far < 0.5f - 6e-5f && __fmul_rn(range, inv) < 15.4f;  // not so for NaN
+    if (!sure) w = kv4_codes_exact(f, lo, s);
   }
   reinterpret_cast<uint32_t*>(row)[chunk] = w;
   if ((chunk & 3) == 0) {
@@ -131,31 +169,144 @@ kv4_append_kernel(T* __restrict__ qkv, uint8_t* __restrict__ pages, const int* _
   }
 }
 
+// The same for heads that are rotated as a whole (D = 64, 128, 256), which is what most models do. A thread takes one
+// 16-byte item of 8 rotary pairs of q, two pairs of k (4 bytes each side) and one code word: at 32 / 8 heads of 128 that
+// is one of each for all 256 threads, loaded before the angles are computed. k passes through shared memory between
+// its rotation, whose 64-bit pairs want all threads, and its quantisation, where four neighbouring lanes own a group.
+template <typename T, int D>
+__global__ void __launch_bounds__(KV4_APPEND_THREADS)
+kv4_append_whole_kernel(T* __restrict__ qkv, uint8_t* __restrict__ pages, const int* __restrict__ pos,
+                        const int* __restrict__ slot, const float* __restrict__ inv_freq, int hq, int hkv, int page,
+                        float attn_factor, long long num_slots, int* status) {
+  constexpr int HALF = D / 2, JG = HALF / 8, CPR = D / 8, RB = kv4_row_bytes(D), STEP = KV4_APPEND_THREADS;
+  __shared__ __align__(16) double sn[HALF], cs[HALF];
+  __shared__ float snf[HALF], csf[HALF];
+  extern __shared__ __align__(16) uint8_t smem[];
+  T* krow = reinterpret_cast<T*>(smem);  // [kv heads of this part][D]
+  const int t = blockIdx.x, parts = gridDim.y, part = blockIdx.y;
+  const int k0 = hkv * part / parts, kn = hkv * (part + 1) / parts - k0;
+  const int q0 = hq * part / parts, qn = hq * (part + 1) / parts - q0;
+  const int nq = qn * JG, nk = kn * (HALF / 2), nw = kn * CPR;  // q items, k items, words of k (and of v)
+  T* row = qkv + static_cast<size_t>(t) * (hq + 2 * hkv) * D;
+  T* qrow = row + q0 * D;
+  T* ksrc = row + (hq + k0) * D;
+  const T* vsrc = row + (hq + hkv + k0) * D;
+  auto q_at = [&](int i) { return reinterpret_cast<uint4*>(qrow + i / JG * D + i % JG * 8); };
+  auto k_at = [&](int i) { return reinterpret_cast<uint32_t*>(ksrc + i / (HALF / 2) * D + i % (HALF / 2) * 2); };
+  const int tid = threadIdx.x;
+  uint4 qa, qb, v;
+  uint32_t ka = 0, kb = 0;
+  qa = qb = v = make_uint4(0, 0, 0, 0);
+  if (tid < nq) {
+    qa = q_at(tid)[0];
+    qb = q_at(tid)[HALF / 8];
+  }
+  if (tid < nk) {
+    ka = k_at(tid)[0];
+    kb = k_at(tid)[HALF / 2];
+  }
+  if (tid >= nw && tid < 2 * nw) v = reinterpret_cast<const uint4*>(vsrc)[tid - nw];
+  const long long sl = slot[t];
+  const double p = static_cast<double>(pos[t]);
+  for (int j = tid; j < HALF; j += STEP) {
+    double s, c;
+    sincospi(p * static_cast<double>(inv_freq[j]) * 0.31830988618379067154, &s, &c);
+    sn[j] = s * attn_factor;
+    cs[j] = c * attn_factor;
+    const int at = j % 8 * JG + j / 8;  // the JG items of a head read neighbouring words
+    snf[at] = static_cast<float>(sn[j]);
+    csf[at] = static_cast<float>(cs[j]);
+  }
+  __syncthreads();
+  for (int i = tid; i < nk; i += STEP) {
+    uint32_t* g = k_at(i);
+    if (i != tid) {
+      ka = g[0];
+      kb = g[HALF / 2];
+    }
+    T* a = reinterpret_cast<T*>(&ka);
+    T* b = reinterpret_cast<T*>(&kb);
+    const int j0 = i % (HALF / 2) * 2;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const double u = static_cast<double>(Cvt<T>::to_f(a[j])), w = static_cast<double>(Cvt<T>::to_f(b[j]));
+      a[j] = Cvt<T>::from_f(static_cast<float>(u * cs[j0 + j] - w * sn[j0 + j]));
+      b[j] = Cvt<T>::from_f(static_cast<float>(w * cs[j0 + j] + u * sn[j0 + j]));
+    }
+    g[0] = ka;
+    g[HALF / 2] = kb;
+    uint32_t* sk = reinterpret_cast<uint32_t*>(krow + i / (HALF / 2) * D + j0);
+    sk[0] = ka;
+    sk[HALF / 2] = kb;
+  }
+  for (int i = tid; i < nq; i += STEP) {
+    uint4* g = q_at(i);
+    if (i != tid) {
+      qa = g[0];
+      qb = g[HALF / 8];
+    }
+    T* a = reinterpret_cast<T*>(&qa);
+    T* b = reinterpret_cast<T*>(&qb);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float u = Cvt<T>::to_f(a[j]), w = Cvt<T>::to_f(b[j]), c = csf[j * JG + i % JG], s = snf[j * JG + i % JG];
+      a[j] = Cvt<T>::from_f(u * c - w * s);
+      b[j] = Cvt<T>::from_f(w * c + u * s);
+    }
+    g[0] = qa;
+    g[HALF / 8] = qb;
+  }
+  if (sl < 0) return;  // rotate only
+  if (sl >= num_slots) {
+    if (tid == 0 && status) atomicCAS(status, 0, ERR_BAD_INDEX);
+    return;
+  }
+  __syncthreads();
+  uint8_t* dst = pages + ((sl / page * 2 * hkv + k0) * page + sl % page) * static_cast<size_t>(RB);
+  for (int i = tid; i < 2 * nw; i += STEP) {
+    const int kv = i >= nw, j = kv ? i - nw : i, h = j / CPR;
+    const uint4 x = kv ? (i == tid ? v : reinterpret_cast<const uint4*>(vsrc)[j]) : reinterpret_cast<const uint4*>(krow)[j];
+    kv4_store8<T>(x, dst + (static_cast<size_t>(kv * hkv) + h) * page * RB, j % CPR, D / 2);
+  }
+}
+
 // ------------------------------------------------------------------ read back
-// Values of the rows at slot[t]: k, v [T, hkv, d]. A thread expands one code word (8 channels, 16 bytes out).
-// Bound by the bytes written, 3.2 times those read. Negative slots read as zeros.
+// Values of the rows at slot[t]: k, v [T, hkv, d]. A thread expands one code word (8 channels, 16 bytes out) of
+// KV4_READ_TOKENS tokens, whose loads it issues together; which word that is costs its divisions once. Bound by the
+// bytes: those written are 3.2 times those read. Negative slots read as zeros.
+constexpr int KV4_READ_TOKENS = 4;
+
 template <typename T>
 __global__ void __launch_bounds__(256)
 kv4_read_kernel(const uint8_t* __restrict__ pages, const int* __restrict__ slot, T* __restrict__ k, T* __restrict__ v,
-                long long items, int hkv, int d, int page, long long num_slots, int* status) {
-  const long long i = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x;
-  if (i >= items) return;
-  const int cpr = d / 8, per_token = 2 * hkv * cpr;
-  const long long t = i / per_token;
-  const int rem = static_cast<int>(i % per_token);
-  const int kv = rem / (hkv * cpr), h = rem / cpr % hkv, chunk = rem % cpr;
-  const long long sl = slot[t];
-  uint32_t out[4] = {0u, 0u, 0u, 0u};
-  if (sl >= num_slots) {
-    if (status) atomicCAS(status, 0, ERR_BAD_INDEX);
-  } else if (sl >= 0) {
-    const uint8_t* row = pages + (((sl / page * 2 + kv) * hkv + h) * page + sl % page) * static_cast<size_t>(kv4_row_bytes(d));
-    const uint32_t w = reinterpret_cast<const uint32_t*>(row)[chunk];
-    const uint32_t meta = reinterpret_cast<const uint32_t*>(row + d / 2)[chunk >> 2];
-    Kv4Type<T>::expand4(w, __byte_perm(meta, meta, 0x3232), __byte_perm(meta, meta, 0x1010), out);
+                int tokens, int hkv, int d, int page, long long num_slots, int* status) {
+  const int cpr = d / 8;
+  const int i = blockIdx.y * 256 + threadIdx.x;
+  if (i >= 2 * hkv * cpr) return;
+  const int kv = i / (hkv * cpr), h = i / cpr % hkv, chunk = i % cpr;
+  const int t0 = blockIdx.x * KV4_READ_TOKENS;
+  const size_t rb = kv4_row_bytes(d);
+  uint32_t w[KV4_READ_TOKENS], meta[KV4_READ_TOKENS];
+#pragma unroll
+  for (int x = 0; x < KV4_READ_TOKENS; ++x) {
+    w[x] = meta[x] = 0u;
+    const int sl = t0 + x < tokens ? slot[t0 + x] : -1;
+    if (sl >= num_slots) {
+      if (status) atomicCAS(status, 0, ERR_BAD_INDEX);
+    } else if (sl >= 0) {
+      const uint8_t* row = pages + ((static_cast<size_t>(sl / page * 2 + kv) * hkv + h) * page + sl % page) * rb;
+      w[x] = reinterpret_cast<const uint32_t*>(row)[chunk];
+      meta[x] = reinterpret_cast<const uint32_t*>(row + d / 2)[chunk >> 2];
+    }
   }
-  T* dst = (kv ? v : k) + (t * hkv + h) * static_cast<size_t>(d) + chunk * 8;
-  *reinterpret_cast<uint4*>(dst) = make_uint4(out[0], out[1], out[2], out[3]);
+  T* dst = (kv ? v : k) + (static_cast<size_t>(t0) * hkv + h) * d + chunk * 8;
+#pragma unroll
+  for (int x = 0; x < KV4_READ_TOKENS; ++x) {
+    if (t0 + x >= tokens) return;
+    uint32_t out[4];
+    Kv4Type<T>::expand4(w[x], __byte_perm(meta[x], meta[x], 0x3232), __byte_perm(meta[x], meta[x], 0x1010), out);
+    *reinterpret_cast<uint4*>(dst + static_cast<size_t>(x) * hkv * d) = make_uint4(out[0], out[1], out[2], out[3]);
+  }
 }
 
 // ------------------------------------------------------------------ generic attention
@@ -277,15 +428,20 @@ MLCB_API int mlcb_kv4_append(void* qkv, void* pages, const int* pos, const int* 
   auto bytes = [&] { return static_cast<size_t>(rot_dim) * 8 + static_cast<size_t>((hkv + parts - 1) / parts) * d * 2; };
   while (bytes() > 48 * 1024) parts *= 2;  // more kv heads than fit: ends at one head, under 3 KB
   const size_t smem = bytes();
-  dim3 grid(tokens, parts);
-  if (dtype == 0)
-    kv4_append_kernel<__half><<<grid, KV4_APPEND_THREADS, smem, stream>>>(
-        static_cast<__half*>(qkv), static_cast<uint8_t*>(pages), pos, slot, inv_freq, hq, hkv, d, rot_dim, page,
-        attn_factor, num_slots, status);
-  else
-    kv4_append_kernel<__nv_bfloat16><<<grid, KV4_APPEND_THREADS, smem, stream>>>(
-        static_cast<__nv_bfloat16*>(qkv), static_cast<uint8_t*>(pages), pos, slot, inv_freq, hq, hkv, d, rot_dim, page,
-        attn_factor, num_slots, status);
+  const dim3 grid(tokens, parts);
+  auto run = [&](auto* rows) {
+    using T = std::remove_pointer_t<decltype(rows)>;
+    uint8_t* dst = static_cast<uint8_t*>(pages);
+    if (rot_dim == d && (d == 64 || d == 128 || d == 256)) {
+      auto kern = d == 64 ? kv4_append_whole_kernel<T, 64> : d == 128 ? kv4_append_whole_kernel<T, 128> : kv4_append_whole_kernel<T, 256>;
+      kern<<<grid, KV4_APPEND_THREADS, smem, stream>>>(rows, dst, pos, slot, inv_freq, hq, hkv, page, attn_factor, num_slots, status);
+    } else {
+      kv4_append_kernel<T><<<grid, KV4_APPEND_THREADS, smem, stream>>>(rows, dst, pos, slot, inv_freq, hq, hkv, d, rot_dim, page,
+                                                                       attn_factor, num_slots, status);
+    }
+  };
+  if (dtype == 0) run(static_cast<__half*>(qkv));
+  else run(static_cast<__nv_bfloat16*>(qkv));
   count_launch();
   return static_cast<int>(cudaGetLastError());
 }
@@ -296,17 +452,15 @@ MLCB_API int mlcb_kv4_read(const void* pages, const int* slot, void* k, void* v,
   if (hkv <= 0 || d <= 0 || d % 32 || d > 256 || page <= 0) return -1;
   if ((reinterpret_cast<uintptr_t>(pages) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15) return -2;
   if (dtype != 0 && dtype != 1) return -3;
-  const long long items = static_cast<long long>(tokens) * 2 * hkv * (d / 8);
-  const long long blocks = (items + 255) / 256;
-  if (blocks > 0x7fffffffLL) return -4;
+  const dim3 grid((tokens + KV4_READ_TOKENS - 1) / KV4_READ_TOKENS, (2 * hkv * (d / 8) + 255) / 256);
+  if (grid.y > 65535) return -4;
   if (dtype == 0)
-    kv4_read_kernel<__half><<<static_cast<unsigned>(blocks), 256, 0, stream>>>(
-        static_cast<const uint8_t*>(pages), slot, static_cast<__half*>(k), static_cast<__half*>(v), items, hkv, d, page,
-        num_slots, status);
+    kv4_read_kernel<__half><<<grid, 256, 0, stream>>>(static_cast<const uint8_t*>(pages), slot, static_cast<__half*>(k),
+                                                      static_cast<__half*>(v), tokens, hkv, d, page, num_slots, status);
   else
-    kv4_read_kernel<__nv_bfloat16><<<static_cast<unsigned>(blocks), 256, 0, stream>>>(
-        static_cast<const uint8_t*>(pages), slot, static_cast<__nv_bfloat16*>(k), static_cast<__nv_bfloat16*>(v), items,
-        hkv, d, page, num_slots, status);
+    kv4_read_kernel<__nv_bfloat16><<<grid, 256, 0, stream>>>(static_cast<const uint8_t*>(pages), slot,
+                                                             static_cast<__nv_bfloat16*>(k), static_cast<__nv_bfloat16*>(v),
+                                                             tokens, hkv, d, page, num_slots, status);
   count_launch();
   return static_cast<int>(cudaGetLastError());
 }

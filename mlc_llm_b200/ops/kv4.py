@@ -25,13 +25,39 @@ import numpy as np
 import torch
 
 from . import reference as ref
-from ._lib import DTYPE_CODE, check, lib, ptr, status_word, stream_ptr
+from ._lib import DTYPE_CODE, check, lib, status_word
 from .attention import AttentionPlan, build_tiles, sm_count
 from .reference import KV4_BOUND, KV4_GROUP, is_kv4, kv4_row
 
-c_int = ctypes.c_int
-c_ll = ctypes.c_longlong
-c_float = ctypes.c_float
+_P, _I, _L, _F = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_float
+_ARGS = {
+    "mlcb_kv4_append": [_P] * 5 + [_I] * 6 + [_F, _L, _I, _P, _P],
+    "mlcb_kv4_read": [_P] * 4 + [_I] * 4 + [_L, _I, _P, _P],
+    "mlcb_kv4_decode": [_P] * 10 + [_I, _I, _L, _I, _I, _I, _L, _F, _I, _I] + [_P] * 7 + [_I, _F],
+    "mlcb_kv4_prefill": [_P] * 10 + [_I, _I, _L, _I, _I, _I, _L, _F, _I, _I] + [_P] * 6 + [_I, _F],
+    "mlcb_kv4_attn_simt": [_P] * 10 + [_I, _L, _I, _I, _I, _I, _L, _I, _F, _F, _I, _P, _P],
+}
+_FN = {}
+
+
+def _call(name: str, *args) -> None:
+    """A kernel entry point with declared argument types: plain numbers and addresses (``None``: null) go in unwrapped,
+    which takes a fifth of the time of a wrapper object per argument."""
+    fn = _FN.get(name)
+    if fn is None:
+        fn = getattr(lib(), name)
+        fn.argtypes = _ARGS[name]
+        _FN[name] = fn
+    check(fn(*args), name)
+
+
+def _at(t: Optional[torch.Tensor]) -> Optional[int]:
+    return None if t is None else t.data_ptr()
+
+
+def _env(device: torch.device):
+    """Status word and current stream of a device."""
+    return status_word(device).data_ptr(), torch._C._cuda_getCurrentRawStream(device.index)  # pylint: disable=protected-access
 
 
 def kv4_cache(num_pages: int, hkv: int, d: int, page: int = 16, dtype: torch.dtype = torch.float16,
@@ -44,29 +70,25 @@ def kv4_cache(num_pages: int, hkv: int, d: int, page: int = 16, dtype: torch.dty
 
 def _guard(device: torch.device):
     """Launches go to the tensors' device, whichever is current."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(device)
+    return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 def _check_cache(kv_pages: torch.Tensor, d: int, what: str) -> None:
-    if kv_pages.dim() != 5 or kv_pages.shape[1] != 2 or not is_kv4(kv_pages, d):
-        raise ValueError(f"{what}: not a 4-bit cache of head size {d}: {tuple(kv_pages.shape)} {kv_pages.dtype}")
+    shape = kv_pages.shape
+    if len(shape) != 5 or shape[1] != 2 or not is_kv4(kv_pages, d):
+        raise ValueError(f"{what}: not a 4-bit cache of head size {d}: {tuple(shape)} {kv_pages.dtype}")
     if not kv_pages.is_contiguous():
         raise ValueError(f"{what}: the cache must be contiguous")
-    if kv_pages.is_cuda and (kv_pages.dtype not in (torch.float16, torch.bfloat16) or d > 256):
+    if kv_pages.is_cuda and (kv_pages.dtype == torch.float32 or d > 256):
         raise ValueError(f"{what}: on a GPU a 4-bit cache holds fp16 or bf16 rows of at most 256 channels, got "
                          f"{kv_pages.dtype} and {d}")
 
 
-def _check_index(t: Optional[torch.Tensor], n: Optional[int], like: torch.Tensor, what: str,
-                 dtype: torch.dtype = torch.int32) -> None:
-    if t is None:
-        return
-    if t.dtype != dtype or t.dim() != 1 or t.device != like.device or not t.is_contiguous() \
-            or (n is not None and t.shape[0] < n):
-        raise ValueError(f"{what} must be a contiguous {dtype} vector on {like.device}"
-                         + (f" of at least {n} entries" if n is not None else "") + f", got {t.dtype} {tuple(t.shape)}")
+def _check_index(t: Optional[torch.Tensor], n: int, where: int, what: str, dtype: torch.dtype = torch.int32) -> None:
+    if t is not None and (t.dtype != dtype or t.get_device() != where or t.dim() != 1 or t.shape[0] < n
+                          or not t.is_contiguous()):
+        raise ValueError(f"{what} must be a contiguous {dtype} vector of at least {n} entries on the cache's device, got "
+                         f"{t.dtype} {tuple(t.shape)} on {t.device}")
 
 
 def append(qkv: torch.Tensor, kv_pages: torch.Tensor, pos: torch.Tensor, slot: torch.Tensor,
@@ -91,24 +113,23 @@ def append(qkv: torch.Tensor, kv_pages: torch.Tensor, pos: torch.Tensor, slot: t
     if rot_dim and (inv_freq.dtype != torch.float32 or inv_freq.numel() < rot_dim // 2 or not inv_freq.is_contiguous()
                     or inv_freq.device != qkv.device):
         raise ValueError(f"rope_append: {rot_dim // 2} fp32 frequencies on {qkv.device} expected")
-    _check_index(pos if rot_dim else None, t, qkv, "rope_append: positions")
-    _check_index(slot, t, qkv, "rope_append: slots")
+    where = qkv.get_device()
+    if rot_dim:
+        _check_index(pos, t, where, "rope_append: positions")
+    _check_index(slot, t, where, "rope_append: slots")
     if not qkv.is_cuda:
         ref.rope_append(qkv, kv_pages, pos, slot, inv_freq, hq, hkv, d, rot_dim, page, attn_factor)
         return
     with _guard(qkv.device):
-        rc = lib().mlcb_kv4_append(ptr(qkv), ptr(kv_pages), ptr(pos), ptr(slot), ptr(inv_freq), c_int(t), c_int(hq),
-                                   c_int(hkv), c_int(d), c_int(rot_dim), c_int(page), c_float(attn_factor),
-                                   c_ll(kv_pages.shape[0] * page), c_int(DTYPE_CODE[qkv.dtype]),
-                                   ptr(status_word(qkv.device)), stream_ptr())
-        check(rc, "mlcb_kv4_append")
+        _call("mlcb_kv4_append", qkv.data_ptr(), kv_pages.data_ptr(), _at(pos), slot.data_ptr(), _at(inv_freq), t, hq, hkv, d,
+              rot_dim, page, attn_factor, kv_pages.shape[0] * page, DTYPE_CODE[qkv.dtype], *_env(qkv.device))
 
 
 def kv4_read(kv_pages: torch.Tensor, slot: torch.Tensor, d: int) -> Tuple[torch.Tensor, torch.Tensor]:
     """The values that the rows at ``slot`` (int32 ``[T]``) of one layer's packed cache stand for: ``k, v [T, hkv, d]``
     in the cache's type. A negative slot reads as zeros."""
     _check_cache(kv_pages, d, "kv4_read")
-    _check_index(slot, None, kv_pages, "kv4_read: slots")
+    _check_index(slot, 0, kv_pages.get_device(), "kv4_read: slots")
     pages, _, hkv, page, _ = kv_pages.shape
     t = slot.shape[0]
     if not kv_pages.is_cuda:
@@ -116,9 +137,8 @@ def kv4_read(kv_pages: torch.Tensor, slot: torch.Tensor, d: int) -> Tuple[torch.
     k = torch.empty(t, hkv, d, dtype=kv_pages.dtype, device=kv_pages.device)
     v = torch.empty_like(k)
     with _guard(kv_pages.device):
-        rc = lib().mlcb_kv4_read(ptr(kv_pages), ptr(slot), ptr(k), ptr(v), c_int(t), c_int(hkv), c_int(d), c_int(page),
-                                 c_ll(pages * page), c_int(DTYPE_CODE[k.dtype]), ptr(status_word(k.device)), stream_ptr())
-        check(rc, "mlcb_kv4_read")
+        _call("mlcb_kv4_read", kv_pages.data_ptr(), slot.data_ptr(), k.data_ptr(), v.data_ptr(), t, hkv, d, page,
+              pages * page, DTYPE_CODE[k.dtype], *_env(k.device))
     return k, v
 
 
@@ -161,12 +181,13 @@ def attend(q: torch.Tensor, kv_pages: torch.Tensor, q_seq: torch.Tensor, q_kvlen
         raise ValueError(f"paged_attention: q is {q.dtype} on {q.device}, the cache {kv_pages.dtype} on {kv_pages.device}")
     if q.dim() != 2 or q.shape[1] != hq * d or (t and (q.stride(1) != 1 or (t > 1 and q.stride(0) < hq * d))):
         raise ValueError(f"paged_attention: q must be [T, {hq * d}] with contiguous rows, got {tuple(q.shape)} {q.stride()}")
-    _check_index(q_seq, t, q, "paged_attention: q_seq")
-    _check_index(q_kvlen, t, q, "paged_attention: q_kvlen")
-    _check_index(q_kvstart, t, q, "paged_attention: q_kvstart")
-    _check_index(page_indptr, None, q, "paged_attention: page_indptr")
-    _check_index(page_indices, None, q, "paged_attention: page_indices")
-    _check_index(tree_mask, t, q, "paged_attention: tree_mask", torch.int64)
+    where = q.get_device()
+    _check_index(q_seq, t, where, "paged_attention: q_seq")
+    _check_index(q_kvlen, t, where, "paged_attention: q_kvlen")
+    _check_index(q_kvstart, t, where, "paged_attention: q_kvstart")
+    _check_index(page_indptr, 2 if t else 0, where, "paged_attention: page_indptr")
+    _check_index(page_indices, 0, where, "paged_attention: page_indices")
+    _check_index(tree_mask, t, where, "paged_attention: tree_mask", torch.int64)
     if not q.is_cuda:
         res = ref.paged_attention(q.reshape(t, hq, d), kv_pages, q_seq, q_kvlen, page_indptr, page_indices, hq, hkv, d,
                                   page, sm_scale, q_kvstart, sink, tree_mask, softcap, return_lse)
@@ -184,15 +205,14 @@ def _decode(q, kv_pages, out, lse, q_kvlen, page_indptr, page_indices, hq, hkv, 
     # with one token per item the rows are the group's heads, whatever the plan was made for
     rows = hq // hkv if q.shape[0] == plan.num_dec else min(16, plan.dec_rows)
     ctas = _decode_ctas(plan.num_dec, rows, hkv, plan.max_pages, q.device)
-    part = torch.empty(ctas * (2 * 16 * (d + 2) + 4), dtype=torch.float32, device=q.device)
-    part_unit, part_ml, part_o = part[: 4 * ctas], part[4 * ctas: 68 * ctas], part[68 * ctas:]
-    rc = lib().mlcb_kv4_decode(ptr(q), ptr(kv_pages), ptr(out), ptr(lse), ptr(plan.dec_seq), ptr(plan.dec_qstart),
-                               ptr(plan.dec_ntok), ptr(q_kvlen), ptr(page_indptr), ptr(page_indices), c_int(plan.num_dec),
-                               c_int(rows), c_ll(q.stride(0)), c_int(hq), c_int(hkv), c_int(d), c_ll(kv_pages.shape[0]),
-                               c_float(sm_scale), c_int(DTYPE_CODE[q.dtype]), c_int(ctas), ptr(part_o), ptr(part_ml),
-                               ptr(part_unit), ptr(status_word(q.device)), stream_ptr(), ptr(q_kvstart), ptr(tree_mask),
-                               c_int(sink), c_float(softcap))
-    check(rc, "mlcb_kv4_decode")
+    # per CTA: a unit descriptor, (max, sum) of two pieces of 16 rows, and their rows
+    scratch = torch.empty(ctas * (2 * 16 * (d + 2) + 4), dtype=torch.float32, device=q.device)
+    part = scratch.data_ptr()
+    _call("mlcb_kv4_decode", q.data_ptr(), kv_pages.data_ptr(), out.data_ptr(), _at(lse), plan.dec_seq.data_ptr(),
+          plan.dec_qstart.data_ptr(), plan.dec_ntok.data_ptr(), q_kvlen.data_ptr(), page_indptr.data_ptr(),
+          page_indices.data_ptr(), plan.num_dec, rows, q.stride(0), hq, hkv, d, kv_pages.shape[0], sm_scale,
+          DTYPE_CODE[q.dtype], ctas, part + ctas * 272, part + ctas * 16, part, *_env(q.device), _at(q_kvstart),
+          _at(tree_mask), sink, softcap)
 
 
 def _prefill_splits(ctas: int, blocks: int, device: torch.device) -> int:
@@ -210,16 +230,15 @@ def _prefill(q, kv_pages, out, lse, q_kvlen, page_indptr, page_indices, hq, hkv,
     ctas = num * hkv * (2 if d == 256 and rows > 128 else 1)
     splits = _prefill_splits(ctas, plan.max_pages // (4 if d == 256 else 8), q.device)
     part_o = part_ml = None
-    if splits > 1:
-        part = torch.empty(num * hkv * splits * 256 * (d + 2), dtype=torch.float32, device=q.device)
-        part_ml, part_o = part[: num * hkv * splits * 512], part[num * hkv * splits * 512:]
-    rc = lib().mlcb_kv4_prefill(ptr(q), ptr(kv_pages), ptr(out), ptr(lse), ptr(seq), ptr(qstart), ptr(ntok), ptr(q_kvlen),
-                                ptr(page_indptr), ptr(page_indices), c_int(num), c_int(rows), c_ll(q.stride(0)), c_int(hq),
-                                c_int(hkv), c_int(d), c_ll(kv_pages.shape[0]), c_float(sm_scale),
-                                c_int(DTYPE_CODE[q.dtype]), c_int(splits), ptr(part_o), ptr(part_ml),
-                                ptr(status_word(q.device)), stream_ptr(), ptr(q_kvstart), ptr(tree_mask), c_int(sink),
-                                c_float(softcap))
-    check(rc, "mlcb_kv4_prefill")
+    if splits > 1:  # 256 rows and their (max, sum) per (tile, kv head, split)
+        blocks = num * hkv * splits
+        scratch = torch.empty(blocks * 256 * (d + 2), dtype=torch.float32, device=q.device)
+        part_ml = scratch.data_ptr()
+        part_o = part_ml + blocks * 2048
+    _call("mlcb_kv4_prefill", q.data_ptr(), kv_pages.data_ptr(), out.data_ptr(), _at(lse), seq.data_ptr(), qstart.data_ptr(),
+          ntok.data_ptr(), q_kvlen.data_ptr(), page_indptr.data_ptr(), page_indices.data_ptr(), num, rows, q.stride(0), hq,
+          hkv, d, kv_pages.shape[0], sm_scale, DTYPE_CODE[q.dtype], splits, part_o, part_ml, *_env(q.device),
+          _at(q_kvstart), _at(tree_mask), sink, softcap)
 
 
 def _launch(q, kv_pages, out, lse, q_seq, q_kvlen, page_indptr, page_indices, hq, hkv, d, page, sm_scale, q_kvstart, sink,
@@ -238,12 +257,9 @@ def _launch(q, kv_pages, out, lse, q_seq, q_kvlen, page_indptr, page_indices, hq
         if plan.num_tiles:
             _prefill(*args, decode_items=False)
         return
-    rc = lib().mlcb_kv4_attn_simt(ptr(q), ptr(kv_pages), ptr(out), ptr(lse), ptr(q_seq), ptr(q_kvlen), ptr(q_kvstart),
-                                  ptr(tree_mask), ptr(page_indptr), ptr(page_indices), c_int(t), c_ll(q.stride(0)),
-                                  c_int(hq), c_int(hkv), c_int(d), c_int(page), c_ll(kv_pages.shape[0]), c_int(sink),
-                                  c_float(sm_scale), c_float(softcap), c_int(DTYPE_CODE[q.dtype]),
-                                  ptr(status_word(q.device)), stream_ptr())
-    check(rc, "mlcb_kv4_attn_simt")
+    _call("mlcb_kv4_attn_simt", q.data_ptr(), kv_pages.data_ptr(), out.data_ptr(), _at(lse), q_seq.data_ptr(),
+          q_kvlen.data_ptr(), _at(q_kvstart), _at(tree_mask), page_indptr.data_ptr(), page_indices.data_ptr(), t, q.stride(0),
+          hq, hkv, d, page, kv_pages.shape[0], sink, sm_scale, softcap, DTYPE_CODE[q.dtype], *_env(q.device))
 
 
 __all__ = ["KV4_BOUND", "KV4_GROUP", "is_kv4", "kv4_cache", "kv4_plan", "kv4_read", "kv4_row"]

@@ -155,7 +155,8 @@ def kv4_row(d: int, dtype: torch.dtype) -> int:
 
 def is_kv4(kv_pages: torch.Tensor, d: int) -> bool:
     """Whether a cache for heads of ``d`` holds packed rows (a packed row is shorter than ``d`` elements)."""
-    return kv_pages.dtype in KV4_BOUND and d > 0 and d % KV4_GROUP == 0 and kv_pages.shape[-1] == kv4_row(d, kv_pages.dtype)
+    row = kv_pages.shape[-1]
+    return row < d and d % KV4_GROUP == 0 and kv_pages.dtype in KV4_BOUND and row == kv4_row(d, kv_pages.dtype)
 
 
 def kv4_pack(x: torch.Tensor) -> torch.Tensor:
