@@ -12,7 +12,7 @@ from ..interface.serve import serve
 
 @dataclasses.dataclass
 class EngineConfigOverride:  # pylint: disable=too-many-instance-attributes
-    """``--overrides "key=value;key=value"`` for the numeric engine options."""
+    """``--overrides "key=value;key=value"`` for the numeric engine options (and ``opt``, ``kv_cache_dtype``)."""
 
     max_num_sequence: Optional[int] = None
     max_total_seq_length: Optional[int] = None
@@ -28,6 +28,7 @@ class EngineConfigOverride:  # pylint: disable=too-many-instance-attributes
     tensor_parallel_shards: Optional[int] = None
     pipeline_parallel_stages: Optional[int] = None
     opt: Optional[str] = None
+    kv_cache_dtype: Optional[str] = None
 
     @staticmethod
     def from_str(source: str) -> "EngineConfigOverride":
@@ -41,7 +42,9 @@ class EngineConfigOverride:  # pylint: disable=too-many-instance-attributes
             key = aliases.get(key, key)
             if key not in fields:
                 raise argparse.ArgumentTypeError(f"unknown engine override {key!r}")
-            if key == "opt":
+            if key == "kv_cache_dtype" and value not in ("auto", "int4"):
+                raise argparse.ArgumentTypeError(f"kv_cache_dtype is auto or int4, not {value!r}")
+            if key in ("opt", "kv_cache_dtype"):
                 setattr(out, key, value)
             elif key == "gpu_memory_utilization":
                 setattr(out, key, float(value))
@@ -98,6 +101,7 @@ def main(argv=None) -> None:
           speculative_mode=args.speculative_mode, spec_draft_length=ov.spec_draft_length,
           spec_tree_width=ov.spec_tree_width, prefix_cache_mode=args.prefix_cache_mode,
           prefix_cache_max_num_recycling_seqs=ov.prefix_cache_max_num_recycling_seqs,
+          kv_cache_dtype=ov.kv_cache_dtype or "auto",
           prefill_mode=args.prefill_mode, enable_tracing=args.enable_tracing, host=args.host, port=args.port,
           allow_credentials=args.allow_credentials, allow_origins=args.allow_origins,
           allow_methods=args.allow_methods, allow_headers=args.allow_headers, api_key=args.api_key)

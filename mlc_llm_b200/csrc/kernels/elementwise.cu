@@ -368,9 +368,15 @@ __global__ void kv_slot_copy_kernel(const uint8_t* __restrict__ src, uint8_t* __
                     static_cast<size_t>(ss % page) * row_bytes;
   const size_t dof = l * dst_layer_stride + ((static_cast<size_t>(ds / page) * 2 + kv) * hkv + h) * head_bytes +
                      static_cast<size_t>(ds % page) * row_bytes;
-  const uint4* sp = reinterpret_cast<const uint4*>(src + so);
-  uint4* dp = reinterpret_cast<uint4*>(dst + dof);
-  for (int v = lane; v < row_bytes / 16; v += 32) dp[v] = sp[v];
+  if (row_bytes % 16 == 0) {
+    const uint4* sp = reinterpret_cast<const uint4*>(src + so);
+    uint4* dp = reinterpret_cast<uint4*>(dst + dof);
+    for (int v = lane; v < row_bytes / 16; v += 32) dp[v] = sp[v];
+  } else {  // packed 4-bit rows of head sizes below 128
+    const uint32_t* sp = reinterpret_cast<const uint32_t*>(src + so);
+    uint32_t* dp = reinterpret_cast<uint32_t*>(dst + dof);
+    for (int v = lane; v < row_bytes / 4; v += 32) dp[v] = sp[v];
+  }
 }
 
 // One decode token of the gated delta rule (Qwen3.5 linear-attention layers; reference:
@@ -524,7 +530,7 @@ MLCB_API int mlcb_enable_peer_access(int device, int peer) {
   return static_cast<int>(err);
 }
 
-// Strides in bytes; row_bytes = head_dim * element size (multiple of 16). Slots must lie in
+// Strides in bytes; row_bytes = bytes of one head's row (multiple of 4). Slots must lie in
 // [0, src_pages * page) and [0, dst_pages * page): the host checks before the launch and the kernel
 // skips (and reports ERR_BAD_INDEX for) any row that is not.
 MLCB_API int mlcb_kv_slot_copy(const void* src, void* dst, const int* src_slots, const int* dst_slots, int n,
@@ -532,7 +538,7 @@ MLCB_API int mlcb_kv_slot_copy(const void* src, void* dst, const int* src_slots,
                                int page, int row_bytes, int src_pages, int dst_pages, int* status,
                                cudaStream_t stream) {
   if (n <= 0) return 0;
-  if (row_bytes % 16 || page <= 0 || src_pages <= 0 || dst_pages <= 0) return -1;
+  if (row_bytes % 4 || page <= 0 || src_pages <= 0 || dst_pages <= 0) return -1;
   if (static_cast<long long>(src_pages) * page > 0x7fffffffLL || static_cast<long long>(dst_pages) * page > 0x7fffffffLL)
     return -1;
   const long long warps = static_cast<long long>(n) * layers * 2 * hkv;

@@ -507,6 +507,7 @@ PYBIND11_MODULE(_core, m) {
           mi.max_batch_size = geti("max_batch_size", 128);
           mi.pipeline_parallel_stages = static_cast<int>(geti("pipeline_parallel_stages", 1));
           mi.kv_bytes_per_element = static_cast<int>(geti("kv_bytes_per_element", 2));
+          mi.kv_row_bytes = geti("kv_row_bytes", 0);
           mi.rnn_state_bytes_per_sequence = geti("rnn_state_bytes_per_sequence", 0);
           mi.hidden_size = geti("hidden_size", 0);
           infos.push_back(mi);

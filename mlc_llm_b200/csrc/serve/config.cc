@@ -208,6 +208,9 @@ EngineConfig EngineConfig::FromJSON(const std::string& json_str) {
     throw std::runtime_error("gpu_memory_utilization must be in (0, 1]");
   c.kv_cache_page_size = json::get_or<int>(o, "kv_cache_page_size", 16);
   if (c.kv_cache_page_size != 16) throw std::runtime_error("KV cache page size other than 16 is not supported.");
+  c.kv_cache_dtype = json::get_or<std::string>(o, "kv_cache_dtype", "auto");
+  if (c.kv_cache_dtype != "auto" && c.kv_cache_dtype != "int4")
+    throw std::runtime_error("Invalid kv_cache_dtype " + c.kv_cache_dtype + " (auto or int4)");
   c.max_num_sequence = opt_int(o, "max_num_sequence");
   c.max_total_sequence_length = opt_int(o, "max_total_sequence_length");
   c.max_single_sequence_length = opt_int(o, "max_single_sequence_length");
@@ -255,6 +258,7 @@ Value EngineConfig::AsJSON() const {
   o["opt"] = opt;
   o["gpu_memory_utilization"] = gpu_memory_utilization;
   o["kv_cache_page_size"] = kv_cache_page_size;
+  o["kv_cache_dtype"] = kv_cache_dtype;
   o["max_num_sequence"] = max_num_sequence;
   o["max_total_sequence_length"] = max_total_sequence_length;
   o["max_single_sequence_length"] = max_single_sequence_length;
@@ -315,7 +319,8 @@ CapacityResult InferCapacity(const EngineConfig& user, const std::vector<ModelCa
   double kv_bytes_per_token = 0, aux = 0, workspace = 0, logit_ws = 0, params = 0;
   for (auto& m : models) {
     const int64_t layers = m.num_layers / std::max(1, m.pipeline_parallel_stages);
-    kv_bytes_per_token += static_cast<double>(m.head_dim * m.num_kv_heads * layers * 2 * m.kv_bytes_per_element) + 1.25;
+    const int64_t row_bytes = m.kv_row_bytes > 0 ? m.kv_row_bytes : m.head_dim * m.kv_bytes_per_element;
+    kv_bytes_per_token += static_cast<double>(row_bytes * m.num_kv_heads * layers * 2) + 1.25;
     const int64_t hidden = m.head_dim * m.num_qo_heads;
     aux += (c.max_num_sequence + 1) * 88.0 + c.prefill_chunk_size * (m.num_qo_heads + 1) * 8.0 +
            c.prefill_chunk_size * m.head_dim * (m.num_qo_heads + m.num_kv_heads) * 4.0 + 48.0 * 1024 * 1024;

@@ -80,6 +80,7 @@ struct EngineConfig {
   std::string opt;
   double gpu_memory_utilization = 0.85;
   int kv_cache_page_size = 16;
+  std::string kv_cache_dtype = "auto";  // "auto": the model's 16-bit type; "int4": packed 4-bit rows
   int64_t max_num_sequence = -1;
   int64_t max_total_sequence_length = -1;
   int64_t max_single_sequence_length = -1;
@@ -114,6 +115,7 @@ struct ModelCapacityInfo {
   int64_t max_batch_size = 128;
   int pipeline_parallel_stages = 1;
   int kv_bytes_per_element = 2;
+  int64_t kv_row_bytes = 0;         // bytes of one head's K (or V) row where it is not head_dim * kv_bytes_per_element
   // recurrent-state models: bytes of state one sequence holds (all layers), and the hidden size that the
   // workspace estimate needs (these models have no attention heads to derive it from)
   int64_t rnn_state_bytes_per_sequence = 0;

@@ -60,6 +60,7 @@ def serve(  # pylint: disable=too-many-arguments,too-many-locals
     prefix_cache_mode: Literal["disable", "radix"] = "radix",
     prefix_cache_max_num_recycling_seqs: Optional[int] = None,
     prefill_mode: Literal["hybrid", "chunked"] = "hybrid",
+    kv_cache_dtype: Literal["auto", "int4"] = "auto",
     enable_tracing: bool = False,
     host: str = "127.0.0.1",
     port: int = 8000,
@@ -78,7 +79,8 @@ def serve(  # pylint: disable=too-many-arguments,too-many-locals
         max_history_size=max_history_size, gpu_memory_utilization=gpu_memory_utilization,
         speculative_mode=speculative_mode, spec_draft_length=spec_draft_length or 0,
         spec_tree_width=spec_tree_width or 1, prefix_cache_mode=prefix_cache_mode,
-        prefix_cache_max_num_recycling_seqs=prefix_cache_max_num_recycling_seqs, prefill_mode=prefill_mode)
+        prefix_cache_max_num_recycling_seqs=prefix_cache_max_num_recycling_seqs, prefill_mode=prefill_mode,
+        kv_cache_dtype=kv_cache_dtype)
     async_engine = engine.AsyncMLCEngine(model=model, device=device, model_lib=model_lib, mode=mode,
                                          engine_config=cfg, enable_tracing=enable_tracing)
     emb_engine = None

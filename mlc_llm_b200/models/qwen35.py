@@ -146,14 +146,14 @@ class Qwen35Model(DecoderModel):
     # ------------------------------------------------------------------ caches
     def create_kv_cache(self, num_pages: int, page_size: int = 16) -> None:
         self.page = page_size
-        self.kv_pages = torch.zeros(max(1, len(self.attn_layers)), num_pages, 2, self.hkv, page_size, self.d,
+        self.kv_pages = torch.zeros(max(1, len(self.attn_layers)), num_pages, 2, self.hkv, page_size, self.kv_row(),
                                     dtype=self.kv_dtype, device=self.device)
 
     def _kv_layer(self, li: int) -> int:
         return self._kv_of[li]
 
     def kv_bytes_per_token(self) -> int:
-        return 2 * self.hkv * self.d * max(1, len(self.attn_layers)) * (2 if self.kv_dtype != torch.float32 else 4)
+        return 2 * self.hkv * self.kv_row() * max(1, len(self.attn_layers)) * (2 if self.kv_dtype != torch.float32 else 4)
 
     def move_tokens(self, moves: torch.Tensor) -> None:
         if moves.numel():

@@ -81,6 +81,7 @@ class DecoderModel:
         self.last_stage = self.layers.stop == config.num_hidden_layers
         self.kv_pages: Optional[torch.Tensor] = None
         self.page = 16
+        self.kv4 = False  # rows of the KV cache are packed to 4 bits (``use_kv4``)
         self.sm_scale = (config.query_pre_attn_scalar ** -0.5 if config.query_pre_attn_scalar > 0
                          else self.d ** -0.5)
         self.inv_freq = None
@@ -108,6 +109,21 @@ class DecoderModel:
             self.cache_head_dim = (mla["qk_rope_head_dim"] + mla["kv_lora_rank"] + 1) // 2  # K and V halves of a row
 
     # ------------------------------------------------------------------ KV cache
+    def use_kv4(self) -> None:
+        """Hold the KV cache in 4 bits (before :meth:`create_kv_cache`). Raises ``ValueError`` for models whose rows
+        cannot be packed: latent attention, recurrent states, head sizes that are no multiple of 32 (or above 256 on
+        a GPU)."""
+        if self.cfg.extra.get("mla") or self.cfg.extra.get("rwkv") or self.cfg.extra.get("medusa"):
+            raise ValueError(f"a 4-bit KV cache is not available for {self.cfg.model_type} models")
+        if self.device.type == "cuda" and self.d > 256:
+            raise ValueError(f"a 4-bit KV cache holds heads of at most 256 channels, the model has {self.d}")
+        ops.kv4_row(self.d, self.kv_dtype)
+        self.kv4 = True
+
+    def kv_row(self) -> int:
+        """Elements of one head's K or V row in the cache."""
+        return ops.kv4_row(self.d, self.kv_dtype) if self.kv4 else self.d
+
     def create_kv_cache(self, num_pages: int, page_size: int = 16) -> None:
         self.page = page_size
         n = len(self.layers)
@@ -116,7 +132,7 @@ class DecoderModel:
             self.kv_pages = torch.zeros(n, num_pages, 1, 1, page_size, m["qk_rope_head_dim"] + m["kv_lora_rank"],
                                         dtype=self.kv_dtype, device=self.device)
             return
-        self.kv_pages = torch.zeros(n, num_pages, 2, self.hkv, page_size, self.d, dtype=self.kv_dtype,
+        self.kv_pages = torch.zeros(n, num_pages, 2, self.hkv, page_size, self.kv_row(), dtype=self.kv_dtype,
                                     device=self.device)
 
     def _kv_layer(self, li: int) -> int:
@@ -132,7 +148,7 @@ class DecoderModel:
         if self.mla_latent:
             m = self.cfg.extra["mla"]
             return (m["qk_rope_head_dim"] + m["kv_lora_rank"]) * len(self.layers) * es
-        return 2 * self.hkv * self.d * len(self.layers) * es
+        return 2 * self.hkv * self.kv_row() * len(self.layers) * es
 
     def copy_pages(self, pairs: torch.Tensor) -> None:
         """(src, dst) page copies for copy-on-write, applied to every layer."""

@@ -144,6 +144,7 @@ def kv4_read(kv_pages: torch.Tensor, slot: torch.Tensor, d: int) -> Tuple[torch.
 
 # --------------------------------------------------------------------------- attention
 KV4_TILE_ROWS = 256  # query rows that share one expansion of the cached blocks
+KV4_HEAD_DIMS = (64, 96, 128, 256)  # of the tensor-core kernels; other multiples of 32 take the generic one
 
 
 def kv4_plan(q_indptr, q_kvlen: torch.Tensor, page_indptr: torch.Tensor, page_indices: torch.Tensor, hq: int, hkv: int,
@@ -161,10 +162,21 @@ def kv4_plan(q_indptr, q_kvlen: torch.Tensor, page_indptr: torch.Tensor, page_in
                          dec_rows=int(tiles["dec_ntok"].max()) * (hq // hkv) if num_dec else 16)
 
 
-def _decode_ctas(num_items: int, rows: int, hkv: int, max_pages: int, device: torch.device) -> int:
-    """CTAs of the decode kernel: as many as stay resident, but no more than one per four 32-token slots."""
-    slots = num_items * hkv * ((rows + 7) // 8) * max(1, (max_pages + 1) // 2)
-    return max(1, min(4 * sm_count(device), (slots + 3) // 4))
+def _decode_ctas(num_items: int, hkv: int, max_pages: int, device: torch.device) -> int:
+    """CTAs of the decode kernel: no more than one per four 32-token slots, rounded up to a power of two (a captured
+    launch serves every length up to the next one), and no more than can be resident."""
+    slots = num_items * hkv * max(1, (max_pages + 1) // 2)
+    return min(4 * sm_count(device), 1 << max(0, (slots + 3) // 4 - 1).bit_length())
+
+
+def decode_launch(num_dec: int, hkv: int, d: int, max_pages: int, device: torch.device) -> int:
+    """What the launch of ``num_dec`` decode items depends on besides array shapes: a captured graph holds for equal
+    values of this number."""
+    if d not in KV4_HEAD_DIMS:
+        return 0
+    if d == 96:
+        return _prefill_splits(num_dec * hkv, max_pages // 8, device)
+    return _decode_ctas(num_dec, hkv, max_pages, device)
 
 
 def attend(q: torch.Tensor, kv_pages: torch.Tensor, q_seq: torch.Tensor, q_kvlen: torch.Tensor, page_indptr: torch.Tensor,
@@ -204,7 +216,7 @@ def _decode(q, kv_pages, out, lse, q_kvlen, page_indptr, page_indices, hq, hkv, 
             softcap, plan) -> None:
     # with one token per item the rows are the group's heads, whatever the plan was made for
     rows = hq // hkv if q.shape[0] == plan.num_dec else min(16, plan.dec_rows)
-    ctas = _decode_ctas(plan.num_dec, rows, hkv, plan.max_pages, q.device)
+    ctas = _decode_ctas(plan.num_dec, hkv, plan.max_pages, q.device)
     # per CTA: a unit descriptor, (max, sum) of two pieces of 16 rows, and their rows
     scratch = torch.empty(ctas * (2 * 16 * (d + 2) + 4), dtype=torch.float32, device=q.device)
     part = scratch.data_ptr()
@@ -217,8 +229,9 @@ def _decode(q, kv_pages, out, lse, q_kvlen, page_indptr, page_indices, hq, hkv, 
 
 def _prefill_splits(ctas: int, blocks: int, device: torch.device) -> int:
     """KV splits of the prefill kernel (one CTA per SM): few tiles are cut so that they cover the SMs, two blocks of
-    cached positions per split at least."""
-    return max(1, min(sm_count(device) // max(1, ctas), blocks // 2, 64))
+    cached positions per split at least; a power of two, as in :func:`_decode_ctas`."""
+    most = max(1, min(sm_count(device) // max(1, ctas), blocks // 2, 64))
+    return 1 << (most.bit_length() - 1)
 
 
 def _prefill(q, kv_pages, out, lse, q_kvlen, page_indptr, page_indices, hq, hkv, d, sm_scale, q_kvstart, sink, tree_mask,
@@ -245,7 +258,7 @@ def _launch(q, kv_pages, out, lse, q_seq, q_kvlen, page_indptr, page_indices, hq
             tree_mask, softcap, plan) -> None:
     t = q.shape[0]
     aligned = q.data_ptr() % 16 == 0 and (q.stride(0) % 8 == 0 or t == 1)
-    if plan is not None and plan.use_tensor_core and page == 16 and d in (64, 96, 128, 256) and aligned \
+    if plan is not None and plan.use_tensor_core and page == 16 and d in KV4_HEAD_DIMS and aligned \
             and hq // hkv <= plan.tile_rows:
         args = (q, kv_pages, out, lse, q_kvlen, page_indptr, page_indices, hq, hkv, d, sm_scale, q_kvstart, sink, tree_mask,
                 softcap, plan)

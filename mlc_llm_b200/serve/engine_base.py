@@ -332,6 +332,15 @@ class EngineRuntime:
                 cfg.kv_state_kind = "hybrid"
             else:
                 model = DecoderModel(mcfg, quant, store, self.device, comm if tp > 1 else None, layers)
+            if cfg.kv_cache_dtype == "int4":
+                try:
+                    model.use_kv4()
+                except ValueError:
+                    if mi == 0:
+                        raise
+                    # a draft model or head whose rows cannot be packed keeps its own, much smaller cache in 16 bits
+            elif cfg.kv_cache_dtype != "auto":
+                raise ValueError(f"kv_cache_dtype must be auto or int4, got {cfg.kv_cache_dtype!r}")
             if mi == 0 and mcfg.extra.get("vision"):
                 self._attach_vision_tower(model, info, mcfg)
             self.models.append(model)
@@ -344,6 +353,7 @@ class EngineRuntime:
                 "prefill_chunk_size": mcfg.prefill_chunk_size, "max_batch_size": mcfg.max_batch_size,
                 "pipeline_parallel_stages": mcfg.pipeline_parallel_stages,
                 "kv_bytes_per_element": 4 if model.kv_dtype == torch.float32 else 2,
+                "kv_row_bytes": model.kv_row() * model.kv_dtype.itemsize if model.kv4 else 0,
                 "hidden_size": mcfg.hidden_size,
                 "rnn_state_bytes_per_sequence": int(model.state_bytes_per_sequence())
                 if hasattr(model, "state_bytes_per_sequence") else 0,

@@ -375,12 +375,17 @@ class ModelExecutor:
                                         dec_seq=dev["dec_seq"], dec_qstart=dev["dec_qstart"],
                                         dec_ntok=dev["dec_ntok"], num_dec=n_dec,
                                         dec_splits=choose_splits(n_dec, model.hkv, max_pages, self.device)
-                                        if n_dec else 1, max_pages=max_pages)
+                                        if n_dec else 1, max_pages=max_pages, tile_rows=self._tile_rows(model))
         return b
 
     def _tc_attention_ok(self, model: DecoderModel) -> bool:
-        return (self.use_tensor_core_attention and model.d == 128 and model.page == 16
-                and model.kv_dtype in (torch.float16, torch.bfloat16))
+        return (self.use_tensor_core_attention and model.d in (ops.kv4.KV4_HEAD_DIMS if model.kv4 else (128,))
+                and model.page == 16 and model.kv_dtype in (torch.float16, torch.bfloat16))
+
+    @staticmethod
+    def _tile_rows(model: DecoderModel) -> int:
+        """Query rows per tile of the tensor-core prefill kernel of the model's cache."""
+        return ops.kv4.KV4_TILE_ROWS if model.kv4 else 128
 
     @staticmethod
     def _masked_attention(model: DecoderModel) -> bool:
@@ -404,7 +409,7 @@ class ModelExecutor:
         if self._tc_attention_ok(model):
             from ..ops.attention import build_tiles  # pylint: disable=import-outside-toplevel
 
-            arrays.update(build_tiles(arrays["q_indptr"], model.hq // model.hkv))
+            arrays.update(build_tiles(arrays["q_indptr"], model.hq // model.hkv, tile_rows=self._tile_rows(model)))
         if sp is not None:
             for k in _S_INT:
                 arrays["s_" + k] = np.ascontiguousarray(sp[k], dtype=np.int32)
@@ -468,7 +473,9 @@ class ModelExecutor:
 
         model = self.models[model_id]
         max_pages = (int(plan["max_seq_len"]) + 15) // 16
-        splits = choose_splits(int(dev["dec_seq"].numel()), model.hkv, max_pages, self.device)
+        n_dec = int(dev["dec_seq"].numel())
+        splits = ops.kv4.decode_launch(n_dec, model.hkv, model.d, max_pages, self.device) if model.kv4 \
+            else choose_splits(n_dec, model.hkv, max_pages, self.device)
         shape = tuple((k, int(v.numel())) for k, v in dev.items() if not k.startswith("s_") and k != "page_indices")
         key = (model_id, self.staging.generation, splits, shape)
         entry = self._graphs.get(key)
@@ -1185,6 +1192,8 @@ class ModelExecutor:
         ss = torch.from_numpy(src_slots.astype(np.int32)).to(self.device)
         ds = torch.from_numpy(dst_slots.astype(np.int32)).to(self.device)
         es = src.element_size()
+        if src.shape[5] * es % 4:
+            raise kv_handoff.HandoffError(f"KV rows of {src.shape[5] * es} bytes cannot be handed off between GPU engines")
         dst_layer_stride = int(np.prod(dshape[1:], dtype=np.int64))
         rc = lib().mlcb_kv_slot_copy(
             ptr(src), ctypes.c_void_p(dst_ptr), ptr(ss), ptr(ds), ctypes.c_int(len(src_slots)),

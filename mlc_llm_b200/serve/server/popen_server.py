@@ -17,7 +17,8 @@ import requests
 _OVERRIDE_KEYS = {"max_num_sequence", "max_total_sequence_length", "max_single_sequence_length",
                   "prefill_chunk_size", "sliding_window_size", "attention_sink_size", "max_history_size",
                   "gpu_memory_utilization", "spec_draft_length", "spec_tree_width",
-                  "prefix_cache_max_num_recycling_seqs", "tensor_parallel_shards", "pipeline_parallel_stages", "opt"}
+                  "prefix_cache_max_num_recycling_seqs", "tensor_parallel_shards", "pipeline_parallel_stages", "opt",
+                  "kv_cache_dtype"}
 
 
 class PopenServer:  # pylint: disable=too-many-instance-attributes
@@ -63,7 +64,7 @@ class PopenServer:  # pylint: disable=too-many-instance-attributes
                     continue
                 if key in ("speculative_mode", "prefix_cache_mode", "prefill_mode"):
                     cmd += ["--" + key.replace("_", "-"), str(value)]
-                elif key in _OVERRIDE_KEYS:
+                elif key in _OVERRIDE_KEYS and (key, value) != ("kv_cache_dtype", "auto"):
                     overrides.append(f"{key}={value}")
         if self.tensor_parallel_shards is not None:
             overrides.append(f"tensor_parallel_shards={self.tensor_parallel_shards}")
