@@ -8,19 +8,18 @@
 //                 usual orientation, whose M = 16 rows would be mostly padding. Two k-steps cover one quantisation
 //                 group, so K needs no expansion: the fragments hold the integers bias + c that a nibble is
 //                 under a suitable exponent (64 + c in fp16, 128 + c in bf16: one and-or), and the group's step
-//                 multiplies the fp32 result. Bias and minimum are one more k-step: lo_g and s_g against
-//                 sum_g(q) and -bias * sum_g(q), those split into two (bf16: three) terms of the rows' type. K is
-//                 thus never rounded. fp16 queries of 32 and more are first scaled by a power of two, so that the
-//                 sums stay finite.
+//                 multiplies the fp32 result. Bias and minimum are two more k-steps: lo_g and s_g against the group
+//                 sums of q, split into two (bf16: three) terms of the rows' type. K is thus never rounded.
 //   softmax       in the S^T accumulators: a lane has two query rows and 4 tokens of 16. The reference maximum is
 //                 raised only when some score exceeds it by more than 8 (log2), so the usual step has no shuffle
 //                 and no rescaling; P stays below 2^8 and the final division by the row sum makes it exact.
 //   O^T += V^T P^T  M = 16 channels, N = 8 query rows; P^T fragments come from the S^T accumulators by one
 //                 8 x 8 transpose (movmatrix) per 8 tokens. A fragments want pairs of tokens: two tokens' code
-//                 words are interleaved by halves (prmt) and expanded, lo + s c rounded once to the rows' type.
-//                 (The step cannot move to P as it does for K: p * s underflows fp16 for small s.)
+//                 words are interleaved by halves (prmt) and expanded, lo + s c rounded once to fp16. For bf16 rows
+//                 lo and s are first scaled by a power of two that follows the largest of them, so that V and P keep
+//                 11 bits. (The step cannot move to P as it does for K: p * s underflows fp16 for small s.)
 //
-// P is rounded to the rows' type; sums, maxima and accumulators are fp32.
+// P is rounded to fp16; sums, maxima and accumulators are fp32.
 //
 // Work: a unit is one (sequence, kv head, block of 8 or 16 query rows). All units' slots of 32 tokens (two pages),
 // laid end to end, are cut into equal shares, one per persistent CTA, so ragged batches and single long sequences
@@ -45,14 +44,13 @@ struct Kv4DecParams {
   float* lse;
   float* part_o;   // [2 CTAs][16][D] fp32: partial rows of a share's first and last unit
   float* part_ml;  // [2 CTAs][16][2]
-  int* part_unit;  // [CTAs][4]: unit begun here and cut (item or -1, kv head * row blocks + block, pieces)
+  int* part_unit;  // [CTAs][4]: unit begun here and cut: rows (0: none), first token, kv head * 16 + first row, pieces
   const int *item_seq, *item_qstart, *item_ntok, *q_kvlen, *page_indptr, *page_indices;
   const int* q_kvstart;
   const unsigned long long* tree_mask;
   int* status;
   long long q_stride, num_pages;
   int hq, hkv, group, row_blocks, num_items, sink;
-  uint32_t q_flip;           // sign bits of a pair where sm_scale is negative: scale_log2 is its magnitude
   float scale_log2;          // sm_scale * log2(e)
   float cap_k, cap_log2;     // soft cap: scores are kv4_softcap(raw, cap_k, cap_log2); 0 = none
 };
@@ -161,14 +159,12 @@ struct Kv4Bias;
 template <>
 struct Kv4Bias<__half> {
   static constexpr float BIAS = 64.f;
-  static constexpr uint32_t MINUS = 0xd400d400u;  // a pair of -64
-  static constexpr int TERMS = 2;                 // 11 bits each: the group sums to 2^-22
+  static constexpr uint32_t ONES = 0x3c003c00u;
 };
 template <>
 struct Kv4Bias<__nv_bfloat16> {
   static constexpr float BIAS = 128.f;
-  static constexpr uint32_t MINUS = 0xc300c300u;  // a pair of -128
-  static constexpr int TERMS = 3;                 // 8 bits each: 2^-24
+  static constexpr uint32_t ONES = 0x3f803f80u;
 };
 
 // s of a (lo, s) word as fp32
@@ -204,9 +200,13 @@ struct Kv4DecShape {
   static constexpr int SLOT_BYTES = 4 * PAGE_BYTES;            // K, V of two pages
   static constexpr int SLOTS = D == 256 ? 4 : 8;               // a multiple of the four consumer warps
   static constexpr int ROWS = 8 * NT;
-  static constexpr int CTAS = D < 256 && NT == 1 ? 3 : 2;      // resident per SM: what the registers allow
-  static constexpr int Q_BYTES = ROWS * D * 2;                 // query rows of a piece; two pieces are held
-  static constexpr int MERGE_BYTES = 4 * ROWS * (D + 2) * 4;   // four warps' O rows and (m, l) pairs
+  // resident per SM: what the registers allow without spilling much (D = 128, one n-tile: 3 120 us, 4 129 us)
+  static constexpr int CTAS = D == 64 ? (NT == 1 ? 4 : 3) : D == 128 ? (NT == 1 ? 3 : 2) : 2;
+  // Query rows of a piece; two pieces are held. The pitch spreads a fragment's eight rows over the banks.
+  static constexpr int Q_PITCH = D * 2 + 16;
+  static constexpr int Q_BYTES = ROWS * Q_PITCH;
+  // two warps' partial O in fragment order (16 bytes per lane, pair of tiles and column), and their (m, l)
+  static constexpr int MERGE_BYTES = 2 * (ROWS * D * 4 + ROWS * 8);
   static constexpr int OFF_Q = SLOTS * SLOT_BYTES;
   static constexpr int OFF_MERGE = OFF_Q + 2 * Q_BYTES;
   static constexpr int OFF_BAR = OFF_MERGE + MERGE_BYTES;
@@ -221,10 +221,10 @@ __global__ void __launch_bounds__(KV4_DEC_THREADS, Kv4DecShape<D, NT>::CTAS) kv4
   constexpr int ROW = Shape::ROW, PB = Shape::PAGE_BYTES, SLOTS = Shape::SLOTS, ROWS = Shape::ROWS;
   constexpr int GROUPS = D / KV4_GROUP;
   constexpr int VW = D / 64;   // V code words per lane and token
+  constexpr bool BF16 = Kv4Type<T>::IS_BF16;
   pdl_launch_dependents();
   extern __shared__ __align__(128) uint8_t smem[];
-  float* sm_o = reinterpret_cast<float*>(smem + Shape::OFF_MERGE);  // [4][ROWS][D]
-  float* sm_ml = sm_o + 4 * ROWS * D;                               // [4][ROWS][2]
+  uint8_t* merge = smem + Shape::OFF_MERGE;
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + Shape::OFF_BAR);
   uint64_t* empty = full + SLOTS;
   uint64_t* piece_full = empty + SLOTS;   // [2]
@@ -268,7 +268,7 @@ __global__ void __launch_bounds__(KV4_DEC_THREADS, Kv4DecShape<D, NT>::CTAS) kv4
   const long long share = max((total + gridDim.x - 1) / gridDim.x, static_cast<long long>(KV4_DEC_MIN_SHARE));
   const long long begin = blockIdx.x * share, end = min(total, begin + share);
   if (begin >= end) {
-    if (threadIdx.x == 0) p.part_unit[blockIdx.x * 4] = -1;
+    if (threadIdx.x == 0) p.part_unit[blockIdx.x * 4] = 0;
     return;
   }
 
@@ -320,36 +320,38 @@ __global__ void __launch_bounds__(KV4_DEC_THREADS, Kv4DecShape<D, NT>::CTAS) kv4
           // pieces of a unit that begins here and runs on: this share's and those of the CTAs after it
           const long long rest = n - take;
           int* pu = p.part_unit + blockIdx.x * 4;
-          pu[0] = begins && !ends ? item : -1;
-          pu[1] = unit;
-          pu[2] = 1 + static_cast<int>((rest + share - 1) / share);
+          pu[0] = begins && !ends ? max(0, rows) : 0;
+          pu[1] = d.qstart;
+          pu[2] = hk * 16 + row0;
+          pu[3] = 1 + static_cast<int>((rest + share - 1) / share);
         }
         mbar_expect_tx(&piece_full[e], max(0, rows) * D * 2);
       }
       __syncwarp();
-      for (int tok = row0 / p.group + lane; tok * p.group < row0 + rows; tok += 32) {
-        const int r0 = max(row0, tok * p.group), r1 = min(row0 + rows, (tok + 1) * p.group);
+      if (lane < rows) {
+        const int row = row0 + lane;
         const uint8_t* src = reinterpret_cast<const uint8_t*>(p.q) +
-                             (static_cast<size_t>(d.qstart + tok) * p.q_stride +
-                              static_cast<size_t>(hk * p.group + r0 - tok * p.group) * D) * 2;
-        bulk_load(smem + Shape::OFF_Q + e * Shape::Q_BYTES + (r0 - row0) * D * 2, src, (r1 - r0) * D * 2, &piece_full[e]);
+                             (static_cast<size_t>(d.qstart + row / p.group) * p.q_stride +
+                              static_cast<size_t>(hk * p.group + row % p.group) * D) * 2;
+        bulk_load(smem + Shape::OFF_Q + e * Shape::Q_BYTES + lane * Shape::Q_PITCH, src, D * 2, &piece_full[e]);
       }
       ++k;
-      // ---- pages: lane i holds the number of page base + i (one coalesced load per 32); lanes 0..3 issue a slot's
-      // copies (K and V of its two pages)
+      // ---- pages: lane i holds the address of page base + i (one coalesced load of page numbers per 32) and issues
+      // its two copies, K and V, when its slot's turn comes
       const int pg0 = slot0 * 2, pg1 = min(d.npg, (slot0 + take) * 2);
       for (int base = pg0; base < pg1 && ok; base += 32) {
-        int mine = 0;
-        if (base + lane < pg1) {
-          const int li = base + lane;
-          mine = d.list[li < d.sink_pg ? li : li + d.skip];
-          if (mine >= p.num_pages) {
-            if (p.status) atomicCAS(p.status, 0, ERR_BAD_INDEX);
-            mine = 0;
-          }
-          if (mine < 0) mine = 0;  // released by a sliding window: every position of it is masked
-        }
         const int m = min(32, pg1 - base);
+        const uint8_t* src = p.pages;
+        if (lane < m) {
+          const int li = base + lane;
+          int pg = d.list[li < d.sink_pg ? li : li + d.skip];
+          if (pg >= p.num_pages) {
+            if (p.status) atomicCAS(p.status, 0, ERR_BAD_INDEX);
+            pg = 0;
+          }
+          // a negative page was released by a sliding window: every position of it is masked
+          src += (static_cast<size_t>(max(pg, 0)) * 2 * p.hkv + hk) * PB;
+        }
         for (int i = 0; i < m; i += 2, ++g) {
           const int s = g % SLOTS;
           if (g >= SLOTS) {
@@ -357,13 +359,12 @@ __global__ void __launch_bounds__(KV4_DEC_THREADS, Kv4DecShape<D, NT>::CTAS) kv4
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
           }
-          const int here = min(2, m - i);
-          if (lane == 0) mbar_expect_tx(&full[s], here * 2 * PB);
+          if (lane == i) mbar_expect_tx(&full[s], min(2, m - i) * 2 * PB);
           __syncwarp();
-          const int pg = __shfl_sync(0xffffffffu, mine, i + ((lane >> 1) & 1));
-          if (lane < 2 * here) {
-            const size_t block = (static_cast<size_t>(pg) * 2 + (lane & 1)) * p.hkv + hk;
-            bulk_load(smem + s * Shape::SLOT_BYTES + lane * PB, p.pages + block * PB, PB, &full[s]);
+          if ((lane ^ i) < 2 && lane < m) {
+            uint8_t* dst = smem + s * Shape::SLOT_BYTES + (lane & 1) * 2 * PB;
+            bulk_load(dst, src, PB, &full[s]);
+            bulk_load(dst + PB, src + static_cast<size_t>(p.hkv) * PB, PB, &full[s]);
           }
         }
       }
@@ -383,76 +384,55 @@ __global__ void __launch_bounds__(KV4_DEC_THREADS, Kv4DecShape<D, NT>::CTAS) kv4
     // may be <= 0: an empty row block. After a wait that ran out nothing of the piece is touched.
     const int rows = ok ? min(ROWS, pc.ntok * p.group - pc.row0) : 0;
     const int npg = pc.npg;
-    // Q^T fragments: lane (r, t) holds channels 8 t .. 8 t + 7 of every group of row r (+ 8 per n-tile): two k-steps
-    uint32_t qb[NT][GROUPS][4];
-    uint32_t top_bits = 0;
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      const uint4* src = reinterpret_cast<const uint4*>(smem + Shape::OFF_Q + e * Shape::Q_BYTES + (nt * 8 + r) * D * 2) + t;
-      const bool live = nt * 8 + r < rows;
-#pragma unroll
-      for (int grp = 0; grp < GROUPS; ++grp) {
-        const uint4 v = live ? src[grp * 4] : make_uint4(0, 0, 0, 0);
-        qb[nt][grp][0] = v.x ^ p.q_flip;
-        qb[nt][grp][1] = v.y ^ p.q_flip;
-        qb[nt][grp][2] = v.z ^ p.q_flip;
-        qb[nt][grp][3] = v.w ^ p.q_flip;
-        if constexpr (!Kv4Type<T>::IS_BF16) {
-          const uint32_t mag = 0x7fff7fffu;
-          top_bits = __vmaxu2(top_bits, __vmaxu2(__vmaxu2(v.x & mag, v.y & mag), __vmaxu2(v.z & mag, v.w & mag)));
-        }
-      }
-    }
-    float unit_scale = 1.f;
-    if constexpr (!Kv4Type<T>::IS_BF16) {
-      // fp16: the largest magnitude's exponent field is 20 for 32 <= |q| < 64; below 32, 64 sum|q| stays finite
-      const uint32_t all = __reduce_max_sync(0xffffffffu, max(top_bits & 0xffffu, top_bits >> 16));
-      const int over = static_cast<int>(all >> 10) - 19;
-      if (over > 0 && over < 12) {  // 12: infinity or NaN, left alone
-        const __half2 f = __float2half2_rn(exp2f(static_cast<float>(-over)));
-        unit_scale = exp2f(static_cast<float>(over));
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int grp = 0; grp < GROUPS; ++grp)
-#pragma unroll
-            for (int x = 0; x < 4; ++x) {
-              const __half2 v = __hmul2(*reinterpret_cast<const __half2*>(&qb[nt][grp][x]), f);
-              qb[nt][grp][x] = *reinterpret_cast<const uint32_t*>(&v);
-            }
-      }
-    }
-    // scores in log2 units are raw * scale (or capped: kv4_softcap(raw, cap_k, cap_log2), scale 1)
-    const float cap_k = EXT ? p.cap_k * unit_scale : 0.f;
-    const float scale = EXT && p.cap_log2 != 0.f ? 1.f : p.scale_log2 * unit_scale;
-    // B fragments of the minimum / bias k-step: sums of q over groups 2 t and 2 t + 1 of row r, and -bias times them
-    uint32_t ql[NT][Kv4Bias<T>::TERMS][2];
+    // Q^T fragments: lane (r, t) has channels 8 t .. 8 t + 7 of every group of row r (+ 8 per n-tile), two k-steps each.
+    // They stay in shared memory, one 16-byte load per group and slot. Rows behind the last hold anything: a column of
+    // the products is its own, and theirs are never written out.
+    const uint8_t* q_rows = smem + Shape::OFF_Q + e * Shape::Q_BYTES + r * Shape::Q_PITCH + t * 16;
+    // B fragments of the minimum / bias k-steps: sums of q over groups 2 t and 2 t + 1 of row r, leading and trailing term
+    // (bf16: and a third, with -bias times it), each row scaled by a power of two so that its largest sum is in
+    // [2^12, 2^13): fp16 would lose the trailing terms of small queries and the sums of large ones. `undo` is the inverse
+    // for this lane's score columns, rows 2 t and 2 t + 1.
+    uint32_t ql[NT][BF16 ? 4 : 2];
+    float undo[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       float sum[2] = {0.f, 0.f};
 #pragma unroll
       for (int grp = 0; grp < GROUPS; ++grp) {
+        const uint4 v = *reinterpret_cast<const uint4*>(q_rows + nt * 8 * Shape::Q_PITCH + grp * 64);
         const float zero[4] = {0.f, 0.f, 0.f, 0.f};
         float c[4];
-        constexpr uint32_t mb = Kv4Bias<T>::MINUS;
-        kv4_mma<T>(c, mb, mb, mb, mb, qb[nt][grp][0], qb[nt][grp][1], zero);
-        kv4_mma<T>(c, mb, mb, mb, mb, qb[nt][grp][2], qb[nt][grp][3], c);
+        constexpr uint32_t ones = Kv4Bias<T>::ONES;
+        kv4_mma<T>(c, ones, ones, ones, ones, v.x, v.y, zero);
+        kv4_mma<T>(c, ones, ones, ones, ones, v.z, v.w, c);
         // c[0], c[1] are columns 2 t, 2 t + 1; column r sits in the lanes with t = r / 2
         const float x = __shfl_sync(0xffffffffu, c[0], (lane & 28) | (r >> 1));
         const float y = __shfl_sync(0xffffffffu, c[1], (lane & 28) | (r >> 1));
         if (grp / 2 == t) sum[grp & 1] = (r & 1) ? y : x;
       }
+      float most = fmaxf(fabsf(sum[0]), fabsf(sum[1]));
+      most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+      most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+      const int up = min(12 + 127 - static_cast<int>(__float_as_uint(most) >> 23), 126);  // >= -116
+      sum[0] *= exp2f(static_cast<float>(up));
+      sum[1] *= exp2f(static_cast<float>(up));
 #pragma unroll
-      for (int k2 = 0; k2 < Kv4Bias<T>::TERMS; ++k2) {
+      for (int c = 0; c < 2; ++c) undo[nt][c] = exp2f(static_cast<float>(-__shfl_sync(0xffffffffu, up, (2 * t + c) * 4)));
+#pragma unroll
+      for (int k2 = 0; k2 < 2; ++k2) {
         const float h0 = Cvt<T>::to_f(Cvt<T>::from_f(sum[0])), h1 = Cvt<T>::to_f(Cvt<T>::from_f(sum[1]));
-        ql[nt][k2][0] = Kv4Type<T>::pack(h0 * (-1.f / Kv4Bias<T>::BIAS), h1 * (-1.f / Kv4Bias<T>::BIAS));
-        ql[nt][k2][1] = Kv4Type<T>::pack(h0, h1);
+        ql[nt][k2] = Kv4Type<T>::pack(h0, h1);
         sum[0] -= h0;
         sum[1] -= h1;
+      }
+      if constexpr (BF16) {
+        ql[nt][2] = Kv4Type<T>::pack(sum[0], sum[1]);
+        ql[nt][3] = Kv4Type<T>::pack(sum[0] * -Kv4Bias<T>::BIAS, sum[1] * -Kv4Bias<T>::BIAS);
       }
     }
     float o[NT][D / 16][4];
     float m[NT][2], l[NT][2];
+    int v_exp = -1000;  // bf16: V is scaled by 2^-v_exp into fp16's range
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       m[nt][0] = m[nt][1] = -INFINITY;
@@ -469,41 +449,47 @@ __global__ void __launch_bounds__(KV4_DEC_THREADS, Kv4DecShape<D, NT>::CTAS) kv4
       const uint8_t* slot = smem + s * Shape::SLOT_BYTES;
       // ---- S^T = K Q^T
       float sc[2][NT][4];
+      uint32_t m0[2][GROUPS], m1[2][GROUPS];  // (lo, s) of tokens r and r + 8
 #pragma unroll
       for (int pg = 0; pg < 2; ++pg) {
-        const uint8_t* k0 = slot + pg * 2 * PB + r * ROW;
-        const uint8_t* k1 = k0 + 8 * ROW;
-        {
-          // k-slots 2 t, 2 t + 1 are the minima of groups 2 t, 2 t + 1, k-slots + 8 their steps. Where there are fewer
-          // groups than slots ql is 0 and any group's words do.
-          const int go = (2 * t) % GROUPS * 4;
-          const uint2 x = *reinterpret_cast<const uint2*>(k0 + D / 2 + go), y = *reinterpret_cast<const uint2*>(k1 + D / 2 + go);
-          const uint32_t a0 = __byte_perm(x.x, x.y, 0x5410), a1 = __byte_perm(y.x, y.y, 0x5410);
-          const uint32_t a2 = __byte_perm(x.x, x.y, 0x7632), a3 = __byte_perm(y.x, y.y, 0x7632);
+        const uint8_t* k0 = slot + pg * 2 * PB + r * ROW + D / 2;
+        // k-slots 2 t, 2 t + 1 (and those + 8) are groups 2 t, 2 t + 1: minima in one product, steps in the other. Where
+        // there are fewer groups than slots ql is 0 and any group's words do.
+        const int go = (2 * t) % GROUPS * 4;
+        const uint2 x = *reinterpret_cast<const uint2*>(k0 + go), y = *reinterpret_cast<const uint2*>(k0 + 8 * ROW + go);
+        const uint32_t lo0 = __byte_perm(x.x, x.y, 0x5410), lo1 = __byte_perm(y.x, y.y, 0x5410);
+        const uint32_t st0 = __byte_perm(x.x, x.y, 0x7632), st1 = __byte_perm(y.x, y.y, 0x7632);
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            const float zero[4] = {0.f, 0.f, 0.f, 0.f};
-            kv4_mma<T>(sc[pg][nt], a0, a1, a2, a3, ql[nt][0][0], ql[nt][0][1], zero);
+        for (int nt = 0; nt < NT; ++nt) {
+          const float zero[4] = {0.f, 0.f, 0.f, 0.f};
+          float a[4], b[4];
+          kv4_mma<T>(a, lo0, lo1, lo0, lo1, ql[nt][0], ql[nt][1], zero);
+          kv4_mma<T>(b, st0, st1, st0, st1, ql[nt][0], ql[nt][1], zero);
+          if constexpr (BF16) kv4_mma<T>(a, lo0, lo1, st0, st1, ql[nt][2], ql[nt][3], a);
 #pragma unroll
-            for (int k2 = 1; k2 < Kv4Bias<T>::TERMS; ++k2)
-              kv4_mma<T>(sc[pg][nt], a0, a1, a2, a3, ql[nt][k2][0], ql[nt][k2][1], sc[pg][nt]);
-          }
+          for (int c = 0; c < 4; ++c) sc[pg][nt][c] = fmaf(b[c], -Kv4Bias<T>::BIAS, a[c]) * undo[nt][c & 1];
         }
-        uint32_t m0[GROUPS], m1[GROUPS];
-        kv4_words<GROUPS>(k0 + D / 2, m0);
-        kv4_words<GROUPS>(k1 + D / 2, m1);
+        kv4_words<GROUPS>(k0, m0[pg]);
+        kv4_words<GROUPS>(k0 + 8 * ROW, m1[pg]);
+      }
 #pragma unroll
-        for (int grp = 0; grp < GROUPS; ++grp) {
+      for (int grp = 0; grp < GROUPS; ++grp) {
+        uint4 q[NT];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) q[nt] = *reinterpret_cast<const uint4*>(q_rows + nt * 8 * Shape::Q_PITCH + grp * 64);
+#pragma unroll
+        for (int pg = 0; pg < 2; ++pg) {
+          const uint8_t* k0 = slot + pg * 2 * PB + r * ROW + grp * 16 + t * 4;
           uint32_t e0[4], e1[4];
-          kv4_raw4<T>(*reinterpret_cast<const uint32_t*>(k0 + grp * 16 + t * 4), e0);
-          kv4_raw4<T>(*reinterpret_cast<const uint32_t*>(k1 + grp * 16 + t * 4), e1);
-          const float s0 = kv4_step<T>(m0[grp]), s1 = kv4_step<T>(m1[grp]);
+          kv4_raw4<T>(*reinterpret_cast<const uint32_t*>(k0), e0);
+          kv4_raw4<T>(*reinterpret_cast<const uint32_t*>(k0 + 8 * ROW), e1);
+          const float s0 = kv4_step<T>(m0[pg][grp]), s1 = kv4_step<T>(m1[pg][grp]);
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
             const float zero[4] = {0.f, 0.f, 0.f, 0.f};
             float c[4];
-            kv4_mma<T>(c, e0[0], e1[0], e0[1], e1[1], qb[nt][grp][0], qb[nt][grp][1], zero);
-            kv4_mma<T>(c, e0[2], e1[2], e0[3], e1[3], qb[nt][grp][2], qb[nt][grp][3], c);
+            kv4_mma<T>(c, e0[0], e1[0], e0[1], e1[1], q[nt].x, q[nt].y, zero);
+            kv4_mma<T>(c, e0[2], e1[2], e0[3], e1[3], q[nt].z, q[nt].w, c);
             sc[pg][nt][0] = fmaf(s0, c[0], sc[pg][nt][0]);
             sc[pg][nt][1] = fmaf(s0, c[1], sc[pg][nt][1]);
             sc[pg][nt][2] = fmaf(s1, c[2], sc[pg][nt][2]);
@@ -520,14 +506,15 @@ __global__ void __launch_bounds__(KV4_DEC_THREADS, Kv4DecShape<D, NT>::CTAS) kv4
       bool plain = at1 + KV4_PAGE <= pc.all_to;
       if (EXT) plain = plain && (at0 >= pc.all_from || at0 + KV4_PAGE <= p.sink) && (at1 >= pc.all_from || at1 + KV4_PAGE <= p.sink);
       uint32_t seen = 0xffffffffu;
-      if (EXT && p.cap_log2 != 0.f) {
 #pragma unroll
-        for (int pg = 0; pg < 2; ++pg)
+      for (int pg = 0; pg < 2; ++pg)
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int c = 0; c < 4; ++c) sc[pg][nt][c] = kv4_softcap(sc[pg][nt][c], cap_k, p.cap_log2);
-      }
+          for (int c = 0; c < 4; ++c) {
+            const float v = sc[pg][nt][c];
+            sc[pg][nt][c] = EXT && p.cap_log2 != 0.f ? kv4_softcap(v, p.cap_k, p.cap_log2) : v * p.scale_log2;
+          }
       if (!plain) {
         auto sees = [&](int pos, int tok) {
           return kv4_visible(pos, p.q_kvlen[tok], EXT && p.q_kvstart ? p.q_kvstart[tok] : 0, p.sink,
@@ -558,7 +545,7 @@ __global__ void __launch_bounds__(KV4_DEC_THREADS, Kv4DecShape<D, NT>::CTAS) kv4
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          top[nt][c] = fmaxf(fmaxf(sc[0][nt][c], sc[0][nt][c + 2]), fmaxf(sc[1][nt][c], sc[1][nt][c + 2])) * scale;
+          top[nt][c] = fmaxf(fmaxf(sc[0][nt][c], sc[0][nt][c + 2]), fmaxf(sc[1][nt][c], sc[1][nt][c + 2]));
           raise = raise || top[nt][c] > m[nt][c] + 8.f;
         }
       if (__any_sync(0xffffffffu, raise)) {
@@ -590,44 +577,77 @@ __global__ void __launch_bounds__(KV4_DEC_THREADS, Kv4DecShape<D, NT>::CTAS) kv4
         for (int pg = 0; pg < 2; ++pg)
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const float2 x = kv4_fma2(make_float2(sc[pg][nt][2 * h], sc[pg][nt][2 * h + 1]), make_float2(scale, scale), shift);
+            const float2 x = kv4_add2(make_float2(sc[pg][nt][2 * h], sc[pg][nt][2 * h + 1]), shift);
             const float2 w = make_float2(exp2f(x.x), exp2f(x.y));
             ls = kv4_add2(ls, w);
-            pb[pg][nt][h] = kv4_movmatrix(Kv4Type<T>::pack(w.x, w.y));
+            pb[pg][nt][h] = kv4_movmatrix(Kv4Type<__half>::pack(w.x, w.y));
           }
         l[nt][0] = ls.x;
         l[nt][1] = ls.y;
       }
       // ---- O^T += V^T P^T: this lane expands channels [r D / 8, (r + 1) D / 8) of tokens 2t, 2t+1, 2t+8, 2t+9
+      uint32_t meta[2][4];
 #pragma unroll
-      for (int pg = 0; pg < 2; ++pg) {
-        const uint8_t* vb = slot + (pg * 2 + 1) * PB + 2 * t * ROW;
-        uint32_t w[4][VW], meta[4];
+      for (int pg = 0; pg < 2; ++pg)
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
-          const uint8_t* v = vb + ((x & 1) + (x >> 1) * 8) * ROW;
-          kv4_words<VW>(v + r * (D / 16), w[x]);
-          meta[x] = *reinterpret_cast<const uint32_t*>(v + D / 2 + (r * (D / 8) / KV4_GROUP) * 4);
+          meta[pg][x] = *reinterpret_cast<const uint32_t*>(slot + (pg * 2 + 1) * PB + (2 * t + (x & 1) + (x >> 1) * 8) * ROW +
+                                                           D / 2 + (r * (D / 8) / KV4_GROUP) * 4);
+          if (!plain && !((seen >> (pg * 16 + 2 * t + (x & 1) + (x >> 1) * 8)) & 1u)) meta[pg][x] = 0u;
         }
-        if (!plain) {
+      float shrink = 1.f;
+      if constexpr (BF16) {
+        // |v| <= |lo| + 15 s: with |lo| < 2^(v_exp + 13) and s < 2^(v_exp + 9) the scaled values stay below 2^14. A larger
+        // one raises v_exp for good (O is rescaled); smaller ones keep their 11 bits down to 2^-28 of the largest.
+        uint32_t top = 0;
 #pragma unroll
-          for (int x = 0; x < 4; ++x)
-            if (!((seen >> (pg * 16 + 2 * t + (x & 1) + (x >> 1) * 8)) & 1u)) meta[x] = 0u;
+        for (int pg = 0; pg < 2; ++pg)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) top = __vmaxu2(top, meta[pg][x] & 0xffff7fffu);
+        const int need = max(static_cast<int>(top >> 23) - 9, static_cast<int>((top & 0xffffu) >> 7) - 13) - 126;
+        if (__any_sync(0xffffffffu, need > v_exp)) {
+          const int e2 = (__reduce_max_sync(0xffffffffu, need) + 1027) / 4 * 4 - 1024;  // in steps of 4
+          const float f = v_exp == -1000 ? 1.f : exp2f(static_cast<float>(max(v_exp - e2, -126)));
+          v_exp = max(e2, -120);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int j = 0; j < D / 16; ++j)
+#pragma unroll
+              for (int c = 0; c < 4; ++c) o[nt][j][c] *= f;
         }
-        const uint32_t lo_ab = __byte_perm(meta[0], meta[1], 0x5410), s_ab = __byte_perm(meta[0], meta[1], 0x7632);
-        const uint32_t lo_cd = __byte_perm(meta[2], meta[3], 0x5410), s_cd = __byte_perm(meta[2], meta[3], 0x7632);
+        shrink = exp2f(static_cast<float>(-v_exp));
+      }
+#pragma unroll
+      for (int pg = 0; pg < 2; ++pg) {
+        const uint8_t* vb = slot + (pg * 2 + 1) * PB + 2 * t * ROW + r * (D / 16);
+        uint32_t w[4][VW];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) kv4_words<VW>(vb + ((x & 1) + (x >> 1) * 8) * ROW, w[x]);
+        uint32_t lo[2], st[2];  // of token pairs (2t, 2t+1) and (2t+8, 2t+9), in fp16
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const uint32_t ma = meta[pg][2 * x], mb = meta[pg][2 * x + 1];
+          if constexpr (BF16) {
+            lo[x] = Kv4Type<__half>::pack(__uint_as_float(ma << 16) * shrink, __uint_as_float(mb << 16) * shrink);
+            st[x] = Kv4Type<__half>::pack(__uint_as_float(ma & 0xffff0000u) * shrink, __uint_as_float(mb & 0xffff0000u) * shrink);
+          } else {
+            lo[x] = __byte_perm(ma, mb, 0x5410);
+            st[x] = __byte_perm(ma, mb, 0x7632);
+          }
+        }
 #pragma unroll
         for (int i2 = 0; i2 < VW; ++i2) {
           uint32_t a0[4], a1[4], a2[4], a3[4];
-          Kv4Type<T>::expand4(__byte_perm(w[0][i2], w[1][i2], 0x5410), s_ab, lo_ab, a0);
-          Kv4Type<T>::expand4(__byte_perm(w[0][i2], w[1][i2], 0x7632), s_ab, lo_ab, a1);
-          Kv4Type<T>::expand4(__byte_perm(w[2][i2], w[3][i2], 0x5410), s_cd, lo_cd, a2);
-          Kv4Type<T>::expand4(__byte_perm(w[2][i2], w[3][i2], 0x7632), s_cd, lo_cd, a3);
+          Kv4Type<__half>::expand4(__byte_perm(w[0][i2], w[1][i2], 0x5410), st[0], lo[0], a0);
+          Kv4Type<__half>::expand4(__byte_perm(w[0][i2], w[1][i2], 0x7632), st[0], lo[0], a1);
+          Kv4Type<__half>::expand4(__byte_perm(w[2][i2], w[3][i2], 0x5410), st[1], lo[1], a2);
+          Kv4Type<__half>::expand4(__byte_perm(w[2][i2], w[3][i2], 0x7632), st[1], lo[1], a3);
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int x = 0; x < 4; ++x)
-              kv4_mma<T>(o[nt][i2 * 4 + x], a0[x], a1[x], a2[x], a3[x], pb[pg][nt][0], pb[pg][nt][1], o[nt][i2 * 4 + x]);
+              kv4_mma<__half>(o[nt][i2 * 4 + x], a0[x], a1[x], a2[x], a3[x], pb[pg][nt][0], pb[pg][nt][1], o[nt][i2 * 4 + x]);
         }
       }
       __syncwarp();
@@ -637,59 +657,94 @@ __global__ void __launch_bounds__(KV4_DEC_THREADS, Kv4DecShape<D, NT>::CTAS) kv4
     __syncwarp();
     if (lane == 0) mbar_arrive(&piece_empty[e]);  // descriptor and query rows are in registers
     // ---------------------------------------------------------------- merge the four warps of the unit
+    // Two rounds (2 -> 0 and 3 -> 1, then 1 -> 0) through two buffers in fragment order; a lane keeps its place, so the
+    // accesses are whole 512-byte rows and the arithmetic stays in registers.
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        float x = l[nt][c];
-        x += __shfl_xor_sync(0xffffffffu, x, 4);
-        x += __shfl_xor_sync(0xffffffffu, x, 8);
-        x += __shfl_xor_sync(0xffffffffu, x, 16);
-        const int row = nt * 8 + 2 * t + c;
-        if (r == 0) {
-          sm_ml[(warp * ROWS + row) * 2] = m[nt][c];
-          sm_ml[(warp * ROWS + row) * 2 + 1] = x;
-        }
-        if (row < rows) {
-          float* dst = sm_o + (warp * ROWS + row) * D + r * (D / 8);
-#pragma unroll
-          for (int j = 0; j < D / 16; ++j) *reinterpret_cast<float2*>(dst + 2 * j) = make_float2(o[nt][j][c], o[nt][j][c + 2]);
-        }
+        l[nt][c] += __shfl_xor_sync(0xffffffffu, l[nt][c], 4);
+        l[nt][c] += __shfl_xor_sync(0xffffffffu, l[nt][c], 8);
+        l[nt][c] += __shfl_xor_sync(0xffffffffu, l[nt][c], 16);
       }
-    asm volatile("bar.sync 1, 128;" ::: "memory");
-    for (int row = warp; row < rows; row += 4) {
-      float M = -INFINITY, L = 0.f, wgt[4];
+    if constexpr (BF16) {
+      const float f = exp2f(static_cast<float>(max(v_exp, -126)));  // untouched (-1000): o is 0
 #pragma unroll
-      for (int w = 0; w < 4; ++w) M = fmaxf(M, sm_ml[(w * ROWS + row) * 2]);
+      for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        const float mw = sm_ml[(w * ROWS + row) * 2];
-        wgt[w] = mw == -INFINITY ? 0.f : exp2f(mw - M);
-        const float lw = sm_ml[(w * ROWS + row) * 2 + 1];
-        L += lw != lw ? lw : lw * wgt[w];
-      }
-      float acc[D / 32];
+        for (int j = 0; j < D / 16; ++j)
 #pragma unroll
-      for (int c = 0; c < D / 32; ++c) acc[c] = 0.f;
-#pragma unroll
-      for (int w = 0; w < 4; ++w)
-#pragma unroll
-        for (int c = 0; c < D / 32; ++c) acc[c] = fmaf(sm_o[(w * ROWS + row) * D + c * 32 + lane], wgt[w], acc[c]);
-      if (pc.part >= 0) {
-        const size_t base = static_cast<size_t>(pc.part) * 16 + row;
-#pragma unroll
-        for (int c = 0; c < D / 32; ++c) p.part_o[base * D + c * 32 + lane] = acc[c];
-        if (lane == 0) {
-          p.part_ml[base * 2] = M;
-          p.part_ml[base * 2 + 1] = L;
-        }
-      } else {
-        kv4_finish_row<T, D>(p, pc.qstart, pc.hk, pc.row0 + row, M, L, acc);
-      }
+          for (int c = 0; c < 4; ++c) o[nt][j][c] *= f;
     }
-    // The scratch area is rewritten by the next unit. One thread samples the abort flag between the barriers, so that
-    // all four warps leave together if a wait of any role ran out.
+    auto give = [&](int b) {
+      float4* dst = reinterpret_cast<float4*>(merge + b * (ROWS * D * 4)) + lane;
+      float* ml = reinterpret_cast<float*>(merge + 2 * ROWS * D * 4 + b * ROWS * 8);
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+        for (int j = 0; j < D / 16; ++j)
+          dst[(nt * (D / 16) + j) * 32] = make_float4(o[nt][j][0], o[nt][j][1], o[nt][j][2], o[nt][j][3]);
+        if (r == 0)
+          reinterpret_cast<float4*>(ml)[nt * 4 + t] = make_float4(m[nt][0], l[nt][0], m[nt][1], l[nt][1]);
+      }
+    };
+    auto take = [&](int b) {
+      const float4* src = reinterpret_cast<const float4*>(merge + b * (ROWS * D * 4)) + lane;
+      const float* ml = reinterpret_cast<const float*>(merge + 2 * ROWS * D * 4 + b * ROWS * 8);
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        const float4 x = reinterpret_cast<const float4*>(ml)[nt * 4 + t];
+        const float M0 = fmaxf(m[nt][0], x.x), M1 = fmaxf(m[nt][1], x.z);
+        const float a0 = m[nt][0] == -INFINITY ? 0.f : exp2f(m[nt][0] - M0), a1 = m[nt][1] == -INFINITY ? 0.f : exp2f(m[nt][1] - M1);
+        const float b0 = x.x == -INFINITY ? 0.f : exp2f(x.x - M0), b1 = x.z == -INFINITY ? 0.f : exp2f(x.z - M1);
+        l[nt][0] = l[nt][0] * a0 + x.y * b0;
+        l[nt][1] = l[nt][1] * a1 + x.w * b1;
+        m[nt][0] = M0;
+        m[nt][1] = M1;
+#pragma unroll
+        for (int j = 0; j < D / 16; ++j) {
+          const float4 y = src[(nt * (D / 16) + j) * 32];
+          o[nt][j][0] = o[nt][j][0] * a0 + y.x * b0;
+          o[nt][j][1] = o[nt][j][1] * a1 + y.y * b1;
+          o[nt][j][2] = o[nt][j][2] * a0 + y.z * b0;
+          o[nt][j][3] = o[nt][j][3] * a1 + y.w * b1;
+        }
+      }
+    };
+    if (warp >= 2) give(warp - 2);
+    asm volatile("bar.sync 1, 128;" ::: "memory");
+    if (warp < 2) take(warp);
+    if (warp == 1) give(1);  // its own buffer, which no other warp reads before the barrier
     if (threadIdx.x == 0) leave_word = *abort_flag;
+    asm volatile("bar.sync 1, 128;" ::: "memory");
+    if (warp == 0) {
+      take(1);
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const int row = nt * 8 + 2 * t + c;
+          if (row >= rows) continue;
+          if (pc.part >= 0) {
+            const size_t at = static_cast<size_t>(pc.part) * 16 + row;
+            float2* dst = reinterpret_cast<float2*>(p.part_o + at * D + r * (D / 8));
+#pragma unroll
+            for (int j = 0; j < D / 16; ++j) dst[j] = make_float2(o[nt][j][c], o[nt][j][c + 2]);
+            if (r == 0) reinterpret_cast<float2*>(p.part_ml)[at] = make_float2(m[nt][c], l[nt][c]);
+          } else {
+            // a row that sees nothing is 0; NaN stays NaN
+            const float L = l[nt][c], inv = L == 0.f ? 0.f : 1.f / L;
+            const size_t at = static_cast<size_t>(pc.qstart + (pc.row0 + row) / p.group) * p.hq + pc.hk * p.group +
+                              (pc.row0 + row) % p.group;
+            uint32_t* dst = reinterpret_cast<uint32_t*>(reinterpret_cast<T*>(p.out) + at * D + r * (D / 8));
+#pragma unroll
+            for (int j = 0; j < D / 16; ++j) dst[j] = Kv4Type<T>::pack(o[nt][j][c] * inv, o[nt][j][c + 2] * inv);
+            if (p.lse && r == 0) p.lse[at] = L == 0.f ? -INFINITY : (m[nt][c] + log2f(L)) * 0.6931471805599453f;
+          }
+        }
+    }
+    // Buffer 1 is read by warp 0 until here and written next by warp 3. One thread sampled the abort flag, so that the
+    // warps leave together if a wait of any role ran out.
     asm volatile("bar.sync 1, 128;" ::: "memory");
     if (leave_word || pc.last) break;
   }
@@ -698,31 +753,45 @@ __global__ void __launch_bounds__(KV4_DEC_THREADS, Kv4DecShape<D, NT>::CTAS) kv4
 // Joins the pieces of the units that were cut: block c has the unit that began in CTA c's share, if any. Its first
 // piece is that CTA's last, the others are the first pieces of the CTAs after it.
 template <typename T, int D>
-__global__ void __launch_bounds__(128) kv4_decode_merge_kernel(const Kv4DecParams p, int rows_per_block) {
+__global__ void __launch_bounds__(128) kv4_decode_merge_kernel(const Kv4DecParams p) {
   pdl_launch_dependents();
   pdl_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int4 pu = reinterpret_cast<const int4*>(p.part_unit)[blockIdx.x];
-  const int item = pu.x, pieces = pu.z;
-  if (item < 0) return;
-  const int hk = pu.y / p.row_blocks, row0 = pu.y % p.row_blocks * rows_per_block;
-  const int qstart = p.item_qstart[item];
-  const int rows = min(rows_per_block, p.item_ntok[item] * p.group - row0);
+  const int rows = pu.x, qstart = pu.y, hk = pu.z >> 4, row0 = pu.z & 15, pieces = pu.w;
   for (int row = warp; row < rows; row += 4) {
     auto block = [&](int i) { return (i == 0 ? blockIdx.x * 2 + 1 : (blockIdx.x + i) * 2) * static_cast<size_t>(16) + row; };
-    float M = -INFINITY;
-    for (int i = lane; i < pieces; i += 32) M = fmaxf(M, p.part_ml[block(i) * 2]);
-    M = warp_max(M);
-    float L = 0.f, acc[D / 32];
+    // running maximum over batches of four pieces, whose loads are issued together
+    float M = -INFINITY, L = 0.f, acc[D / 32];
 #pragma unroll
     for (int c = 0; c < D / 32; ++c) acc[c] = 0.f;
-    for (int i = 0; i < pieces; ++i) {
-      const size_t b = block(i);
-      const float ms = p.part_ml[b * 2], ls = p.part_ml[b * 2 + 1];
-      const float w = ms == -INFINITY ? 0.f : exp2f(ms - M);
-      L += ls != ls ? ls : ls * w;
+    for (int base = 0; base < pieces; base += 4) {
+      float2 ml[4];
+      float v[4][D / 32];
 #pragma unroll
-      for (int c = 0; c < D / 32; ++c) acc[c] = fmaf(p.part_o[b * D + c * 32 + lane], w, acc[c]);
+      for (int i = 0; i < 4; ++i) {
+        ml[i] = make_float2(-INFINITY, 0.f);
+        if (base + i < pieces) {
+          const size_t b = block(base + i);
+          ml[i] = reinterpret_cast<const float2*>(p.part_ml)[b];
+#pragma unroll
+          for (int c = 0; c < D / 32; ++c) v[i][c] = p.part_o[b * D + c * 32 + lane];
+        }
+      }
+      const float Mn = fmaxf(M, fmaxf(fmaxf(ml[0].x, ml[1].x), fmaxf(ml[2].x, ml[3].x)));
+      const float f = M == -INFINITY ? 0.f : exp2f(M - Mn);
+      L *= f;
+#pragma unroll
+      for (int c = 0; c < D / 32; ++c) acc[c] *= f;
+      M = Mn;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (base + i >= pieces) continue;
+        const float w = ml[i].x == -INFINITY ? 0.f : exp2f(ml[i].x - M);
+        L += ml[i].y * w;
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) acc[c] = fmaf(v[i][c], w, acc[c]);
+      }
     }
     kv4_finish_row<T, D>(p, qstart, hk, row0 + row, M, L, acc);
   }
@@ -766,7 +835,7 @@ int kv4_decode_launch(Kv4DecParams p, int num_items, int max_ctas, cudaStream_t 
     attr.val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
-    err = cudaLaunchKernelEx(&cfg, kv4_decode_merge_kernel<T, D>, part, Shape::ROWS);
+    err = cudaLaunchKernelEx(&cfg, kv4_decode_merge_kernel<T, D>, part);
     if (err != cudaSuccess) return static_cast<int>(err);
     count_launch();
   }
@@ -835,9 +904,8 @@ MLCB_API int mlcb_kv4_decode(const void* q, const void* pages, void* out, float*
   p.row_blocks = 1;
   p.num_items = num_items;
   p.sink = q_kvstart ? sink : 0;
-  p.q_flip = sm_scale < 0.f ? 0x80008000u : 0u;
-  p.scale_log2 = fmaxf(fabsf(sm_scale) * 1.4426950408889634f, 1e-30f);  // a hidden score is -inf * scale: not 0
-  p.cap_k = softcap > 0.f ? 2.f * 1.4426950408889634f * fabsf(sm_scale) / softcap : 0.f;
+  p.scale_log2 = sm_scale * 1.4426950408889634f;
+  p.cap_k = softcap > 0.f ? 2.f * 1.4426950408889634f * sm_scale / softcap : 0.f;
   p.cap_log2 = softcap > 0.f ? softcap * 1.4426950408889634f : 0.f;
   const bool ext = q_kvstart || tree_mask || softcap > 0.f;
   if (dtype == 0) {
