@@ -435,7 +435,10 @@ __global__ void __launch_bounds__(KV4_DEC_THREADS, Kv4DecShape<D, NT>::CTAS) kv4
     int v_exp = -1000;  // bf16: V is scaled by 2^-v_exp into fp16's range
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      m[nt][0] = m[nt][1] = -INFINITY;
+      // A column behind the last row has an infinite maximum, weights of 0 and never asks for a rescaling: it holds the
+      // products of whatever the shared memory held, which must not decide when the warp's live rows are rounded.
+#pragma unroll
+      for (int c = 0; c < 2; ++c) m[nt][c] = nt * 8 + 2 * t + c < rows ? -INFINITY : INFINITY;
       l[nt][0] = l[nt][1] = 0.f;
 #pragma unroll
       for (int j = 0; j < D / 16; ++j) o[nt][j][0] = o[nt][j][1] = o[nt][j][2] = o[nt][j][3] = 0.f;
@@ -714,6 +717,7 @@ __global__ void __launch_bounds__(KV4_DEC_THREADS, Kv4DecShape<D, NT>::CTAS) kv4
     if (warp >= 2) give(warp - 2);
     asm volatile("bar.sync 1, 128;" ::: "memory");
     if (warp < 2) take(warp);
+    __syncwarp();
     if (warp == 1) give(1);  // its own buffer, which no other warp reads before the barrier
     if (threadIdx.x == 0) leave_word = *abort_flag;
     asm volatile("bar.sync 1, 128;" ::: "memory");

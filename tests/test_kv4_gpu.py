@@ -252,6 +252,23 @@ def test_decode(dtype, case):
     assert _same_bytes(out, again)   # no atomics: the same call gives the same bits
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_decode_ignores_what_ran_before(dtype, d):
+    """Four live rows use half of a column block. What earlier launches left in shared memory for the other half, here
+    rows of very small and very large queries, changes no bit of theirs."""
+    st = Step(dtype, [2000] * 24, [1] * 24, 8, 2, d, seed=1)
+    small = Step(dtype, [2000] * 24, [1] * 24, 16, 2, d, seed=2, q_by=1e-4)
+    large = Step(dtype, [2000] * 24, [1] * 24, 16, 2, d, seed=2, q_by=200.0)
+    outs = []
+    for other in (small, large, small):
+        other.run()
+        outs.append(st.run())
+    ops.check_status(st.cache.device)
+    for out, lse in outs[1:]:
+        assert _same_bytes(out, outs[0][0]) and _same_bytes(lse, outs[0][1])
+
+
 PREFILL = [
     ([100], [100], 8, 2, 128, {}),
     ([300, 17, 64, 1], [300, 17, 64, 1], 8, 2, 128, {}),           # two query tiles, one, and decode items next to them
