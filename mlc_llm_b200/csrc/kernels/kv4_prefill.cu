@@ -5,13 +5,16 @@
 // by side -- as two accumulator tiles of 128 rows, and walks the cached positions in blocks of 128:
 //
 //   raw       a warp copies the blocks' packed rows (80 bytes per token at D = 128) into a ring of shared memory
-//   expand    four warps turn them into 16-bit K and V tiles in the layout the tensor core reads (128-byte
-//             swizzle; V MN-major), lo + s c rounded once. One expansion feeds both query tiles: at 600 issue
-//             slots per scheduler and block it hides under the 2048 clocks of the block's products.
+//   expand    four warps turn them into fp16 K and V tiles in the layout the tensor core reads (128-byte swizzle; V
+//             MN-major), lo + s c rounded once. One expansion feeds both query tiles: at 600 issue slots per
+//             scheduler and block it hides under the 2048 clocks of the block's products. bf16 rows are scaled by a
+//             power of two per 32 positions (and queries per row) into fp16's range, so that K, V and P keep 11 bits:
+//             the scale of K multiplies the scores, that of V the weights.
 //   S = Q K^T    tcgen05.mma, both operands in shared memory, D in TMEM (128 columns per tile)
-//   softmax      one thread per row, 32 columns of TMEM at a time. Weights are taken against the running reference
-//                maximum of the blocks before; only if a score exceeds it by more than 8 (log2) is the block redone
-//                with a raised one and O rescaled. P (16 bits) overwrites S in TMEM.
+//   softmax      one thread per row, 32 columns of TMEM at a time, in two passes: the block's maximum, then its weights
+//                against a running reference that is raised (and O rescaled) only when a score exceeds it by more
+//                than 8 (log2). One vote per block: with one per 32 columns the code between the votes could not be
+//                interleaved, and a block took 2630 clocks instead of 2100. P (fp16) overwrites S in TMEM.
 //   O += P V     tcgen05.mma, A = P in TMEM, B = V in shared memory, D accumulates in TMEM for the whole loop
 //
 // While the softmax of one tile runs, the tensor core works on the other tile. With D = 256 one tile fills TMEM (O
@@ -47,6 +50,15 @@ struct Kv4PreParams {
   float cap_k, cap_log2;   // soft cap: scores are kv4_softcap(raw, cap_k, cap_log2); 0 = none
 };
 
+// One lane of a converged warp, in the form the compiler knows to be a single thread: what the elected lane does with
+// warp-uniform values stays in uniform registers, which the tensor-core instructions take their operands from. (Issued
+// under `lane == 0` an instruction took about 130 clocks, more than most of the products.)
+__device__ __forceinline__ bool kv4_elect() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+  return p != 0;
+}
+
 template <int D>
 struct Kv4PreShape {
   static constexpr int SUB = D == 256 ? 1 : 2;           // query tiles of 128 rows
@@ -57,14 +69,17 @@ struct Kv4PreShape {
   static constexpr int TILE_BYTES = BLK * HALVES * 128;  // one expanded K or V tile
   static constexpr int TILES = 4;                        // K, V, K, V
   static constexpr int Q_BYTES = 128 * HALVES * 128;     // one query tile
-  static constexpr int RAW_TOKENS = 64;                  // a raw slot: packed K or V rows of 64 positions
-  static constexpr int RAW_BYTES = RAW_TOKENS * ROW;
-  static constexpr int RAW_PER_TILE = BLK / RAW_TOKENS;
-  static constexpr int RAW_SLOTS = D == 256 ? 3 : 6;
+  static constexpr int RAW_BYTES = BLK * ROW;            // a raw slot: packed K or V rows of a block
+  static constexpr int RAW_SLOTS = 3;
+  static constexpr int CHUNKS = BLK / 32;                // a warp expands 32 positions; with two chunks for the four
+  static constexpr int SHARES = 4 / CHUNKS;              // warps, two warps share the channels of each
   static constexpr int OFF_TILE = SUB * Q_BYTES;
   static constexpr int OFF_RAW = OFF_TILE + TILES * TILE_BYTES;
   static constexpr int SMEM = OFF_RAW + RAW_SLOTS * RAW_BYTES + 1024;
-  static constexpr int THREADS = SUB * 128 + 128 + 64;
+  // Two query tiles: four warpgroups that share the launch's 4 x 128 registers per thread as 168 + 168 + 96 + 80 (the
+  // last holds the copying and the issuing warp and two idle ones). One tile: 320 threads have registers to spare.
+  static constexpr bool SPLIT = SUB == 2;
+  static constexpr int THREADS = SPLIT ? 512 : SUB * 128 + 128 + 64;
   static constexpr int O_COL = SUB == 2 ? 256 : 128;     // TMEM: S tiles first, then O
   static constexpr int O_STEP = 128;
 };
@@ -91,7 +106,21 @@ __device__ __forceinline__ void kv4_tmem_st32(uint32_t taddr, const uint32_t* r)
       "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
       : "memory");
 }
+__device__ __forceinline__ void kv4_tmem_st16(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+      "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
 __device__ __forceinline__ void kv4_tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+template <int N, bool UP>
+__device__ __forceinline__ void kv4_set_regs() {
+  if constexpr (UP) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+  else asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
 
 // What a CTA needs to know of its tile, found by all threads together.
 struct Kv4Tile {
@@ -106,6 +135,7 @@ __global__ void __launch_bounds__(Kv4PreShape<D>::THREADS, 1) kv4_prefill_kernel
   using Shape = Kv4PreShape<D>;
   constexpr int SUB = Shape::SUB, BLK = Shape::BLK, ROW = Shape::ROW;
   constexpr int GROUPS = D / KV4_GROUP;
+  constexpr bool BF16 = Kv4Type<T>::IS_BF16;
   pdl_launch_dependents();
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -113,6 +143,7 @@ __global__ void __launch_bounds__(Kv4PreShape<D>::THREADS, 1) kv4_prefill_kernel
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_word;
   __shared__ Kv4Tile info;
+  __shared__ int exps[4][2][Shape::CHUNKS];  // bf16: exponents of a block's K and V chunks; blocks j - 3 .. j are live
   uint64_t* raw_full = bars;
   uint64_t* raw_empty = raw_full + Shape::RAW_SLOTS;
   uint64_t* tile_full = raw_empty + Shape::RAW_SLOTS;
@@ -216,7 +247,9 @@ __global__ void __launch_bounds__(Kv4PreShape<D>::THREADS, 1) kv4_prefill_kernel
   const int nmax = SUB == 2 ? max(nblk[0], nblk[1]) : nblk[0];
   auto base_of = [&](int j) { return (!EXT || j0 + j < sink_blks ? j0 + j : j0 + j + skip) * BLK; };
 
-  if (warp == COPIER) {
+  if (warp >= COPIER) {
+   if constexpr (Shape::SPLIT) kv4_set_regs<80, false>();
+   if (warp == COPIER) {
     // ---------------------------------------------------------------- packed rows -> raw ring
     bool ok = true;
     int m = 0;  // raw slots so far
@@ -231,71 +264,78 @@ __global__ void __launch_bounds__(Kv4PreShape<D>::THREADS, 1) kv4_prefill_kernel
         }
         if (mine < 0) mine = 0;  // released by a sliding window: every position of it is masked
       }
-      for (int n = 0; n < 2 * Shape::RAW_PER_TILE && ok; ++n, ++m) {
-        const int kv = n / Shape::RAW_PER_TILE, part = n % Shape::RAW_PER_TILE;
+      const int here = max(0, min(BLK / KV4_PAGE, held - pg0));  // pages of this block that exist
+      for (int kv = 0; kv < 2; ++kv, ++m) {
         const int s = m % Shape::RAW_SLOTS;
         if (m >= Shape::RAW_SLOTS) {
           ok = mbar_wait(&raw_empty[s], ((m / Shape::RAW_SLOTS) & 1) ^ 1, abort_flag, p.status, ERR_WAIT_PRODUCER);
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
         }
-        const int first = part * 4, here = max(0, min(4, held - pg0 - first));  // pages of this slot that exist
         if (lane == 0) mbar_expect_tx(&raw_full[s], here * Shape::PAGE_BYTES);
         __syncwarp();
-        const int pg = __shfl_sync(0xffffffffu, mine, first + (lane & 3));
         if (lane < here) {
-          const size_t block = (static_cast<size_t>(pg) * 2 + kv) * p.hkv + hk;
+          const size_t block = (static_cast<size_t>(mine) * 2 + kv) * p.hkv + hk;
           bulk_load(smem + Shape::OFF_RAW + s * Shape::RAW_BYTES + lane * Shape::PAGE_BYTES,
                     p.pages + block * Shape::PAGE_BYTES, Shape::PAGE_BYTES, &raw_full[s]);
         }
       }
     }
-  } else if (warp == ISSUER) {
+   } else if (warp == ISSUER) {
     // ---------------------------------------------------------------- tensor core
-    if (lane == 0 && nmax > 0) {
-      const uint32_t idesc_qk = umma_idesc(Kv4Type<T>::IS_BF16 ? 1 : 0, 128, BLK, 0, 0);
-      const uint32_t idesc_pv = umma_idesc(Kv4Type<T>::IS_BF16 ? 1 : 0, 128, D, 0, 1);
-      bool ok = mbar_wait(q_ready, 0, abort_flag, p.status, ERR_WAIT_PRODUCER);
+    if (nmax > 0) {
+      const uint32_t idesc_qk = umma_idesc(0, 128, BLK, 0, 0);
+      const uint32_t idesc_pv = umma_idesc(0, 128, D, 0, 1);
+      bool ok = __all_sync(0xffffffffu, mbar_wait(q_ready, 0, abort_flag, p.status, ERR_WAIT_PRODUCER));
       auto tile_wait = [&](int n) {
-        return mbar_wait(&tile_full[n % Shape::TILES], (n / Shape::TILES) & 1, abort_flag, p.status, ERR_WAIT_DEQUANT);
+        return __all_sync(0xffffffffu, mbar_wait(&tile_full[n % Shape::TILES], (n / Shape::TILES) & 1, abort_flag, p.status,
+                                                 ERR_WAIT_DEQUANT)) != 0;
       };
       auto s_col = [&](int i, int j) { return tmem + (SUB == 2 ? i * 128 : (j & 1) * BLK); };
       auto qk = [&](int i, int j) {
-        const uint32_t sq = smem_u32(smem + i * Shape::Q_BYTES);
-        const uint32_t sk = smem_u32(smem + Shape::OFF_TILE + (2 * j) % Shape::TILES * Shape::TILE_BYTES);
+        const uint64_t da = umma_smem_desc(smem_u32(smem + i * Shape::Q_BYTES), 16, 1024);
+        const uint64_t db = umma_smem_desc(smem_u32(smem + Shape::OFF_TILE + (2 * j) % Shape::TILES * Shape::TILE_BYTES), 16, 1024);
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) {
-          const uint64_t a = umma_smem_desc(sq + (kk >> 2) * (128 * 128) + (kk & 3) * 32, 16, 1024);
-          const uint64_t b = umma_smem_desc(sk + (kk >> 2) * (BLK * 128) + (kk & 3) * 32, 16, 1024);
+          const uint64_t a = da + ((kk >> 2) * (128 * 128) + (kk & 3) * 32) / 16;
+          const uint64_t b = db + ((kk >> 2) * (BLK * 128) + (kk & 3) * 32) / 16;
           umma_f16(s_col(i, j), a, b, idesc_qk, kk ? 1u : 0u);
         }
         umma_commit(&s_full[SUB == 2 ? i : j & 1]);
       };
       auto pv = [&](int i, int j) {
-        const uint32_t sv = smem_u32(smem + Shape::OFF_TILE + (2 * j + 1) % Shape::TILES * Shape::TILE_BYTES);
+        const uint64_t dv = umma_smem_desc(smem_u32(smem + Shape::OFF_TILE + (2 * j + 1) % Shape::TILES * Shape::TILE_BYTES), BLK * 128, 1024);
 #pragma unroll
         for (int kk = 0; kk < BLK / 16; ++kk) {
           // V: MN-major, 64-wide atoms along channels (LBO), 8-position groups (SBO)
-          const uint64_t b = umma_smem_desc(sv + kk * 2048, BLK * 128, 1024);
+          const uint64_t b = dv + kk * 2048 / 16;
           kv4_umma_ts(tmem + Shape::O_COL + i * Shape::O_STEP, s_col(i, j) + kk * 8, b, idesc_pv, (j | kk) ? 1u : 0u);
         }
         if (SUB == 1) umma_commit(pv_done);
       };
+      auto one = [&](auto&& f) {
+        if (kv4_elect()) f();
+        __syncwarp();
+      };
       ok = ok && tile_wait(0);
       if (ok) {
         tc_fence_after();
+        one([&] {
 #pragma unroll
-        for (int i = 0; i < SUB; ++i)
-          if (nblk[i] > 0) qk(i, 0);
-        umma_commit(&tile_empty[0]);
+          for (int i = 0; i < SUB; ++i)
+            if (nblk[i] > 0) qk(i, 0);
+          umma_commit(&tile_empty[0]);
+        });
       }
       for (int j = 0; j < nmax && ok; ++j) {
         if (SUB == 1 && j + 1 < nmax) {
           ok = tile_wait(2 * j + 2);
           if (!ok) break;
           tc_fence_after();
-          qk(0, j + 1);
-          umma_commit(&tile_empty[(2 * j + 2) % Shape::TILES]);
+          one([&] {
+            qk(0, j + 1);
+            umma_commit(&tile_empty[(2 * j + 2) % Shape::TILES]);
+          });
         }
         ok = tile_wait(2 * j + 1);
 #pragma unroll
@@ -303,102 +343,146 @@ __global__ void __launch_bounds__(Kv4PreShape<D>::THREADS, 1) kv4_prefill_kernel
           if (!ok || j >= nblk[i]) continue;
           ok = SUB == 2 ? mbar_wait(&p_full[i], j & 1, abort_flag, p.status, ERR_WAIT_EPILOGUE)
                         : mbar_wait(&p_full[j & 1], (j >> 1) & 1, abort_flag, p.status, ERR_WAIT_EPILOGUE);
+          ok = __all_sync(0xffffffffu, ok);
           if (!ok) continue;
           tc_fence_after();
-          pv(i, j);
-          if (j + 1 == nblk[i]) umma_commit(&o_done[i]);
+          one([&] {
+            pv(i, j);
+            if (j + 1 == nblk[i]) umma_commit(&o_done[i]);
+          });
           if (SUB == 2 && j + 1 < nblk[i]) {
             ok = tile_wait(2 * j + 2);
             if (!ok) continue;
             tc_fence_after();
-            qk(i, j + 1);
+            one([&] { qk(i, j + 1); });
           }
         }
         if (!ok) break;
-        umma_commit(&tile_empty[(2 * j + 1) % Shape::TILES]);
-        if (SUB == 2 && j + 1 < nmax) umma_commit(&tile_empty[(2 * j + 2) % Shape::TILES]);
+        one([&] {
+          umma_commit(&tile_empty[(2 * j + 1) % Shape::TILES]);
+          if (SUB == 2 && j + 1 < nmax) umma_commit(&tile_empty[(2 * j + 2) % Shape::TILES]);
+        });
       }
     }
+   }
   } else if (warp >= SUB * 4) {
     // ---------------------------------------------------------------- expanding warps
-    // A warp takes 32 of a raw slot's 64 positions and half of the groups; lane = position, so the 16-byte loads
-    // (row pitch 5/8 D bytes) and the swizzled 16-byte stores are free of bank conflicts.
+    if constexpr (Shape::SPLIT) kv4_set_regs<96, false>();
+    // A warp takes 32 positions of a block, lane = position, so the loads (row pitch 5/8 D bytes) and the swizzled
+    // 16-byte stores are free of bank conflicts.
     const int w = warp - SUB * 4;
-    const int token = (w & 1) * 32 + lane;
+    const int chunk = w % Shape::CHUNKS, token = chunk * 32 + lane;
+    constexpr int MINE = (GROUPS + Shape::SHARES - 1) / Shape::SHARES;
+    const int g0 = w / Shape::CHUNKS * MINE;
     const int reach = max(info.reach[0], SUB == 2 ? info.reach[1] : 0);
     const int first = EXT && p.q_kvstart ? info.first : 0;
     bool ok = true;
-    int m = 0;
     for (int n = 0; n < 2 * nmax && ok; ++n) {
+      const int j = n >> 1;
       const int b = n % Shape::TILES;
       if (n >= Shape::TILES) {
         ok = mbar_wait(&tile_empty[b], ((n / Shape::TILES) & 1) ^ 1, abort_flag, p.status, ERR_WAIT_MMA);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
       }
-      uint8_t* dst = smem + Shape::OFF_TILE + b * Shape::TILE_BYTES;
-      const int base = base_of(n >> 1);
-      for (int part = 0; part < Shape::RAW_PER_TILE; ++part, ++m) {
-        const int s = m % Shape::RAW_SLOTS;
-        ok = mbar_wait(&raw_full[s], (m / Shape::RAW_SLOTS) & 1, abort_flag, p.status, ERR_WAIT_TMA);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-        const uint8_t* src = smem + Shape::OFF_RAW + s * Shape::RAW_BYTES + token * ROW;
-        const int at = part * Shape::RAW_TOKENS + token;  // position in the block
-        // V of a position that no row sees counts as 0 whatever its bytes hold (P is 0 there; 0 * NaN is not)
-        const bool live = !(n & 1) || (base + at < reach && base + at < room && (base + at >= first || base + at < p.sink));
-        uint8_t* row = dst + at * 128;
-#pragma unroll
-        for (int gi = 0; gi < (GROUPS + 1) / 2; ++gi) {
-          const int g = gi * 2 + (w >> 1);
-          if (GROUPS % 2 && g >= GROUPS) break;
-          uint32_t c[4];
-          if constexpr (ROW % 16 == 0) {
-            kv4_words<4>(src + g * 16, c);
-          } else {
-#pragma unroll
-            for (int x = 0; x < 4; ++x) c[x] = reinterpret_cast<const uint32_t*>(src)[g * 4 + x];
-          }
-          uint32_t meta = reinterpret_cast<const uint32_t*>(src + D / 2)[g];
-          if (!live) meta = 0u;
-          const uint32_t lo2 = __byte_perm(meta, meta, 0x1010), s2 = __byte_perm(meta, meta, 0x3232);
-#pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            uint32_t v[4];
-            Kv4Type<T>::expand4(c[x], s2, lo2, v);
-            const int chunk = (g & 1) * 4 + x;  // 16-byte chunk of the 64-channel atom
-            *reinterpret_cast<uint4*>(row + (g >> 1) * (BLK * 128) + ((chunk ^ (at & 7)) << 4)) =
-                make_uint4(v[0], v[1], v[2], v[3]);
-          }
-        }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&raw_empty[s]);
-      }
+      const int s = n % Shape::RAW_SLOTS;
+      ok = mbar_wait(&raw_full[s], (n / Shape::RAW_SLOTS) & 1, abort_flag, p.status, ERR_WAIT_TMA);
+      ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
+      const uint8_t* src = smem + Shape::OFF_RAW + s * Shape::RAW_BYTES + token * ROW;
+      uint8_t* row = smem + Shape::OFF_TILE + b * Shape::TILE_BYTES + token * 128;
+      // a position that no row sees counts as 0 whatever its bytes hold (its weight is 0, but 0 * NaN is not)
+      const int at = base_of(j) + token;
+      const bool live = at < reach && at < room && (at >= first || at < p.sink);
+      const uint32_t* pairs = reinterpret_cast<const uint32_t*>(src + D / 2);
+      uint32_t meta[MINE];
+#pragma unroll
+      for (int i = 0; i < MINE; ++i) meta[i] = live ? pairs[g0 + i] : 0u;
+      float shrink = 1.f;
+      if constexpr (BF16) {
+        // |v| <= |lo| + 15 s: with |lo| < 2^(e + 13) and s < 2^(e + 9) the scaled values stay below 2^14; in steps of 4
+        uint32_t top = 0;
+#pragma unroll
+        for (int i = 0; i < MINE; ++i) top = __vmaxu2(top, meta[i] & 0xffff7fffu);
+        if constexpr (Shape::SHARES == 2) {  // the other warp's groups count too: both warps come to the same exponent
+#pragma unroll
+          for (int i = 0; i < MINE; ++i) top = __vmaxu2(top, live ? pairs[(g0 ^ MINE) + i] & 0xffff7fffu : 0u);
+        }
+        const int need = max(static_cast<int>(top >> 23) - 9, static_cast<int>((top & 0xffffu) >> 7) - 13) - 126;
+        const int e = max((__reduce_max_sync(0xffffffffu, need) + 1027) / 4 * 4 - 1024, -120);
+        if (lane == 0) exps[j & 3][n & 1][chunk] = e;
+        shrink = exp2f(static_cast<float>(-e));
+      }
+#pragma unroll
+      for (int i = 0; i < MINE; ++i) {
+        const int g = g0 + i;
+        uint32_t c[4], lo2, s2;
+        if constexpr (ROW % 16 == 0) {
+          kv4_words<4>(src + g * 16, c);
+        } else {
+#pragma unroll
+          for (int x = 0; x < 4; ++x) c[x] = reinterpret_cast<const uint32_t*>(src)[g * 4 + x];
+        }
+        if constexpr (BF16) {
+          const float lo = __uint_as_float(meta[i] << 16) * shrink, st = __uint_as_float(meta[i] & 0xffff0000u) * shrink;
+          lo2 = Kv4Type<__half>::pack(lo, lo);
+          s2 = Kv4Type<__half>::pack(st, st);
+        } else {
+          lo2 = __byte_perm(meta[i], meta[i], 0x1010);
+          s2 = __byte_perm(meta[i], meta[i], 0x3232);
+        }
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          uint32_t v[4];
+          Kv4Type<__half>::expand4(c[x], s2, lo2, v);
+          const int unit = (g & 1) * 4 + x;  // 16-byte unit of the 64-channel atom
+          *reinterpret_cast<uint4*>(row + (g >> 1) * (BLK * 128) + ((unit ^ (token & 7)) << 4)) =
+              make_uint4(v[0], v[1], v[2], v[3]);
+        }
+      }
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&tile_full[b]);
+      if (lane == 0) {
+        mbar_arrive(&raw_empty[s]);
+        mbar_arrive(&tile_full[b]);
+      }
     }
   } else {
     // ---------------------------------------------------------------- softmax / epilogue
+    if constexpr (Shape::SPLIT) kv4_set_regs<168, true>();
     const int sub = warp >> 2;
     const int row = threadIdx.x & 127;                 // row of the tile
     const int grow = sub * 128 + row;                  // row of the CTA
     const bool row_valid = grow < valid_rows;
     const bool warp_active = sub * 128 + (warp & 3) * 32 < valid_rows;
     const int tok = qstart + (row_valid ? (row0 + grow) / G : 0), head = hk * G + (row_valid ? (row0 + grow) % G : 0);
+    float row_scale = 1.f;  // of the scores, undoing that of the staged query row
     {
       const uint4* src = reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(p.q) +
                                                         (static_cast<size_t>(tok) * p.q_stride + static_cast<size_t>(head) * D) * 2);
       uint8_t* dst = smem + sub * Shape::Q_BYTES + row * 128;
+      float q_scale = 1.f;
+      if constexpr (BF16) {
+        // into fp16 with the row's largest magnitude in [2^10, 2^11); infinity and NaN stay what they are
+        uint32_t top = 0;
+#pragma unroll
+        for (int c = 0; c < D / 8; ++c) {
+          const uint4 v = row_valid ? src[c] : make_uint4(0, 0, 0, 0);
+          top = __vmaxu2(__vmaxu2(top, __vmaxu2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu)), __vmaxu2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu));
+        }
+        const int e = max(static_cast<int>(max(top & 0xffffu, top >> 16) >> 7) - 127 - 10, -120);
+        q_scale = exp2f(static_cast<float>(-e));
+        row_scale = exp2f(static_cast<float>(e));
+      }
 #pragma unroll
       for (int c = 0; c < D / 8; ++c) {
         uint4 v = row_valid ? src[c] : make_uint4(0, 0, 0, 0);
-        if (row_valid) {
-          v.x ^= p.q_flip;
-          v.y ^= p.q_flip;
-          v.z ^= p.q_flip;
-          v.w ^= p.q_flip;
+        uint32_t* x = reinterpret_cast<uint32_t*>(&v);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          x[i] ^= p.q_flip;
+          if constexpr (BF16)
+            x[i] = Kv4Type<__half>::pack(__uint_as_float(x[i] << 16) * q_scale, __uint_as_float(x[i] & 0xffff0000u) * q_scale);
         }
         *reinterpret_cast<uint4*>(dst + (c >> 3) * (128 * 128) + (((c & 7) ^ (row & 7)) << 4)) = v;
       }
@@ -413,15 +497,27 @@ __global__ void __launch_bounds__(Kv4PreShape<D>::THREADS, 1) kv4_prefill_kernel
       if (p.q_kvstart) start = p.q_kvstart[tok];
       if (p.tree_mask) tm = p.tree_mask[tok];
     }
-    const float scale = EXT && p.cap_log2 != 0.f ? 1.f : p.scale_log2;
     const int mine = sub ? nblk[1] : nblk[0], all_to = info.all_to[sub], all_from = info.all_from[sub];
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t t_o = tmem + lanes + Shape::O_COL + sub * Shape::O_STEP;
     float m_ref = -INFINITY, l = 0.f;
+    int v_exp = -1000;  // bf16: O holds sums of V * 2^-v_exp
     bool ok = true;
     for (int j = 0; j < mine && ok; ++j) {
-      ok = SUB == 2 ? mbar_wait(&s_full[sub], j & 1, abort_flag, p.status, ERR_WAIT_MMA)
-                    : mbar_wait(&s_full[j & 1], (j >> 1) & 1, abort_flag, p.status, ERR_WAIT_MMA);
+      // bf16: the exponents of the block's K and V (the warps that expanded V wrote both before they released it)
+      int k_exp[Shape::CHUNKS], v_log[Shape::CHUNKS], v_top = v_exp;
+      if constexpr (BF16) {
+        const int n = 2 * j + 1;
+        ok = mbar_wait(&tile_full[n % Shape::TILES], (n / Shape::TILES) & 1, abort_flag, p.status, ERR_WAIT_DEQUANT);
+#pragma unroll
+        for (int c = 0; c < Shape::CHUNKS; ++c) {
+          k_exp[c] = exps[j & 3][0][c];
+          v_log[c] = exps[j & 3][1][c];
+          v_top = max(v_top, v_log[c]);
+        }
+      }
+      ok = ok && (SUB == 2 ? mbar_wait(&s_full[sub], j & 1, abort_flag, p.status, ERR_WAIT_MMA)
+                           : mbar_wait(&s_full[j & 1], (j >> 1) & 1, abort_flag, p.status, ERR_WAIT_MMA));
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       tc_fence_after();
@@ -429,58 +525,52 @@ __global__ void __launch_bounds__(Kv4PreShape<D>::THREADS, 1) kv4_prefill_kernel
       if (warp_active) {
         const int base = base_of(j);
         const bool plain = base + BLK <= all_to && (!EXT || base >= all_from || base + BLK <= p.sink);
-        uint32_t pk[BLK / 2];
-        float sum = 0.f, mx = -INFINITY;
-        // 32 columns: scores, their maximum, weights against the reference `shift` = -m
-        auto columns = [&](int c, float shift, bool weights) {
-          uint32_t r[32];
-          __syncwarp();
-          tmem_ld32(t_s + c * 32, r);
-          tmem_ld_wait();
-          if (EXT && p.cap_log2 != 0.f) {
+        const bool capped = EXT && p.cap_log2 != 0.f;
+        // ---- maximum of the block's scores, 32 columns at a time (log2 units). Capped and masked ones are written back.
+        float scale[BLK / 32], mx = -INFINITY;
+        uint32_t r[2][32];
+        __syncwarp();
+        tmem_ld32(t_s, r[0]);
 #pragma unroll
-            for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(kv4_softcap(__uint_as_float(r[i]), p.cap_k, p.cap_log2));
+        for (int c = 0; c < BLK / 32; ++c) {
+          uint32_t (&x)[32] = r[c & 1];
+          const float undo = BF16 ? row_scale * exp2f(static_cast<float>(k_exp[c])) : row_scale;
+          // (not 0 where zeros scaled it away: a hidden score is -inf * scale)
+          scale[c] = capped ? 1.f : fmaxf(p.scale_log2 * undo, 1e-30f);
+          tmem_ld_wait();
+          if (c + 1 < BLK / 32) tmem_ld32(t_s + (c + 1) * 32, r[(c + 1) & 1]);
+          if (capped) {
+            const float k = p.cap_k * undo;
+#pragma unroll
+            for (int i = 0; i < 32; ++i) x[i] = __float_as_uint(kv4_softcap(__uint_as_float(x[i]), k, p.cap_log2));
           }
           if (!plain) {
 #pragma unroll
             for (int i = 0; i < 32; ++i)
-              if (!kv4_visible(base + c * 32 + i, kvlen, start, EXT ? p.sink : 0, tm)) r[i] = 0xff800000u;
+              if (!kv4_visible(base + c * 32 + i, kvlen, start, EXT ? p.sink : 0, tm)) x[i] = 0xff800000u;
           }
-          if (!weights) {
+          if (capped || !plain) kv4_tmem_st32(t_s + c * 32, x);
+          float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-            for (int i = 0; i < 32; ++i) mx = fmaxf(mx, __uint_as_float(r[i]));
-            return;
+          for (int i = 0; i < 32; i += 4) {
+            top[0] = fmaxf(top[0], fmaxf(__uint_as_float(x[i]), __uint_as_float(x[i + 1])));
+            top[1] = fmaxf(top[1], fmaxf(__uint_as_float(x[i + 2]), __uint_as_float(x[i + 3])));
           }
-          float2 acc = make_float2(0.f, 0.f);
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const float2 v = make_float2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
-            mx = fmaxf(mx, fmaxf(v.x, v.y));
-            const float2 x = kv4_fma2(v, make_float2(scale, scale), make_float2(shift, shift));
-            const float2 e = make_float2(exp2f(x.x), exp2f(x.y));
-            acc = kv4_add2(acc, e);
-            pk[c * 16 + i] = Kv4Type<T>::pack(e.x, e.y);
-          }
-          sum += acc.x + acc.y;
-        };
-        bool redo = j == 0;
-        if (j > 0) {
-          const float shift = m_ref == -INFINITY ? 0.f : -m_ref;
-#pragma unroll
-          for (int c = 0; c < BLK / 32; ++c) columns(c, shift, true);
-          redo = mx * scale > m_ref + 8.f;
-        } else {
-#pragma unroll
-          for (int c = 0; c < BLK / 32; ++c) columns(c, 0.f, false);
+          mx = fmaxf(mx, fmaxf(top[0], top[1]) * scale[c]);
         }
-        if (__any_sync(0xffffffffu, redo)) {
-          const float m_new = fmaxf(m_ref, mx * scale);
+        if (capped || !plain) kv4_tmem_st_wait();
+        tmem_ld32(t_s, r[0]);
+        // ---- raise the reference (and the exponent of V) where the block needs it
+        if (__any_sync(0xffffffffu, mx > m_ref + 8.f || v_top > v_exp)) {
+          const float m_new = fmaxf(m_ref, mx);
           const float alpha = m_ref == -INFINITY ? 0.f : exp2f(m_ref - m_new);
+          // (the first block finds O undefined and leaves it alone; rows that saw nothing so far hold zeros)
+          const float o_alpha = BF16 ? alpha * exp2f(static_cast<float>(max(v_exp - v_top, -126))) : alpha;
+          v_exp = v_top;
           if (j > 0) {
             if (SUB == 1) {  // the scores of this block were computed before the last P V ended
               ok = mbar_wait(pv_done, (j - 1) & 1, abort_flag, p.status, ERR_WAIT_MMA);
               ok = __all_sync(0xffffffffu, ok);
-              if (!ok) break;
               tc_fence_after();
             }
 #pragma unroll 1
@@ -489,20 +579,36 @@ __global__ void __launch_bounds__(Kv4PreShape<D>::THREADS, 1) kv4_prefill_kernel
               tmem_ld32(t_o + c, o);
               tmem_ld_wait();
 #pragma unroll
-              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * o_alpha);
               kv4_tmem_st32(t_o + c, o);
             }
           }
           l *= m_ref == -INFINITY ? 1.f : alpha;
           m_ref = m_new;
-          sum = 0.f;
-          const float shift = m_ref == -INFINITY ? 0.f : -m_ref;
-#pragma unroll
-          for (int c = 0; c < BLK / 32; ++c) columns(c, shift, true);
         }
-        l += sum;
+        // ---- weights against the reference; they overwrite columns that were read before. bf16: they carry the scale
+        // 2^v_log of their V against the one of O, and their sum is relieved of it. (Behind 2^-60 no fp16 weight is left,
+        // while the sum still counts what fp32 has.)
 #pragma unroll
-        for (int c = 0; c < BLK / 64; ++c) kv4_tmem_st32(t_s + c * 32, pk + c * 32);
+        for (int c = 0; c < BLK / 32; ++c) {
+          uint32_t (&x)[32] = r[c & 1];
+          const float lift = BF16 ? static_cast<float>(max(v_log[c] - v_top, -60)) : 0.f;
+          const float shift = m_ref == -INFINITY ? 0.f : lift - m_ref;
+          tmem_ld_wait();
+          if (c + 1 < BLK / 32) tmem_ld32(t_s + (c + 1) * 32, r[(c + 1) & 1]);
+          float2 acc = make_float2(0.f, 0.f);
+          uint32_t w[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const float2 v = make_float2(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1]));
+            const float2 y = kv4_fma2(v, make_float2(scale[c], scale[c]), make_float2(shift, shift));
+            const float2 e = make_float2(exp2f(y.x), exp2f(y.y));
+            acc = kv4_add2(acc, e);
+            w[i] = Kv4Type<__half>::pack(e.x, e.y);
+          }
+          l += BF16 ? (acc.x + acc.y) * exp2f(-lift) : acc.x + acc.y;
+          kv4_tmem_st16(t_s + c * 16, w);
+        }
         kv4_tmem_st_wait();
       }
       tc_fence_before();
@@ -516,7 +622,8 @@ __global__ void __launch_bounds__(Kv4PreShape<D>::THREADS, 1) kv4_prefill_kernel
     }
     if (ok && warp_active) {
       tc_fence_after();
-      const float inv = l == 0.f ? 0.f : 1.f / l;  // a row that sees nothing is 0; NaN stays NaN
+      const float grow_v = BF16 && mine > 0 ? exp2f(static_cast<float>(v_exp)) : 1.f;
+      const float inv = l == 0.f ? 0.f : 1.f / l * grow_v;  // a row that sees nothing is 0; NaN stays NaN
       const size_t prow = ((static_cast<size_t>(work) * p.hkv + hk) * p.splits + split) * (SUB * 128) + grow;
 #pragma unroll 1
       for (int c = 0; c < D; c += 32) {
@@ -533,7 +640,9 @@ __global__ void __launch_bounds__(Kv4PreShape<D>::THREADS, 1) kv4_prefill_kernel
           float* dst = p.part_o + prow * D + c;
 #pragma unroll
           for (int i = 0; i < 8; ++i)
-            reinterpret_cast<uint4*>(dst)[i] = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+            reinterpret_cast<float4*>(dst)[i] =
+                make_float4(__uint_as_float(o[4 * i]) * grow_v, __uint_as_float(o[4 * i + 1]) * grow_v,
+                            __uint_as_float(o[4 * i + 2]) * grow_v, __uint_as_float(o[4 * i + 3]) * grow_v);
         } else if (row_valid) {
           uint8_t* dst = reinterpret_cast<uint8_t*>(p.out) + ((static_cast<size_t>(tok) * p.hq + head) * D + c) * 2;
 #pragma unroll
