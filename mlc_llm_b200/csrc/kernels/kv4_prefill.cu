@@ -163,6 +163,8 @@ __global__ void __launch_bounds__(Kv4PreShape<D>::THREADS, 1) kv4_prefill_kernel
   const int tile = work / p.parts, row0 = work % p.parts * 128;  // first row of the tile that is this CTA's
   const int seq = p.tile_seq[tile], qstart = p.tile_qstart[tile], ntok = p.tile_ntok[tile];
   const int valid_rows = max(0, min(ntok * G - row0, SUB * 128));
+  const int p0 = p.page_indptr[seq];
+  const int held = p.page_indptr[seq + 1] - p0;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < Shape::RAW_SLOTS; ++i) {
@@ -216,8 +218,6 @@ __global__ void __launch_bounds__(Kv4PreShape<D>::THREADS, 1) kv4_prefill_kernel
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
-  const int p0 = p.page_indptr[seq];
-  const int held = p.page_indptr[seq + 1] - p0;
   const int* list = p.page_indices + p0;
   const long long room = static_cast<long long>(held) * KV4_PAGE;
   if (threadIdx.x == 0 && p.status && max(info.reach[0], info.reach[1]) > room) atomicCAS(p.status, 0, ERR_BAD_INDEX);
@@ -456,46 +456,71 @@ __global__ void __launch_bounds__(Kv4PreShape<D>::THREADS, 1) kv4_prefill_kernel
     const bool row_valid = grow < valid_rows;
     const bool warp_active = sub * 128 + (warp & 3) * 32 < valid_rows;
     const int tok = qstart + (row_valid ? (row0 + grow) / G : 0), head = hk * G + (row_valid ? (row0 + grow) % G : 0);
-    float row_scale = 1.f;  // of the scores, undoing that of the staged query row
-    {
-      const uint4* src = reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(p.q) +
-                                                        (static_cast<size_t>(tok) * p.q_stride + static_cast<size_t>(head) * D) * 2);
-      uint8_t* dst = smem + sub * Shape::Q_BYTES + row * 128;
-      float q_scale = 1.f;
-      if constexpr (BF16) {
-        // into fp16 with the row's largest magnitude in [2^10, 2^11); infinity and NaN stay what they are
-        uint32_t top = 0;
-#pragma unroll
-        for (int c = 0; c < D / 8; ++c) {
-          const uint4 v = row_valid ? src[c] : make_uint4(0, 0, 0, 0);
-          top = __vmaxu2(__vmaxu2(top, __vmaxu2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu)), __vmaxu2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu));
-        }
-        const int e = max(static_cast<int>(max(top & 0xffffu, top >> 16) >> 7) - 127 - 10, -120);
-        q_scale = exp2f(static_cast<float>(-e));
-        row_scale = exp2f(static_cast<float>(e));
-      }
-#pragma unroll
-      for (int c = 0; c < D / 8; ++c) {
-        uint4 v = row_valid ? src[c] : make_uint4(0, 0, 0, 0);
-        uint32_t* x = reinterpret_cast<uint32_t*>(&v);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          x[i] ^= p.q_flip;
-          if constexpr (BF16)
-            x[i] = Kv4Type<__half>::pack(__uint_as_float(x[i] << 16) * q_scale, __uint_as_float(x[i] & 0xffff0000u) * q_scale);
-        }
-        *reinterpret_cast<uint4*>(dst + (c >> 3) * (128 * 128) + (((c & 7) ^ (row & 7)) << 4)) = v;
-      }
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(q_ready);
-    }
     const int kvlen = row_valid ? p.q_kvlen[tok] : 0;
     int start = 0;
     unsigned long long tm = 0ull;
     if (EXT && row_valid) {
       if (p.q_kvstart) start = p.q_kvstart[tok];
       if (p.tree_mask) tm = p.tree_mask[tok];
+    }
+    float row_scale = 1.f;  // of the scores, undoing that of the staged query row
+    {
+      // Query rows: the warp loads its 32 whole, neighbouring lanes neighbouring bytes, a batch of loads at a time (one
+      // thread per row and load after load took 9000 clocks for 32 KB).
+      constexpr int UNITS = D / 8, BATCH = UNITS % 8 ? 6 : 8;  // 16-byte units of a row
+      static_assert(UNITS % BATCH == 0, "whole batches");
+      uint8_t* tile = smem + sub * Shape::Q_BYTES;
+      auto place = [&](int r, int c) { return reinterpret_cast<uint4*>(tile + r * 128 + (c >> 3) * (128 * 128) + (((c & 7) ^ (r & 7)) << 4)); };
+#pragma unroll 1
+      for (int b = 0; b < UNITS; b += BATCH) {
+        uint4 v[BATCH];
+#pragma unroll
+        for (int i = 0; i < BATCH; ++i) {
+          const int at = (b + i) * 32 + lane, r = row0 + sub * 128 + (warp & 3) * 32 + at / UNITS;
+          v[i] = make_uint4(0, 0, 0, 0);
+          if (r - row0 < valid_rows)
+            v[i] = reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(p.q) +
+                (static_cast<size_t>(qstart + r / G) * p.q_stride + static_cast<size_t>(hk * G + r % G) * D) * 2)[at % UNITS];
+        }
+#pragma unroll
+        for (int i = 0; i < BATCH; ++i) {
+          const int at = (b + i) * 32 + lane;
+          if constexpr (!BF16) {
+            v[i].x ^= p.q_flip;
+            v[i].y ^= p.q_flip;
+            v[i].z ^= p.q_flip;
+            v[i].w ^= p.q_flip;
+          }
+          *place((warp & 3) * 32 + at / UNITS, at % UNITS) = v[i];
+        }
+      }
+      __syncwarp();
+      if constexpr (BF16) {
+        // into fp16 with the row's largest magnitude in [2^10, 2^11); infinity and NaN stay what they are
+        uint32_t top = 0;
+#pragma unroll
+        for (int c = 0; c < UNITS; ++c) {
+          const uint4 v = *place(row, c);
+          top = __vmaxu2(__vmaxu2(top, __vmaxu2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu)), __vmaxu2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu));
+        }
+        const int e = max(static_cast<int>(max(top & 0xffffu, top >> 16) >> 7) - 127 - 10, -120);
+        const float q_scale = exp2f(static_cast<float>(-e));
+        row_scale = exp2f(static_cast<float>(e));
+#pragma unroll 4
+        for (int c = 0; c < UNITS; ++c) {
+          uint4 v = *place(row, c);
+          uint32_t* x = reinterpret_cast<uint32_t*>(&v);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            x[i] ^= p.q_flip;
+            x[i] = Kv4Type<__half>::pack(__uint_as_float(x[i] << 16) * q_scale, __uint_as_float(x[i] & 0xffff0000u) * q_scale);
+          }
+          *place(row, c) = v;
+        }
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(q_ready);
     }
     const int mine = sub ? nblk[1] : nblk[0], all_to = info.all_to[sub], all_from = info.all_from[sub];
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
@@ -625,6 +650,19 @@ __global__ void __launch_bounds__(Kv4PreShape<D>::THREADS, 1) kv4_prefill_kernel
       const float grow_v = BF16 && mine > 0 ? exp2f(static_cast<float>(v_exp)) : 1.f;
       const float inv = l == 0.f ? 0.f : 1.f / l * grow_v;  // a row that sees nothing is 0; NaN stays NaN
       const size_t prow = ((static_cast<size_t>(work) * p.hkv + hk) * p.splits + split) * (SUB * 128) + grow;
+      // By way of shared memory (this tile's queries are used up), so that neighbouring lanes write neighbouring bytes:
+      // 32 columns of the warp's rows, 8 units of 16 bytes each as fp32, 4 in the output's type.
+      const bool partial = p.splits > 1;
+      uint8_t* stage = smem + sub * Shape::Q_BYTES + (warp & 3) * 4096;
+      const int wrow0 = sub * 128 + (warp & 3) * 32;
+      uint8_t* part = reinterpret_cast<uint8_t*>(p.part_o) + (prow - lane) * D * 4;
+      uint8_t* dst[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int r = row0 + wrow0 + i * 8 + (lane >> 2);
+        dst[i] = r - row0 < valid_rows ? reinterpret_cast<uint8_t*>(p.out) +
+                     (static_cast<size_t>(qstart + r / G) * p.hq + hk * G + r % G) * D * 2 + (lane & 3) * 16 : nullptr;
+      }
 #pragma unroll 1
       for (int c = 0; c < D; c += 32) {
         uint32_t o[32];
@@ -636,22 +674,36 @@ __global__ void __launch_bounds__(Kv4PreShape<D>::THREADS, 1) kv4_prefill_kernel
 #pragma unroll
           for (int i = 0; i < 32; ++i) o[i] = 0;
         }
-        if (row_valid && p.splits > 1) {
-          float* dst = p.part_o + prow * D + c;
+        if (partial) {
 #pragma unroll
           for (int i = 0; i < 8; ++i)
-            reinterpret_cast<float4*>(dst)[i] =
+            *reinterpret_cast<float4*>(stage + lane * 128 + ((i ^ (lane & 7)) << 4)) =
                 make_float4(__uint_as_float(o[4 * i]) * grow_v, __uint_as_float(o[4 * i + 1]) * grow_v,
                             __uint_as_float(o[4 * i + 2]) * grow_v, __uint_as_float(o[4 * i + 3]) * grow_v);
-        } else if (row_valid) {
-          uint8_t* dst = reinterpret_cast<uint8_t*>(p.out) + ((static_cast<size_t>(tok) * p.hq + head) * D + c) * 2;
+          __syncwarp();
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int r = i * 4 + (lane >> 3);
+            if (wrow0 + r < valid_rows)
+              *reinterpret_cast<uint4*>(part + static_cast<size_t>(r) * D * 4 + c * 4 + (lane & 7) * 16) =
+                  *reinterpret_cast<const uint4*>(stage + r * 128 + (((lane & 7) ^ (r & 7)) << 4));
+          }
+        } else {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             uint32_t v[4];
 #pragma unroll
             for (int k = 0; k < 4; ++k)
               v[k] = Kv4Type<T>::pack(__uint_as_float(o[i * 8 + 2 * k]) * inv, __uint_as_float(o[i * 8 + 2 * k + 1]) * inv);
-            reinterpret_cast<uint4*>(dst)[i] = make_uint4(v[0], v[1], v[2], v[3]);
+            *reinterpret_cast<uint4*>(stage + lane * 64 + ((i ^ ((lane >> 1) & 3)) << 4)) = make_uint4(v[0], v[1], v[2], v[3]);
+          }
+          __syncwarp();
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int r = i * 8 + (lane >> 2);
+            if (dst[i])
+              *reinterpret_cast<uint4*>(dst[i] + c * 2) =
+                  *reinterpret_cast<const uint4*>(stage + r * 64 + (((lane & 3) ^ ((r >> 1) & 3)) << 4));
           }
         }
       }
