@@ -455,7 +455,11 @@ __global__ void __launch_bounds__(Kv4PreShape<D>::THREADS, 1) kv4_prefill_kernel
     const int grow = sub * 128 + row;                  // row of the CTA
     const bool row_valid = grow < valid_rows;
     const bool warp_active = sub * 128 + (warp & 3) * 32 < valid_rows;
-    const int tok = qstart + (row_valid ? (row0 + grow) / G : 0), head = hk * G + (row_valid ? (row0 + grow) % G : 0);
+    // row / G of rows below 2^20: (row + 1/2) / G is half a step of 1 / G away from any whole number
+    const float per_group = 1.f / static_cast<float>(G);
+    auto token_of = [&](int r) { return static_cast<int>((static_cast<float>(r) + 0.5f) * per_group); };
+    const int ahead_of_row = row_valid ? token_of(row0 + grow) : 0;
+    const int tok = qstart + ahead_of_row, head = hk * G + (row_valid ? row0 + grow - ahead_of_row * G : 0);
     const int kvlen = row_valid ? p.q_kvlen[tok] : 0;
     int start = 0;
     unsigned long long tm = 0ull;
@@ -471,16 +475,15 @@ __global__ void __launch_bounds__(Kv4PreShape<D>::THREADS, 1) kv4_prefill_kernel
       static_assert(UNITS % BATCH == 0, "whole batches");
       uint8_t* tile = smem + sub * Shape::Q_BYTES;
       auto place = [&](int r, int c) { return reinterpret_cast<uint4*>(tile + r * 128 + (c >> 3) * (128 * 128) + (((c & 7) ^ (r & 7)) << 4)); };
+      const uint8_t* q0 = reinterpret_cast<const uint8_t*>(p.q) + (static_cast<size_t>(qstart) * p.q_stride + static_cast<size_t>(hk) * G * D) * 2;
 #pragma unroll 1
       for (int b = 0; b < UNITS; b += BATCH) {
         uint4 v[BATCH];
 #pragma unroll
-        for (int i = 0; i < BATCH; ++i) {
-          const int at = (b + i) * 32 + lane, r = row0 + sub * 128 + (warp & 3) * 32 + at / UNITS;
-          v[i] = make_uint4(0, 0, 0, 0);
-          if (r - row0 < valid_rows)
-            v[i] = reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(p.q) +
-                (static_cast<size_t>(qstart + r / G) * p.q_stride + static_cast<size_t>(hk * G + r % G) * D) * 2)[at % UNITS];
+        for (int i = 0; i < BATCH; ++i) {  // rows behind the last are copies of it
+          const int at = (b + i) * 32 + lane, r = row0 + max(0, min(sub * 128 + (warp & 3) * 32 + at / UNITS, valid_rows - 1));
+          const int ahead = token_of(r);
+          v[i] = reinterpret_cast<const uint4*>(q0 + (ahead * p.q_stride + (r - ahead * G) * D) * 2)[at % UNITS];
         }
 #pragma unroll
         for (int i = 0; i < BATCH; ++i) {
@@ -660,17 +663,20 @@ __global__ void __launch_bounds__(Kv4PreShape<D>::THREADS, 1) kv4_prefill_kernel
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int r = row0 + wrow0 + i * 8 + (lane >> 2);
-        dst[i] = r - row0 < valid_rows ? reinterpret_cast<uint8_t*>(p.out) +
-                     (static_cast<size_t>(qstart + r / G) * p.hq + hk * G + r % G) * D * 2 + (lane & 3) * 16 : nullptr;
+        const int ahead = token_of(r);
+        dst[i] = reinterpret_cast<uint8_t*>(p.out) + (static_cast<size_t>(qstart + ahead) * p.hq + hk * G + r - ahead * G) * D * 2 + (lane & 3) * 16;
+        if (r - row0 >= valid_rows) dst[i] = nullptr;
       }
-#pragma unroll 1
+      uint32_t o2[2][32];
+      __syncwarp();
+      tmem_ld32(t_o, o2[0]);
+#pragma unroll
       for (int c = 0; c < D; c += 32) {
-        uint32_t o[32];
+        uint32_t (&o)[32] = o2[(c / 32) & 1];
+        tmem_ld_wait();
+        if (c + 32 < D) tmem_ld32(t_o + c + 32, o2[(c / 32 + 1) & 1]);
         __syncwarp();
-        if (mine > 0) {
-          tmem_ld32(t_o + c, o);
-          tmem_ld_wait();
-        } else {
+        if (mine == 0) {
 #pragma unroll
           for (int i = 0; i < 32; ++i) o[i] = 0;
         }
