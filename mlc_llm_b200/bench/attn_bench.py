@@ -40,10 +40,22 @@ def bench_attention(which: str, small: bool):
         cases += [("attn_decode", b, c, 1) for b, c in ([(64, 1024)] if small else [(256, 640), (256, 2048), (8, 16384)])]
     if which in ("attn_prefill", "all"):
         cases += [("attn_prefill", b, c, c) for b, c in ([(4, 1024)] if small else [(16, 512), (4, 4096), (1, 16384)])]
+    if which in ("attn_kv4", "all"):  # the same steps over a 4-bit cache
+        cases += [("attn_kv4", b, c, n) for b, c, n in ([(64, 1024, 1), (4, 1024, 1024)] if small else
+                                                        [(256, 640, 1), (256, 2048, 1), (8, 16384, 1), (16, 512, 512),
+                                                         (4, 4096, 4096), (1, 16384, 16384)])]
     for kind, batch, ctx, append in cases:
         pages = batch * ((ctx + 15) // 16)
-        kv = (torch.randn(pages, 2, hkv, 16, d, device=dev) * 0.5).half()
         plan = _plan(batch, ctx, append, hq, hkv, dev)
+        if kind == "attn_kv4":
+            kv = ops.kv4_cache(pages, hkv, d, 16, torch.float16, dev)
+            rows = (torch.randn(pages * 16, 2 * hkv * d, device=dev) * 0.5).half()
+            slots = torch.arange(pages * 16, device=dev, dtype=torch.int32)
+            ops.rope_append(rows, kv, slots, slots, None, 0, hkv, d, 0, 16)
+            del rows
+            plan = ops.kv4_plan(np.arange(batch + 1) * append, plan.q_kvlen, plan.page_indptr, plan.page_indices, hq, hkv, ctx)
+        else:
+            kv = (torch.randn(pages, 2, hkv, 16, d, device=dev) * 0.5).half()
         t = batch * append
         q = (torch.randn(t, (hq + 2 * hkv) * d, device=dev) * 0.5).half()
         q_seq = torch.arange(batch, device=dev, dtype=torch.int32).repeat_interleave(append)
@@ -52,8 +64,8 @@ def bench_attention(which: str, small: bool):
         med, best = _time(fn)
         in_graph = _time_graph(fn)   # the kernel alone: the eager figure carries the host's launch time
         ops.check_status(dev)
-        kv_bytes = pages * 2 * hkv * 16 * d * 2
-        if kind == "attn_decode":
+        kv_bytes = kv.numel() * kv.element_size()
+        if append == 1:
             flops = 4.0 * batch * hq * ctx * d
         else:
             flops = 4.0 * batch * hq * d * (ctx * (ctx + 1) / 2)

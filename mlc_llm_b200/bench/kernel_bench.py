@@ -1,6 +1,6 @@
 """Device-timed micro-benchmarks of the hot kernels, reported against measured peaks.
 
-``python -m mlc_llm_b200.bench.kernel_bench [gemm|gemm_q4|gemm_fp8|gemv_q4|lowm_q4|attn_decode|attn_prefill|rope|norm|sampling|moe|all] [--small]``
+``python -m mlc_llm_b200.bench.kernel_bench [gemm|gemm_q4|gemm_fp8|gemv_q4|lowm_q4|attn_decode|attn_prefill|attn_kv4|rope|norm|sampling|moe|all] [--small]``
 
 Timing follows the usual hygiene: warm-up, CUDA events on the launching stream, and a buffer larger
 than L2 written between timed launches so every launch starts cold.  ``--small`` shrinks the
@@ -301,7 +301,7 @@ def main(argv=None):
         bench_lowm_q4(args.small)
     if args.which in ("gemm_q4", "all"):
         res += bench_gemm(args.small, q4=True)
-    if args.which in ("attn_decode", "attn_prefill", "all"):
+    if args.which in ("attn_decode", "attn_prefill", "attn_kv4", "all"):
         try:
             from .attn_bench import bench_attention  # pylint: disable=import-outside-toplevel
 
