@@ -134,4 +134,10 @@ __device__ __forceinline__ void kv4_words(const uint8_t* p, uint32_t (&w)[N]) {
   }
 }
 
+// After a wait ran out: long enough (over 0.1 ms) for copies in flight to land in the shared memory that the CTA is about
+// to give up.
+__device__ __forceinline__ void kv4_linger() {
+  for (int i = 0; i < 64; ++i) __nanosleep(2000);
+}
+
 }  // namespace mlcb

@@ -25,15 +25,15 @@
 // laid end to end, are cut into equal shares, one per persistent CTA, so ragged batches and single long sequences
 // load every SM alike; a unit cut between CTAs leaves fp32 partial results that a second kernel joins. In a CTA
 // a producer warp streams the share's pages (bulk copies into a ring of slots) and, per unit, its query rows and a
-// descriptor, ahead of four consumer warps that take the slots round-robin and merge at the end of each unit.
+// descriptor, ahead of four consumer warps that take the slots round-robin. At the end of a unit one of them, in turn,
+// joins the results of the four while the others go on (all four waiting for each other: 64 heads over 8, D = 128, two
+// tokens each 100 us instead of 89; D = 256 with a window 68 us instead of 57).
 // Every wait is bounded (common.cuh).
 #include "kv4.cuh"
 
 namespace mlcb {
 
 constexpr int KV4_DEC_THREADS = 160;
-
-
 constexpr int KV4_DEC_ITEMS = 1024;   // items per launch: their prefix sums sit in shared memory
 constexpr int KV4_DEC_MIN_SHARE = 4;  // slots per CTA at least: one per consumer warp
 
@@ -205,12 +205,12 @@ struct Kv4DecShape {
   // Query rows of a piece; two pieces are held. The pitch spreads a fragment's eight rows over the banks.
   static constexpr int Q_PITCH = D * 2 + 16;
   static constexpr int Q_BYTES = ROWS * Q_PITCH;
-  // two warps' partial O in fragment order (16 bytes per lane, pair of tiles and column), and their (m, l)
-  static constexpr int MERGE_BYTES = 2 * (ROWS * D * 4 + ROWS * 8);
+  // three warps' partial O in fragment order (16 bytes per lane, pair of tiles and column), and their (m, l), of two pieces
+  static constexpr int MERGE_BYTES = 6 * (ROWS * D * 4 + ROWS * 8);
   static constexpr int OFF_Q = SLOTS * SLOT_BYTES;
   static constexpr int OFF_MERGE = OFF_Q + 2 * Q_BYTES;
   static constexpr int OFF_BAR = OFF_MERGE + MERGE_BYTES;
-  static constexpr int OFF_PIECE = OFF_BAR + 8 * (2 * SLOTS + 4);
+  static constexpr int OFF_PIECE = OFF_BAR + 8 * (2 * SLOTS + 6);
   static constexpr int OFF_SCAN = OFF_PIECE + 2 * 64;          // item prefix sums, sized by the launch
   static_assert(sizeof(Kv4Piece) <= 64, "a piece descriptor has 64 bytes");
 };
@@ -229,9 +229,10 @@ __global__ void __launch_bounds__(KV4_DEC_THREADS, Kv4DecShape<D, NT>::CTAS) kv4
   uint64_t* empty = full + SLOTS;
   uint64_t* piece_full = empty + SLOTS;   // [2]
   uint64_t* piece_empty = piece_full + 2; // [2]
+  uint64_t* merge_full = piece_empty + 2; // [2]
   Kv4Piece* pieces = reinterpret_cast<Kv4Piece*>(smem + Shape::OFF_PIECE);  // [2], 64 bytes apart
   int* scan = reinterpret_cast<int*>(smem + Shape::OFF_SCAN);               // [num_items + 1]
-  __shared__ int abort_word, leave_word;
+  __shared__ int abort_word;
   volatile int* abort_flag = &abort_word;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x < SLOTS) {
@@ -241,6 +242,7 @@ __global__ void __launch_bounds__(KV4_DEC_THREADS, Kv4DecShape<D, NT>::CTAS) kv4
   if (threadIdx.x < 2) {
     mbar_init(&piece_full[threadIdx.x], 1);
     mbar_init(&piece_empty[threadIdx.x], 4);
+    mbar_init(&merge_full[threadIdx.x], 3);
   }
   mbar_fence_init();
   if (threadIdx.x == 0) abort_word = 0;
@@ -370,6 +372,7 @@ __global__ void __launch_bounds__(KV4_DEC_THREADS, Kv4DecShape<D, NT>::CTAS) kv4
       }
       at += take;
     }
+    if (!ok) kv4_linger();
     return;
   }
 
@@ -381,8 +384,8 @@ __global__ void __launch_bounds__(KV4_DEC_THREADS, Kv4DecShape<D, NT>::CTAS) kv4
     bool ok = mbar_wait(&piece_full[e], (k >> 1) & 1, abort_flag, p.status, ERR_WAIT_TMA);
     ok = __all_sync(0xffffffffu, ok);
     const Kv4Piece pc = *reinterpret_cast<const Kv4Piece*>(reinterpret_cast<const uint8_t*>(pieces) + e * 64);
-    // may be <= 0: an empty row block. After a wait that ran out nothing of the piece is touched.
-    const int rows = ok ? min(ROWS, pc.ntok * p.group - pc.row0) : 0;
+    if (!ok) break;  // a wait of some role ran out: the others find out by the abort flag
+    const int rows = min(ROWS, pc.ntok * p.group - pc.row0);  // may be <= 0: an empty row block
     const int npg = pc.npg;
     // Q^T fragments: lane (r, t) has channels 8 t .. 8 t + 7 of every group of row r (+ 8 per n-tile), two k-steps each.
     // They stay in shared memory, one 16-byte load per group and slot. Rows behind the last hold anything: a column of
@@ -657,11 +660,12 @@ __global__ void __launch_bounds__(KV4_DEC_THREADS, Kv4DecShape<D, NT>::CTAS) kv4
       if (lane == 0) mbar_arrive(&empty[s]);
     }
     g0 += static_cast<uint32_t>(max(0, pc.slots));
-    __syncwarp();
-    if (lane == 0) mbar_arrive(&piece_empty[e]);  // descriptor and query rows are in registers
+    if (!ok) break;
     // ---------------------------------------------------------------- merge the four warps of the unit
-    // Two rounds (2 -> 0 and 3 -> 1, then 1 -> 0) through two buffers in fragment order; a lane keeps its place, so the
-    // accesses are whole 512-byte rows and the arithmetic stays in registers.
+    // The warps take turns: three leave their results in shared memory in fragment order and go on to the next piece, the
+    // fourth adds them to its own in a fixed order. A lane keeps its place, so the accesses are whole 512-byte rows and
+    // the arithmetic stays in registers. A piece's buffers and barrier come round with its descriptor's: all four warps
+    // have released piece k - 2, and with it read its buffers, before piece k is handed out.
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -681,7 +685,7 @@ __global__ void __launch_bounds__(KV4_DEC_THREADS, Kv4DecShape<D, NT>::CTAS) kv4
     }
     auto give = [&](int b) {
       float4* dst = reinterpret_cast<float4*>(merge + b * (ROWS * D * 4)) + lane;
-      float* ml = reinterpret_cast<float*>(merge + 2 * ROWS * D * 4 + b * ROWS * 8);
+      float* ml = reinterpret_cast<float*>(merge + 6 * ROWS * D * 4 + b * ROWS * 8);
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -693,7 +697,7 @@ __global__ void __launch_bounds__(KV4_DEC_THREADS, Kv4DecShape<D, NT>::CTAS) kv4
     };
     auto take = [&](int b) {
       const float4* src = reinterpret_cast<const float4*>(merge + b * (ROWS * D * 4)) + lane;
-      const float* ml = reinterpret_cast<const float*>(merge + 2 * ROWS * D * 4 + b * ROWS * 8);
+      const float* ml = reinterpret_cast<const float*>(merge + 6 * ROWS * D * 4 + b * ROWS * 8);
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         const float4 x = reinterpret_cast<const float4*>(ml)[nt * 4 + t];
@@ -714,15 +718,17 @@ __global__ void __launch_bounds__(KV4_DEC_THREADS, Kv4DecShape<D, NT>::CTAS) kv4
         }
       }
     };
-    if (warp >= 2) give(warp - 2);
-    asm volatile("bar.sync 1, 128;" ::: "memory");
-    if (warp < 2) take(warp);
-    __syncwarp();
-    if (warp == 1) give(1);  // its own buffer, which no other warp reads before the barrier
-    if (threadIdx.x == 0) leave_word = *abort_flag;
-    asm volatile("bar.sync 1, 128;" ::: "memory");
-    if (warp == 0) {
-      take(1);
+    const int turn = (warp - static_cast<int>(k & 3u)) & 3;  // 0: this warp joins
+    if (turn) {
+      give(e * 3 + turn - 1);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&merge_full[e]);
+    } else {
+      ok = mbar_wait(&merge_full[e], (k >> 1) & 1, abort_flag, p.status, ERR_WAIT_EPILOGUE);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+#pragma unroll 1
+      for (int b = 0; b < 3; ++b) take(e * 3 + b);
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -747,11 +753,11 @@ __global__ void __launch_bounds__(KV4_DEC_THREADS, Kv4DecShape<D, NT>::CTAS) kv4
           }
         }
     }
-    // Buffer 1 is read by warp 0 until here and written next by warp 3. One thread sampled the abort flag, so that the
-    // warps leave together if a wait of any role ran out.
-    asm volatile("bar.sync 1, 128;" ::: "memory");
-    if (leave_word || pc.last) break;
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&piece_empty[e]);
+    if (pc.last) break;
   }
+  if (*abort_flag) kv4_linger();
 }
 
 // Joins the pieces of the units that were cut: block c has the unit that began in CTA c's share, if any. Its first

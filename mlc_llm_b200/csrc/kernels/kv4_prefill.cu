@@ -724,6 +724,7 @@ __global__ void __launch_bounds__(Kv4PreShape<D>::THREADS, 1) kv4_prefill_kernel
     }
   }
 
+  if (*abort_flag) kv4_linger();
   tc_fence_before();
   __syncthreads();
   if (warp == ISSUER) {
