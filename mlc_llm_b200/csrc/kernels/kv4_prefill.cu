@@ -480,10 +480,11 @@ __global__ void __launch_bounds__(Kv4PreShape<D>::THREADS, 1) kv4_prefill_kernel
       for (int b = 0; b < UNITS; b += BATCH) {
         uint4 v[BATCH];
 #pragma unroll
-        for (int i = 0; i < BATCH; ++i) {  // rows behind the last are copies of it
-          const int at = (b + i) * 32 + lane, r = row0 + max(0, min(sub * 128 + (warp & 3) * 32 + at / UNITS, valid_rows - 1));
+        for (int i = 0; i < BATCH; ++i) {  // rows behind the last are copies of it; a CTA without rows has none to read
+          const int at = (b + i) * 32 + lane, r = row0 + min(sub * 128 + (warp & 3) * 32 + at / UNITS, valid_rows - 1);
           const int ahead = token_of(r);
-          v[i] = reinterpret_cast<const uint4*>(q0 + (ahead * p.q_stride + (r - ahead * G) * D) * 2)[at % UNITS];
+          v[i] = make_uint4(0, 0, 0, 0);
+          if (valid_rows > 0) v[i] = reinterpret_cast<const uint4*>(q0 + (ahead * p.q_stride + (r - ahead * G) * D) * 2)[at % UNITS];
         }
 #pragma unroll
         for (int i = 0; i < BATCH; ++i) {
