@@ -395,6 +395,8 @@ def paged_attention(q: torch.Tensor, kv_pages: torch.Tensor, q_seq: torch.Tensor
     if is_kv4(kv_pages, d):
         return kv4.attend(q, kv_pages, q_seq, q_kvlen, page_indptr, page_indices, hq, hkv, d, page, sm_scale, q_kvstart,
                           sink, tree_mask, softcap, return_lse, plan)
+    if plan is not None and plan.num_tiles and plan.tile_rows > 128:
+        raise ValueError(f"paged_attention: a plan with tiles of {plan.tile_rows} query rows is for a 4-bit cache")
     t = q.shape[0]
     if not q.is_cuda:
         res = ref.paged_attention(q.reshape(t, hq, d), kv_pages, q_seq, q_kvlen, page_indptr,

@@ -62,6 +62,8 @@ class AttentionPlan:
     max_pages: int = 0
     tile_rows: int = 128  # most query rows of any tile
     dec_rows: int = 16  # most query rows (tokens x heads of a group) of any decode item
+    tokens: int = 0  # what the plan was made for, where its maker says so: query tokens
+    group: int = 0  # ... and query heads per KV head
 
 
 def attention_tcgen05(q: torch.Tensor, kv_pages: torch.Tensor, out: torch.Tensor,

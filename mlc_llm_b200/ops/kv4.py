@@ -95,8 +95,8 @@ def append(qkv: torch.Tensor, kv_pages: torch.Tensor, pos: torch.Tensor, slot: t
            inv_freq: Optional[torch.Tensor], hq: int, hkv: int, d: int, rot_dim: int, page: int,
            attn_factor: float = 1.0) -> None:
     """``ops.rope_append`` for a packed cache: rotate the q and k heads of ``qkv [T, (hq + 2 hkv) d]`` in place and
-    write k and v, quantised, to ``slot`` (negative: rotate only). Angles are computed in 64 bits, so that keys at
-    far positions do not change codes."""
+    write k and v, quantised, to ``slot`` (negative: rotate only; the others differ from each other). Angles are computed
+    in 64 bits, so that keys at far positions do not change codes."""
     _check_cache(kv_pages, d, "rope_append")
     t = qkv.shape[0]
     if kv_pages.shape[2] != hkv or kv_pages.shape[3] != page:
@@ -159,7 +159,8 @@ def kv4_plan(q_indptr, q_kvlen: torch.Tensor, page_indptr: torch.Tensor, page_in
     return AttentionPlan(on["tile_seq"], on["tile_qstart"], on["tile_ntok"], q_kvlen, page_indptr, page_indices,
                          len(tiles["tile_seq"]), dec_seq=on["dec_seq"], dec_qstart=on["dec_qstart"], dec_ntok=on["dec_ntok"],
                          num_dec=num_dec, dec_splits=1, max_pages=(int(max_len) + 15) // 16, tile_rows=KV4_TILE_ROWS,
-                         dec_rows=int(tiles["dec_ntok"].max()) * (hq // hkv) if num_dec else 16)
+                         dec_rows=int(tiles["dec_ntok"].max()) * (hq // hkv) if num_dec else 16,
+                         tokens=int(q_indptr[-1]), group=hq // hkv)
 
 
 def _decode_ctas(num_items: int, hkv: int, max_pages: int, device: torch.device) -> int:
@@ -193,6 +194,9 @@ def attend(q: torch.Tensor, kv_pages: torch.Tensor, q_seq: torch.Tensor, q_kvlen
         raise ValueError(f"paged_attention: q is {q.dtype} on {q.device}, the cache {kv_pages.dtype} on {kv_pages.device}")
     if q.dim() != 2 or q.shape[1] != hq * d or (t and (q.stride(1) != 1 or (t > 1 and q.stride(0) < hq * d))):
         raise ValueError(f"paged_attention: q must be [T, {hq * d}] with contiguous rows, got {tuple(q.shape)} {q.stride()}")
+    if plan is not None and plan.group and (plan.tokens != t or plan.group != hq // hkv):
+        raise ValueError(f"paged_attention: the plan is for {plan.tokens} tokens and {plan.group} query heads per KV head, "
+                         f"the call has {t} and {hq // hkv}")
     where = q.get_device()
     _check_index(q_seq, t, where, "paged_attention: q_seq")
     _check_index(q_kvlen, t, where, "paged_attention: q_kvlen")

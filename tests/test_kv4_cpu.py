@@ -178,3 +178,20 @@ def test_refusals():
         ops.kv4_cache(4, 2, 80, 16, torch.float16, "cpu")
     with pytest.raises(ValueError):
         ops.kv4_cache(4, 2, 64, 16, torch.int8, "cpu")
+
+
+def test_a_plan_serves_only_the_step_and_cache_it_was_made_for():
+    d, hq, hkv = 64, 8, 2
+    cache = ops.kv4_cache(40, hkv, d, 16, torch.float16, "cpu")
+    q = torch.zeros(30, hq * d, dtype=torch.float16)
+    seq, kvlen = torch.zeros(30, dtype=torch.int32), torch.arange(1, 31, dtype=torch.int32)
+    indptr, indices = torch.tensor([0, 2], dtype=torch.int32), torch.tensor([0, 1], dtype=torch.int32)
+    plan = ops.kv4_plan([0, 30], kvlen, indptr, indices, hq, hkv, 30)
+    call = lambda x, kv, heads, p: ops.paged_attention(x, kv, seq, kvlen, indptr, indices, heads, hkv, d, 16, 0.125, plan=p)
+    assert call(q, cache, hq, plan).shape == q.shape
+    with pytest.raises(ValueError, match="the plan is for 30 tokens"):
+        call(q[:29], cache, hq, plan)
+    with pytest.raises(ValueError, match="4 query heads per KV head"):
+        call(q[:, : 4 * d].contiguous(), cache, 4, plan)
+    with pytest.raises(ValueError, match="for a 4-bit cache"):  # tiles of 256 rows
+        call(q, torch.zeros(40, 2, hkv, 16, d, dtype=torch.float16), hq, plan)
