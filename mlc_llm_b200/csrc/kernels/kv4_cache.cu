@@ -273,12 +273,13 @@ kv4_append_whole_kernel(T* __restrict__ qkv, uint8_t* __restrict__ pages, const 
 // ------------------------------------------------------------------ read back
 // Values of the rows at slot[t]: k, v [T, hkv, d]. A thread expands one code word (8 channels, 16 bytes out) of
 // N tokens, whose loads it issues together; which word that is costs its divisions once. Bound by the bytes: those
-// written are 3.2 times those read. Negative slots read as zeros. 65536 scattered rows of 8 heads of 128: N = 1 122 us,
-// 2 100 us, 4 88 us (4.0 TB/s), 8 96 us; 77 rows: 1 2.7 us, 4 3.9 us.
+// written are 3.2 times those read. Negative slots read as zeros. 65536 scattered rows of 8 heads of 128 (153 MB read:
+// 80-byte rows touch sectors of their neighbours; 268 MB written): N = 1 122 us, 2 100 us, 4 88 us, 8 96 us; with the page
+// found by multiplication 4 85 us (4.1 TB/s of wanted bytes; divided: 88). 77 rows: 1 2.7 us, 4 3.9 us.
 template <typename T, int N>
 __global__ void __launch_bounds__(256)
 kv4_read_kernel(const uint8_t* __restrict__ pages, const int* __restrict__ slot, T* __restrict__ k, T* __restrict__ v,
-                int tokens, int hkv, int d, int page, long long num_slots, int* status) {
+                int tokens, int hkv, int d, uint32_t page, uint32_t inv_page, long long num_slots, int* status) {
   const int cpr = d / 8;
   const int i = blockIdx.y * 256 + threadIdx.x;
   if (i >= 2 * hkv * cpr) return;
@@ -293,7 +294,12 @@ kv4_read_kernel(const uint8_t* __restrict__ pages, const int* __restrict__ slot,
     if (sl >= num_slots) {
       if (status) atomicCAS(status, 0, ERR_BAD_INDEX);
     } else if (sl >= 0) {
-      const uint8_t* row = pages + ((static_cast<size_t>(sl / page * 2 + kv) * hkv + h) * page + sl % page) * rb;
+      uint32_t pg = __umulhi(static_cast<uint32_t>(sl), inv_page), in = static_cast<uint32_t>(sl) - pg * page;
+      if (in >= page) {
+        ++pg;
+        in -= page;
+      }
+      const uint8_t* row = pages + ((static_cast<size_t>(pg * 2 + kv) * hkv + h) * page + in) * rb;
       w[x] = reinterpret_cast<const uint32_t*>(row)[chunk];
       meta[x] = reinterpret_cast<const uint32_t*>(row + d / 2)[chunk >> 2];
     }
@@ -456,11 +462,13 @@ MLCB_API int mlcb_kv4_read(const void* pages, const int* slot, void* k, void* v,
   // four tokens per thread once that still leaves two blocks per SM
   const int n = static_cast<long long>(tokens) * words >= 8LL * sm_count() ? 4 : 1;
   const dim3 grid((tokens + n - 1) / n, words);
+  // floor(slot / page) by multiplication with floor((2^32 - 1) / page): for slots below 2^31 short by at most one
+  const uint32_t inv_page = 0xffffffffu / static_cast<uint32_t>(page);
   auto run = [&](auto* rows) {
     using T = std::remove_pointer_t<decltype(rows)>;
     auto kern = n == 4 ? kv4_read_kernel<T, 4> : kv4_read_kernel<T, 1>;
-    kern<<<grid, 256, 0, stream>>>(static_cast<const uint8_t*>(pages), slot, rows, static_cast<T*>(v), tokens, hkv, d, page,
-                                   num_slots, status);
+    kern<<<grid, 256, 0, stream>>>(static_cast<const uint8_t*>(pages), slot, rows, static_cast<T*>(v), tokens, hkv, d,
+                                   static_cast<uint32_t>(page), inv_page, num_slots, status);
   };
   if (dtype == 0) run(static_cast<__half*>(k));
   else run(static_cast<__nv_bfloat16*>(k));
