@@ -157,9 +157,10 @@ __global__ void __launch_bounds__(Kv4PreShape<D>::THREADS, 1) kv4_prefill_kernel
   volatile int* abort_flag = &abort_word;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int G = p.group;
-  // long tiles first: the last tiles of a sequence see the most positions
-  const int split = blockIdx.x % p.splits;
-  const int work = p.num_tiles * p.parts - 1 - static_cast<int>(blockIdx.x) / p.splits, hk = blockIdx.y;
+  // long tiles first, of all heads: the last tiles of a sequence see the most positions, and plans put the longest last (all
+  // tiles of one head before those of the next: 4 x 1024 causal tokens 82 us instead of 74)
+  const int hk = blockIdx.x % p.hkv, split = blockIdx.x / p.hkv % p.splits;
+  const int work = p.num_tiles * p.parts - 1 - static_cast<int>(blockIdx.x) / p.hkv / p.splits;
   const int tile = work / p.parts, row0 = work % p.parts * 128;  // first row of the tile that is this CTA's
   const int seq = p.tile_seq[tile], qstart = p.tile_qstart[tile], ntok = p.tile_ntok[tile];
   const int valid_rows = max(0, min(ntok * G - row0, SUB * 128));
@@ -773,7 +774,7 @@ int kv4_prefill_launch(const Kv4PreParams& p, cudaStream_t stream) {
     const cudaError_t err = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::SMEM);
     if (err != cudaSuccess) return static_cast<int>(err);
   }
-  kern<<<dim3(p.num_tiles * p.parts * p.splits, p.hkv), Shape::THREADS, Shape::SMEM, stream>>>(p);
+  kern<<<p.num_tiles * p.parts * p.splits * p.hkv, Shape::THREADS, Shape::SMEM, stream>>>(p);
   count_launch();
   if (p.splits > 1) {
     kv4_prefill_merge_kernel<T, D><<<dim3(p.num_tiles * p.parts, p.hkv, 8), 256, 0, stream>>>(p);
@@ -809,7 +810,7 @@ MLCB_API int mlcb_kv4_prefill(const void* q, const void* pages, void* out, float
   if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(pages)) & 15) return -2;
   if (q_stride % 8) return -2;
   if (dtype != 0 && dtype != 1) return -3;
-  if (splits < 1 || (splits > 1 && (!part_o || !part_ml)) || static_cast<long long>(num_tiles) * splits * 2 > 0x7fffffffLL) return -4;
+  if (splits < 1 || (splits > 1 && (!part_o || !part_ml)) || static_cast<long long>(num_tiles) * splits * 2 * hkv > 0x7fffffffLL) return -4;
   Kv4PreParams p;
   p.q = q;
   p.pages = static_cast<const uint8_t*>(pages);

@@ -12,14 +12,17 @@ import torch
 from ._lib import DTYPE_CODE, check, lib, ptr, status_word, stream_ptr
 
 
-def build_tiles(q_indptr: np.ndarray, group: int, decode_items: bool = True, tile_rows: int = 128) -> Dict[str, np.ndarray]:
+def build_tiles(q_indptr: np.ndarray, group: int, decode_items: bool = True, tile_rows: int = 128,
+                q_kvlen: Optional[np.ndarray] = None) -> Dict[str, np.ndarray]:
     """Split the appended tokens of a batch into work items for the two attention kernels.
 
     Sequences whose chunk fits 16 query rows (``tokens * group <= 16``: decode and short verify
     chunks) become one item each for the decode kernel (``dec_seq``, ``dec_qstart``, ``dec_ntok``).
     The others are cut into tiles of ``tile_rows // group`` tokens for the tcgen05 kernel (``tile_seq``,
-    ``tile_qstart``, ``tile_ntok``; 128 rows over a 16-bit cache, up to 256 over a 4-bit one). All arrays are int32; ``*_qstart`` are global token indices.
-    ``decode_items=False`` sends every sequence to the tcgen05 kernel.
+    ``tile_qstart``, ``tile_ntok``; 128 rows over a 16-bit cache, up to 256 over a 4-bit one). All arrays are int32;
+    ``*_qstart`` are global token indices. ``decode_items=False`` sends every sequence to the tcgen05 kernel.
+    With ``q_kvlen`` (positions every token sees) the tiles come in rising order of the positions they visit: the kernel
+    over a 4-bit cache starts from the end, the longest first.
     """
     tpt = max(1, tile_rows // group)
     q_indptr = np.asarray(q_indptr, dtype=np.int64)
@@ -37,6 +40,9 @@ def build_tiles(q_indptr: np.ndarray, group: int, decode_items: bool = True, til
     local = np.arange(total, dtype=np.int64) - np.repeat(first_tile, ntiles)
     qstart = q_indptr[seq] + local * tpt
     ntok = np.minimum(tpt, q_indptr[seq + 1] - qstart)
+    if q_kvlen is not None and total > 1:
+        order = np.argsort(np.asarray(q_kvlen)[qstart + ntok - 1], kind="stable")
+        seq, qstart, ntok = seq[order], qstart[order], ntok[order]
     out.update({"tile_seq": seq.astype(np.int32), "tile_qstart": qstart.astype(np.int32),
                 "tile_ntok": ntok.astype(np.int32)})
     return out

@@ -155,9 +155,15 @@ def kv4_plan(q_indptr, q_kvlen: torch.Tensor, page_indptr: torch.Tensor, page_in
     tiles = build_tiles(q_indptr, hq // hkv, tile_rows=KV4_TILE_ROWS)
     dev = q_kvlen.device
     on = {k: torch.from_numpy(a).to(dev) for k, a in tiles.items()}
-    num_dec = len(tiles["dec_seq"])
+    num_dec, num_tiles = len(tiles["dec_seq"]), len(tiles["tile_seq"])
+    if dev.type == "cuda" and num_tiles * hkv > sm_count(dev):
+        # more CTAs than SMs: the longest tiles start first, which is from the end (sequences of 512 to 2048 new tokens
+        # behind 0 to 8192 cached ones: 527 us in the order of the batch, 483 us like this)
+        order = torch.argsort(q_kvlen[(on["tile_qstart"] + on["tile_ntok"] - 1).long()], stable=True)
+        for k in ("tile_seq", "tile_qstart", "tile_ntok"):
+            on[k] = on[k][order]
     return AttentionPlan(on["tile_seq"], on["tile_qstart"], on["tile_ntok"], q_kvlen, page_indptr, page_indices,
-                         len(tiles["tile_seq"]), dec_seq=on["dec_seq"], dec_qstart=on["dec_qstart"], dec_ntok=on["dec_ntok"],
+                         num_tiles, dec_seq=on["dec_seq"], dec_qstart=on["dec_qstart"], dec_ntok=on["dec_ntok"],
                          num_dec=num_dec, dec_splits=1, max_pages=(int(max_len) + 15) // 16, tile_rows=KV4_TILE_ROWS,
                          dec_rows=int(tiles["dec_ntok"].max()) * (hq // hkv) if num_dec else 16,
                          tokens=int(q_indptr[-1]), group=hq // hkv)

@@ -409,7 +409,8 @@ class ModelExecutor:
         if self._tc_attention_ok(model):
             from ..ops.attention import build_tiles  # pylint: disable=import-outside-toplevel
 
-            arrays.update(build_tiles(arrays["q_indptr"], model.hq // model.hkv, tile_rows=self._tile_rows(model)))
+            arrays.update(build_tiles(arrays["q_indptr"], model.hq // model.hkv, tile_rows=self._tile_rows(model),
+                                      q_kvlen=arrays["q_kvlen"] if model.kv4 else None))
         if sp is not None:
             for k in _S_INT:
                 arrays["s_" + k] = np.ascontiguousarray(sp[k], dtype=np.int32)

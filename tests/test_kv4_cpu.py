@@ -195,3 +195,17 @@ def test_a_plan_serves_only_the_step_and_cache_it_was_made_for():
         call(q[:, : 4 * d].contiguous(), cache, 4, plan)
     with pytest.raises(ValueError, match="for a 4-bit cache"):  # tiles of 256 rows
         call(q, torch.zeros(40, 2, hkv, 16, d, dtype=torch.float16), hq, plan)
+
+
+def test_tiles_in_rising_order_of_the_positions_they_visit():
+    from mlc_llm_b200.ops.attention import build_tiles
+
+    q_indptr = np.array([0, 300, 301, 420])                       # 4 heads per KV head: tiles of 64 tokens, one decode item
+    kvlen = np.concatenate([np.arange(2001, 2301), [900], np.arange(1, 120)])
+    plain = build_tiles(q_indptr, 4, tile_rows=256)
+    tiles = build_tiles(q_indptr, 4, tile_rows=256, q_kvlen=kvlen)
+    as_set = lambda t: {tuple(map(int, x)) for x in zip(t["tile_seq"], t["tile_qstart"], t["tile_ntok"])}
+    assert as_set(tiles) == as_set(plain) and len(tiles["tile_seq"]) == 7
+    reach = kvlen[tiles["tile_qstart"] + tiles["tile_ntok"] - 1]
+    assert (np.diff(reach) >= 0).all() and reach[-1] == 2300 and reach[0] == 64
+    assert all(np.array_equal(tiles[k], plain[k]) for k in ("dec_seq", "dec_qstart", "dec_ntok"))
