@@ -23,6 +23,15 @@ namespace mlcb {
 // more SMs share the row. Four neighbouring lanes own a group of 32 channels (one 16-byte load each).
 constexpr int KV4_APPEND_THREADS = 256;
 
+// Sine and cosine of x radians. x / pi is taken in two terms, so that the error stays that of one rounding near 1 however
+// far the position is: with one term it is x 2^-53, which at 131071 moved a key of some million across a rounding border.
+__device__ __forceinline__ void kv4_sincos(double x, double& s, double& c) {
+  constexpr double INV_PI = 0.3183098861837907, INV_PI_REST = -1.9678676675182486e-17;
+  const double turns = x * INV_PI;
+  const double rest = fma(x, INV_PI_REST, fma(x, INV_PI, -turns));
+  sincospi(fma(-2.0, rint(0.5 * turns), turns) + rest, &s, &c);
+}
+
 template <typename T>
 __device__ __forceinline__ float kv4_sane(float v) {
   // fmaxf / fminf would turn NaN into a bound
@@ -119,7 +128,7 @@ kv4_append_kernel(T* __restrict__ qkv, uint8_t* __restrict__ pages, const int* _
     const double p = static_cast<double>(pos[t]);
     for (int j = threadIdx.x; j < half; j += blockDim.x) {
       double s, c;
-      sincospi(p * static_cast<double>(inv_freq[j]) * 0.31830988618379067154, &s, &c);
+      kv4_sincos(p * static_cast<double>(inv_freq[j]), s, c);
       sn[j] = s * attn_factor;
       cs[j] = c * attn_factor;
     }
@@ -210,7 +219,7 @@ kv4_append_whole_kernel(T* __restrict__ qkv, uint8_t* __restrict__ pages, const 
   const double p = static_cast<double>(pos[t]);
   for (int j = tid; j < HALF; j += STEP) {
     double s, c;
-    sincospi(p * static_cast<double>(inv_freq[j]) * 0.31830988618379067154, &s, &c);
+    kv4_sincos(p * static_cast<double>(inv_freq[j]), s, c);
     sn[j] = s * attn_factor;
     cs[j] = c * attn_factor;
     const int at = j % 8 * JG + j / 8;  // the JG items of a head read neighbouring words

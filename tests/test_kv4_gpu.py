@@ -69,6 +69,22 @@ def test_append_matches_the_format(dtype, t, hq, hkv, d, rot, page):
     assert full.shape == (t, 2, hkv, d)
 
 
+@pytest.mark.parametrize("rot", [128, 64])
+def test_append_at_positions_far_beyond_a_million(rot):
+    """Angles keep their 64 bits: the rotated keys and codes are those of 64-bit sines of pos * inv_freq."""
+    g = torch.Generator().manual_seed(rot)
+    t, hkv, d = 1024, 8, 128
+    x = _kv(g, t, hkv, d, torch.float16).contiguous()
+    pos = torch.randint(2 ** 29, 2 ** 30, (t,), generator=g).to(torch.int32)
+    slot, inv = torch.arange(t, dtype=torch.int32), ref.rope_inv_freq(rot, 500000.0)
+    cache, want_cache = (ops.kv4_cache(t // 16, hkv, d, 16, torch.float16, dev) for dev in (DEV, "cpu"))
+    mine, want = x.to(DEV), x.clone()
+    ops.rope_append(mine, cache, pos.to(DEV), slot.to(DEV), inv.to(DEV), 0, hkv, d, rot, 16)
+    ops.rope_append(want, want_cache, pos, slot, inv, 0, hkv, d, rot, 16)
+    ops.check_status(cache.device)
+    assert _same_bytes(mine, want) and _same_bytes(cache, want_cache)
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 def test_append_of_values_that_are_not_finite(dtype):
     big = torch.finfo(dtype).max
