@@ -1,8 +1,9 @@
 // The 4-bit KV cache format, shared by its writer, its reader and the attention kernels.
 //
 // A cache row holds the D values of one (token, K or V, kv head). They are cut into groups of 32 channels; a
-// group keeps its minimum lo and a step s = T((max - lo) / 15), both in the type T of the rows (fp16 / bf16), and
-// a 4-bit code c = clamp(rint((x - lo) / s), 0, 15) per value. The group stands for lo + s * c.
+// group keeps its minimum lo and a step s = T((max - lo) * r), both in the type T of the rows (fp16 / bf16), and a 4-bit
+// code c = clamp(rint((x - lo) / s), 0, 15) per value. The group stands for lo + s * c. r is 1 / 15 in fp32: the product is
+// an fp32 rounding away from the quotient, costs one instruction, and is what dividing a CUDA tensor by 15.0 computes.
 //
 //   row bytes:  D / 2 code bytes | D / 32 x (lo, s)          (80 bytes for D = 128, against 256 in 16 bits)
 //   code word:  8 channels in 32 bits; nibble i of the low half is channel 2 i, of the high half channel 2 i + 1

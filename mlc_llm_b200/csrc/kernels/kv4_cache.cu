@@ -83,7 +83,7 @@ __device__ __forceinline__ void kv4_store8(const uint4& val, uint8_t* row, int c
     hi = fmaxf(hi, __shfl_xor_sync(quad, hi, o));
   }
   const float range = __fsub_rn(hi, lo);
-  const T st = Cvt<T>::from_f(__fdiv_rn(range, 15.f));
+  const T st = Cvt<T>::from_f(__fmul_rn(range, 1.f / 15.f));
   const float s = Cvt<T>::to_f(st);
   uint32_t w = 0;
   if (s > 0.f) {

@@ -1,7 +1,7 @@
 """Paged KV cache held in 4 bits: the cache itself, writing it, reading it back, attention over it.
 
 A row is the ``d`` values of one (token, K or V, KV head), cut into groups of 32 channels. A group keeps its minimum
-``lo`` and a step ``s = T((max - lo) / 15)``, both in the cache's type ``T``, and per value the code
+``lo`` and a step ``s = T((max - lo) * r)``, both in the cache's type ``T`` (``r`` is 1 / 15 in fp32), and per value the code
 ``c = clamp(rint((x - lo) / s), 0, 15)``; it stands for ``lo + s * c`` (``s == 0``: for ``lo``). Before that NaN becomes 0
 and values are clamped to a finite bound (``KV4_BOUND``), so a cache never holds anything but finite numbers and a
 token's NaN cannot reach the tokens after it. That is 5 bits per value with 16-bit steps: 80 bytes for ``d = 128``.

@@ -165,7 +165,7 @@ def kv4_pack(x: torch.Tensor) -> torch.Tensor:
     g = torch.nan_to_num(x.float(), nan=0.0, posinf=bound, neginf=-bound).clamp(-bound, bound)
     g = g.reshape(*x.shape[:-1], d // KV4_GROUP, KV4_GROUP)
     lo, hi = g.amin(-1, keepdim=True), g.amax(-1, keepdim=True)
-    s = ((hi - lo) / 15.0).to(x.dtype).float()
+    s = ((hi - lo) * (1.0 / 15.0)).to(x.dtype).float()  # by the fp32 number next to 1 / 15, on every device
     c = torch.where(s > 0, torch.round((g - lo) / torch.where(s > 0, s, torch.ones_like(s))), torch.zeros_like(g))
     c = c.clamp(0, 15).to(torch.uint8).reshape(*x.shape[:-1], d // 8, 8)
     # nibble i of a word's low half is channel 2 i, of its high half channel 2 i + 1

@@ -23,7 +23,7 @@ def _scalar_row(row, dtype):
     for a in range(0, len(row), 32):
         part = [0.0 if math.isnan(x) else min(max(x, -bound), bound) for x in row[a:a + 32]]
         lo, hi = min(part), max(part)
-        s = _round_to(float(np.float32(np.float32(hi) - np.float32(lo)) / np.float32(15.0)), dtype)
+        s = _round_to(float(np.float32(np.float32(hi) - np.float32(lo)) * np.float32(1.0 / 15.0)), dtype)
         for x in part:
             c = 0 if s == 0 else int(np.clip(np.rint(np.float32(np.float32(x) - np.float32(lo)) / np.float32(s)), 0, 15))
             codes.append(c)
