@@ -6,10 +6,10 @@
 //
 //   raw       a warp copies the blocks' packed rows (80 bytes per token at D = 128) into a ring of shared memory
 //   expand    four warps turn them into fp16 K and V tiles in the layout the tensor core reads (128-byte swizzle; V
-//             MN-major), lo + s c rounded once. One expansion feeds both query tiles: at 600 issue slots per
-//             scheduler and block it hides under the 2048 clocks of the block's products. bf16 rows are scaled by a
-//             power of two per 32 positions (and queries per row) into fp16's range, so that K, V and P keep 11 bits:
-//             the scale of K multiplies the scores, that of V the weights.
+//             MN-major), lo + s c rounded once. One expansion feeds both query tiles; it hides under the rest (without
+//             it 2.16 ms for 2.30, measured at a step before). bf16 rows are scaled by a power of two per 32 positions
+//             (and queries per row) into fp16's range, so that K, V and P keep 11 bits: the scale of K multiplies the
+//             scores, that of V the weights.
 //   S = Q K^T    tcgen05.mma, both operands in shared memory, D in TMEM (128 columns per tile)
 //   softmax      one thread per row, 32 columns of TMEM at a time, in two passes: the block's maximum, then its weights
 //                against a running reference that is raised (and O rescaled) only when a score exceeds it by more
@@ -22,8 +22,14 @@
 // the softmax of block j ends.
 //
 // Few long rows (a short chunk behind a long prefix) are split over the cached positions; fp32 partial rows are
-// joined by a second kernel. Bounds: the tensor core (4 D flops per query row and position), then the exponentials
-// (one per row and position; 16 per clock and SM against 8 K flops per clock).
+// joined by a second kernel. Bounds: the tensor core (4 D flops per query row and position) and, as slow, the exponentials
+// (one per row and position: 2048 clocks each per block at 16 per clock and SM and 8 K flops per clock).
+//
+// Measured, 32 / 8 heads of 128: 16384 causal tokens fp16 2.07 ms (1060 TFLOP/s), bf16 2.23 ms; 512 to 2048 new tokens
+// behind 0 to 8192, bf16 484 us (900 TFLOP/s); 4 x 1024 74 us. A block takes 4000 clocks there: a tile's softmax (2100,
+// latency of one warp per scheduler and tile) and then its products and hand-overs (1900), the other tile in between.
+// Tried and slower at 16384 (2.15 ms then): 16 softmax warps 2.23, eight expanding warps 3.26, P handed over in halves 2.21;
+// a quarter of the exponentials as polynomials 2.13 against 2.07.
 //
 // Roles: 4 warps per query tile (softmax, epilogue), 4 expanding warps, 1 copying warp, 1 issuing warp. Every wait is
 // bounded (common.cuh).
@@ -78,6 +84,7 @@ struct Kv4PreShape {
   static constexpr int SMEM = OFF_RAW + RAW_SLOTS * RAW_BYTES + 1024;
   // Two query tiles: four warpgroups that share the launch's 4 x 128 registers per thread as 168 + 168 + 96 + 80 (the
   // last holds the copying and the issuing warp and two idle ones). One tile: 320 threads have registers to spare.
+  // Without the split (448 threads of 128): 548 us where the split takes 484 (bf16), 2.15 ms for 2.07 (16384, fp16).
   static constexpr bool SPLIT = SUB == 2;
   static constexpr int THREADS = SPLIT ? 512 : SUB * 128 + 128 + 64;
   static constexpr int O_COL = SUB == 2 ? 256 : 128;     // TMEM: S tiles first, then O
