@@ -38,6 +38,7 @@ _ARGS = {
     "mlcb_kv4_attn_simt": [_P] * 10 + [_I, _L, _I, _I, _I, _I, _L, _I, _F, _F, _I, _P, _P],
 }
 _FN = {}
+_HERE = contextlib.nullcontext()
 
 
 def _call(name: str, *args) -> None:
@@ -70,7 +71,7 @@ def kv4_cache(num_pages: int, hkv: int, d: int, page: int = 16, dtype: torch.dty
 
 def _guard(device: torch.device):
     """Launches go to the tensors' device, whichever is current."""
-    return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 def _check_cache(kv_pages: torch.Tensor, d: int, what: str) -> None:
@@ -85,7 +86,7 @@ def _check_cache(kv_pages: torch.Tensor, d: int, what: str) -> None:
 
 
 def _check_index(t: Optional[torch.Tensor], n: int, where: int, what: str, dtype: torch.dtype = torch.int32) -> None:
-    if t is not None and (t.dtype != dtype or t.get_device() != where or t.dim() != 1 or t.shape[0] < n
+    if t is not None and (t.dtype != dtype or t.get_device() != where or t.dim() != 1 or t.numel() < n
                           or not t.is_contiguous()):
         raise ValueError(f"{what} must be a contiguous {dtype} vector of at least {n} entries on the cache's device, got "
                          f"{t.dtype} {tuple(t.shape)} on {t.device}")
