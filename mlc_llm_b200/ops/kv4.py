@@ -153,6 +153,12 @@ def kv4_plan(q_indptr, q_kvlen: torch.Tensor, page_indptr: torch.Tensor, page_in
     """The tiling of one step for ``ops.paged_attention`` over a packed cache (shared by all layers). ``q_indptr``:
     host array, first token of every sequence's chunk; ``max_len``: the longest sequence, appended tokens included."""
     q_indptr = np.asarray(q_indptr, dtype=np.int64)
+    if hkv <= 0 or hq <= 0 or hq % hkv:
+        raise ValueError(f"kv4_plan: {hq} query heads do not divide over {hkv} KV heads")
+    if q_indptr.ndim != 1 or len(q_indptr) < 1 or q_indptr[0] != 0 or (np.diff(q_indptr) < 0).any():
+        raise ValueError("kv4_plan: q_indptr must rise from 0")
+    if q_kvlen.dim() != 1 or q_kvlen.shape[0] < q_indptr[-1]:
+        raise ValueError(f"kv4_plan: {int(q_indptr[-1])} tokens, but lengths of {tuple(q_kvlen.shape)}")
     tiles = build_tiles(q_indptr, hq // hkv, tile_rows=KV4_TILE_ROWS)
     dev = q_kvlen.device
     on = {k: torch.from_numpy(a).to(dev) for k, a in tiles.items()}

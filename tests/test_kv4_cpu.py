@@ -209,3 +209,15 @@ def test_tiles_in_rising_order_of_the_positions_they_visit():
     reach = kvlen[tiles["tile_qstart"] + tiles["tile_ntok"] - 1]
     assert (np.diff(reach) >= 0).all() and reach[-1] == 2300 and reach[0] == 64
     assert all(np.array_equal(tiles[k], plain[k]) for k in ("dec_seq", "dec_qstart", "dec_ntok"))
+
+
+def test_plan_refusals():
+    lens, indptr, indices = torch.ones(4, dtype=torch.int32), torch.tensor([0, 1], dtype=torch.int32), torch.zeros(1, dtype=torch.int32)
+    with pytest.raises(ValueError, match="do not divide"):
+        ops.kv4_plan([0, 4], lens, indptr, indices, 6, 4, 4)
+    for bad in ([1, 4], [0, 3, 2], [[0, 4]], []):
+        with pytest.raises(ValueError, match="rise from 0"):
+            ops.kv4_plan(bad, lens, indptr, indices, 8, 4, 4)
+    with pytest.raises(ValueError, match="5 tokens"):
+        ops.kv4_plan([0, 5], lens, indptr, indices, 8, 4, 5)
+    assert ops.kv4_plan([0], lens[:0], indptr, indices, 8, 4, 0).num_tiles == 0
