@@ -36,7 +36,7 @@ def build_tiles(q_indptr: np.ndarray, group: int, decode_items: bool = True, til
     ntiles = (lens + tpt - 1) // tpt
     total = int(ntiles.sum())
     seq = np.repeat(np.arange(len(lens), dtype=np.int64), ntiles)
-    first_tile = np.concatenate(([0], np.cumsum(ntiles)[:-1]))
+    first_tile = np.cumsum(ntiles) - ntiles
     local = np.arange(total, dtype=np.int64) - np.repeat(first_tile, ntiles)
     qstart = q_indptr[seq] + local * tpt
     ntok = np.minimum(tpt, q_indptr[seq + 1] - qstart)
