@@ -331,6 +331,34 @@ def test_generic_shapes(dtype, lens, new, hq, hkv, d, page, extra):
         st.check(out, lse)
 
 
+@pytest.mark.parametrize("dtype,d,q_by", [(torch.float16, 64, 6.0), (torch.float16, 128, 6.0), (torch.float16, 256, 6.0),
+                                          (torch.bfloat16, 64, 3.0), (torch.bfloat16, 128, 3.0), (torch.bfloat16, 256, 2.5)])
+def test_maxima_that_rise_along_the_sequence(dtype, d, q_by):
+    """Scores of a standard deviation of 6 (bf16: what the oracle's bound on their error allows): later blocks exceed the
+    running reference by more than its slack of 2^8, so sums and accumulators are rescaled."""
+    st = Step(dtype, [1700, 400], [300, 150], 8, 2, d, seed=d, q_by=q_by)
+    assert st.plan.num_tiles
+    out, lse = st.run()
+    ops.check_status(out.device)
+    st.check(out, lse)
+    st = Step(dtype, [3000, 400, 90], [1, 2, 1], 8, 2, d, seed=d + 1, q_by=q_by)
+    assert st.plan.num_tiles == 0
+    out, lse = st.run()
+    ops.check_status(out.device)
+    st.check(out, lse)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_more_tiles_than_the_gpu_holds_at_once(dtype):
+    st = Step(dtype, [500, 1100, 900, 3], [500, 650, 130, 1], 32, 8, 64, seed=5)
+    assert st.plan.num_tiles * 8 > torch.cuda.get_device_properties(0).multi_processor_count and st.plan.num_dec == 1
+    ends = st.kvlen[(st.plan.tile_qstart + st.plan.tile_ntok - 1).long().cpu()]
+    assert bool((ends.diff() >= 0).all())  # the longest last, where the kernel begins
+    out, lse = st.run()
+    ops.check_status(out.device)
+    st.check(out, lse)
+
+
 @pytest.mark.parametrize("d", [128, 64])
 def test_rows_that_see_nothing(d):
     # a padded batch entry (length 0), and a row whose window starts behind it
