@@ -7,9 +7,8 @@
 //   raw       a warp copies the blocks' packed rows (80 bytes per token at D = 128) into a ring of shared memory
 //   expand    four warps turn them into fp16 K and V tiles in the layout the tensor core reads (128-byte swizzle; V
 //             MN-major), lo + s c rounded once. One expansion feeds both query tiles; it hides under the rest (without
-//             it 2.16 ms for 2.30, measured at a step before). bf16 rows are scaled by a power of two per 32 positions
-//             (and queries per row) into fp16's range, so that K, V and P keep 11 bits: the scale of K multiplies the
-//             scores, that of V the weights.
+//             it 2.16 ms for 2.30, measured at a step before). bf16 rows are scaled by a power of two per block (V: of
+//             the largest block so far; queries: per row) into fp16's range, so that K, V and P keep 11 bits.
 //   S = Q K^T    tcgen05.mma, both operands in shared memory, D in TMEM (128 columns per tile)
 //   softmax      one thread per row, 32 columns of TMEM at a time, in two passes: the block's maximum, then its weights
 //                against a running reference that is raised (and O rescaled) only when a score exceeds it by more
@@ -25,8 +24,8 @@
 // joined by a second kernel. Bounds: the tensor core (4 D flops per query row and position) and, as slow, the exponentials
 // (one per row and position: 2048 clocks each per block at 16 per clock and SM and 8 K flops per clock).
 //
-// Measured, 32 / 8 heads of 128: 16384 causal tokens fp16 2.07 ms (1060 TFLOP/s), bf16 2.23 ms; 512 to 2048 new tokens
-// behind 0 to 8192, bf16 484 us (900 TFLOP/s); 4 x 1024 74 us. A block takes 4000 clocks there: a tile's softmax (2100,
+// Measured, 32 / 8 heads of 128: 16384 causal tokens fp16 2.07 ms (1060 TFLOP/s), bf16 2.18 ms; 512 to 2048 new tokens
+// behind 0 to 8192, bf16 474 us (920 TFLOP/s); 4 x 1024 74 us. A block takes 4000 clocks there: a tile's softmax (2100,
 // latency of one warp per scheduler and tile) and then its products and hand-overs (1900), the other tile in between.
 // Tried and slower at 16384 (2.15 ms then): 16 softmax warps 2.23, eight expanding warps 3.26, P handed over in halves 2.21;
 // a quarter of the exponentials as polynomials 2.13 against 2.07.
@@ -84,7 +83,7 @@ struct Kv4PreShape {
   static constexpr int SMEM = OFF_RAW + RAW_SLOTS * RAW_BYTES + 1024;
   // Two query tiles: four warpgroups that share the launch's 4 x 128 registers per thread as 168 + 168 + 96 + 80 (the
   // last holds the copying and the issuing warp and two idle ones). One tile: 320 threads have registers to spare.
-  // Without the split (448 threads of 128): 548 us where the split takes 484 (bf16), 2.15 ms for 2.07 (16384, fp16).
+  // Without the split (448 threads of 128) at a step before: 548 us for 484 (bf16), 2.15 ms for 2.07 (16384, fp16).
   static constexpr bool SPLIT = SUB == 2;
   static constexpr int THREADS = SPLIT ? 512 : SUB * 128 + 128 + 64;
   static constexpr int O_COL = SUB == 2 ? 256 : 128;     // TMEM: S tiles first, then O
@@ -150,7 +149,7 @@ __global__ void __launch_bounds__(Kv4PreShape<D>::THREADS, 1) kv4_prefill_kernel
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_word;
   __shared__ Kv4Tile info;
-  __shared__ int exps[4][2][Shape::CHUNKS];  // bf16: exponents of a block's K and V chunks; blocks j - 3 .. j are live
+  __shared__ int exps[4][2];  // bf16: exponents of a block's K and V; blocks j - 3 .. j are live
   uint64_t* raw_full = bars;
   uint64_t* raw_empty = raw_full + Shape::RAW_SLOTS;
   uint64_t* tile_full = raw_empty + Shape::RAW_SLOTS;
@@ -384,6 +383,7 @@ __global__ void __launch_bounds__(Kv4PreShape<D>::THREADS, 1) kv4_prefill_kernel
     const int g0 = w / Shape::CHUNKS * MINE;
     const int reach = max(info.reach[0], SUB == 2 ? info.reach[1] : 0);
     const int first = EXT && p.q_kvstart ? info.first : 0;
+    int v_most = -120;
     bool ok = true;
     for (int n = 0; n < 2 * nmax && ok; ++n) {
       const int j = n >> 1;
@@ -408,17 +408,31 @@ __global__ void __launch_bounds__(Kv4PreShape<D>::THREADS, 1) kv4_prefill_kernel
       for (int i = 0; i < MINE; ++i) meta[i] = live ? pairs[g0 + i] : 0u;
       float shrink = 1.f;
       if constexpr (BF16) {
+        // One exponent per block for K, and for V that of the largest block so far, so that weights need no scale. Every warp
+        // looks at all positions of the block: all come to the same exponent without meeting. (With one per 32 positions and
+        // the weights carrying the difference P lost bits, and a block 50 clocks.) Values below 2^-28 of the largest lose bits.
         // |v| <= |lo| + 15 s: with |lo| < 2^(e + 13) and s < 2^(e + 9) the scaled values stay below 2^14; in steps of 4
         uint32_t top = 0;
 #pragma unroll
-        for (int i = 0; i < MINE; ++i) top = __vmaxu2(top, meta[i] & 0xffff7fffu);
-        if constexpr (Shape::SHARES == 2) {  // the other warp's groups count too: both warps come to the same exponent
+        for (int c = 0; c < Shape::CHUNKS; ++c) {
+          const int t = c * 32 + lane, pos = base_of(j) + t;
+          const uint8_t* pr = smem + Shape::OFF_RAW + s * Shape::RAW_BYTES + t * ROW + D / 2;
+          uint32_t m[GROUPS];
+          if constexpr (ROW % 16 == 0) {
+            kv4_words<GROUPS>(pr, m);
+          } else {
 #pragma unroll
-          for (int i = 0; i < MINE; ++i) top = __vmaxu2(top, live ? pairs[(g0 ^ MINE) + i] & 0xffff7fffu : 0u);
+            for (int g = 0; g < GROUPS; ++g) m[g] = reinterpret_cast<const uint32_t*>(pr)[g];
+          }
+          uint32_t most = 0;
+#pragma unroll
+          for (int g = 0; g < GROUPS; ++g) most = __vmaxu2(most, m[g] & 0xffff7fffu);
+          if (pos < reach && pos < room && (pos >= first || pos < p.sink)) top = __vmaxu2(top, most);
         }
         const int need = max(static_cast<int>(top >> 23) - 9, static_cast<int>((top & 0xffffu) >> 7) - 13) - 126;
-        const int e = max((__reduce_max_sync(0xffffffffu, need) + 1027) / 4 * 4 - 1024, -120);
-        if (lane == 0) exps[j & 3][n & 1][chunk] = e;
+        int e = max((__reduce_max_sync(0xffffffffu, need) + 1027) / 4 * 4 - 1024, -120);
+        if (n & 1) e = v_most = max(v_most, e);
+        if (w == 0 && lane == 0) exps[j & 3][n & 1] = e;
         shrink = exp2f(static_cast<float>(-e));
       }
 #pragma unroll
@@ -542,16 +556,12 @@ __global__ void __launch_bounds__(Kv4PreShape<D>::THREADS, 1) kv4_prefill_kernel
     bool ok = true;
     for (int j = 0; j < mine && ok; ++j) {
       // bf16: the exponents of the block's K and V (the warps that expanded V wrote both before they released it)
-      int k_exp[Shape::CHUNKS], v_log[Shape::CHUNKS], v_top = v_exp;
+      int k_exp = 0, v_top = v_exp;
       if constexpr (BF16) {
         const int n = 2 * j + 1;
         ok = mbar_wait(&tile_full[n % Shape::TILES], (n / Shape::TILES) & 1, abort_flag, p.status, ERR_WAIT_DEQUANT);
-#pragma unroll
-        for (int c = 0; c < Shape::CHUNKS; ++c) {
-          k_exp[c] = exps[j & 3][0][c];
-          v_log[c] = exps[j & 3][1][c];
-          v_top = max(v_top, v_log[c]);
-        }
+        k_exp = exps[j & 3][0];
+        v_top = exps[j & 3][1];  // not below v_exp
       }
       ok = ok && (SUB == 2 ? mbar_wait(&s_full[sub], j & 1, abort_flag, p.status, ERR_WAIT_MMA)
                            : mbar_wait(&s_full[j & 1], (j >> 1) & 1, abort_flag, p.status, ERR_WAIT_MMA));
@@ -564,16 +574,16 @@ __global__ void __launch_bounds__(Kv4PreShape<D>::THREADS, 1) kv4_prefill_kernel
         const bool plain = base + BLK <= all_to && (!EXT || base >= all_from || base + BLK <= p.sink);
         const bool capped = EXT && p.cap_log2 != 0.f;
         // ---- maximum of the block's scores, 32 columns at a time (log2 units). Capped and masked ones are written back.
-        float scale[BLK / 32], mx = -INFINITY;
+        const float undo = BF16 ? row_scale * exp2f(static_cast<float>(k_exp)) : row_scale;
+        // (not 0 where zeros scaled it away: a hidden score is -inf * scale)
+        const float scale = capped ? 1.f : fmaxf(p.scale_log2 * undo, 1e-30f);
+        float mx = -INFINITY;
         uint32_t r[2][32];
         __syncwarp();
         tmem_ld32(t_s, r[0]);
 #pragma unroll
         for (int c = 0; c < BLK / 32; ++c) {
           uint32_t (&x)[32] = r[c & 1];
-          const float undo = BF16 ? row_scale * exp2f(static_cast<float>(k_exp[c])) : row_scale;
-          // (not 0 where zeros scaled it away: a hidden score is -inf * scale)
-          scale[c] = capped ? 1.f : fmaxf(p.scale_log2 * undo, 1e-30f);
           tmem_ld_wait();
           if (c + 1 < BLK / 32) tmem_ld32(t_s + (c + 1) * 32, r[(c + 1) & 1]);
           if (capped) {
@@ -593,8 +603,9 @@ __global__ void __launch_bounds__(Kv4PreShape<D>::THREADS, 1) kv4_prefill_kernel
             top[0] = fmaxf(top[0], fmaxf(__uint_as_float(x[i]), __uint_as_float(x[i + 1])));
             top[1] = fmaxf(top[1], fmaxf(__uint_as_float(x[i + 2]), __uint_as_float(x[i + 3])));
           }
-          mx = fmaxf(mx, fmaxf(top[0], top[1]) * scale[c]);
+          mx = fmaxf(mx, fmaxf(top[0], top[1]));
         }
+        mx *= scale;
         if (capped || !plain) kv4_tmem_st_wait();
         tmem_ld32(t_s, r[0]);
         // ---- raise the reference (and the exponent of V) where the block needs it
@@ -623,14 +634,11 @@ __global__ void __launch_bounds__(Kv4PreShape<D>::THREADS, 1) kv4_prefill_kernel
           l *= m_ref == -INFINITY ? 1.f : alpha;
           m_ref = m_new;
         }
-        // ---- weights against the reference; they overwrite columns that were read before. bf16: they carry the scale
-        // 2^v_log of their V against the one of O, and their sum is relieved of it. (Behind 2^-60 no fp16 weight is left,
-        // while the sum still counts what fp32 has.)
+        // ---- weights against the reference; they overwrite columns that were read before
+        const float shift = m_ref == -INFINITY ? 0.f : -m_ref;
 #pragma unroll
         for (int c = 0; c < BLK / 32; ++c) {
           uint32_t (&x)[32] = r[c & 1];
-          const float lift = BF16 ? static_cast<float>(max(v_log[c] - v_top, -60)) : 0.f;
-          const float shift = m_ref == -INFINITY ? 0.f : lift - m_ref;
           tmem_ld_wait();
           if (c + 1 < BLK / 32) tmem_ld32(t_s + (c + 1) * 32, r[(c + 1) & 1]);
           float2 acc = make_float2(0.f, 0.f);
@@ -638,12 +646,12 @@ __global__ void __launch_bounds__(Kv4PreShape<D>::THREADS, 1) kv4_prefill_kernel
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
             const float2 v = make_float2(__uint_as_float(x[2 * i]), __uint_as_float(x[2 * i + 1]));
-            const float2 y = kv4_fma2(v, make_float2(scale[c], scale[c]), make_float2(shift, shift));
+            const float2 y = kv4_fma2(v, make_float2(scale, scale), make_float2(shift, shift));
             const float2 e = make_float2(exp2f(y.x), exp2f(y.y));
             acc = kv4_add2(acc, e);
             w[i] = Kv4Type<__half>::pack(e.x, e.y);
           }
-          l += BF16 ? (acc.x + acc.y) * exp2f(-lift) : acc.x + acc.y;
+          l += acc.x + acc.y;
           kv4_tmem_st16(t_s + c * 16, w);
         }
         kv4_tmem_st_wait();

@@ -348,6 +348,27 @@ def test_maxima_that_rise_along_the_sequence(dtype, d, q_by):
     st.check(out, lse)
 
 
+@pytest.mark.parametrize("span", [-32, 16, 32])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_values_of_very_different_sizes_along_the_sequence(d, span, monkeypatch):
+    """bf16 values that shrink or grow, by up to 2^10 within a block of 128: a row that sees only the small ones keeps its
+    precision, although it shares a tile, and larger values beside it, with rows that see them."""
+    plain = _kv
+
+    def scaled(g, n, hkv, d, dtype):
+        rows = plain(g, n, hkv, d, dtype)
+        by = torch.exp2(torch.linspace(-span / 2, span / 2, n).round())
+        rows[:, hkv * d:] = (rows[:, hkv * d:].float() * by[:, None]).to(dtype)
+        return rows
+
+    monkeypatch.setitem(globals(), "_kv", scaled)
+    for lens, new in (([400], [400]), ([150], [150]), ([400], [1])):
+        st = Step(torch.bfloat16, lens, new, 8, 2, d, seed=d)
+        out, lse = st.run()
+        ops.check_status(out.device)
+        st.check(out, lse)
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 def test_more_tiles_than_the_gpu_holds_at_once(dtype):
     st = Step(dtype, [500, 1100, 900, 3], [500, 650, 130, 1], 32, 8, 64, seed=5)
