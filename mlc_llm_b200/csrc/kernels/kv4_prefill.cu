@@ -410,7 +410,7 @@ __global__ void __launch_bounds__(Kv4PreShape<D>::THREADS, 1) kv4_prefill_kernel
       if constexpr (BF16) {
         // One exponent per block for K, and for V that of the largest block so far, so that weights need no scale. Every warp
         // looks at all positions of the block: all come to the same exponent without meeting. (With one per 32 positions and
-        // the weights carrying the difference P lost bits, and a block 50 clocks.) Values below 2^-28 of the largest lose bits.
+        // the weights carrying the difference P lost bits, and it took 2 % longer.) Values below 2^-28 of the largest lose bits.
         // |v| <= |lo| + 15 s: with |lo| < 2^(e + 13) and s < 2^(e + 9) the scaled values stay below 2^14; in steps of 4
         uint32_t top = 0;
 #pragma unroll
