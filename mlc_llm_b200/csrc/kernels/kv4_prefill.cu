@@ -204,7 +204,10 @@ __global__ void __launch_bounds__(Kv4PreShape<D>::THREADS, 1) kv4_prefill_kernel
     tmem_relinquish();
   }
   __syncthreads();
-  for (int i = row0 / G + threadIdx.x; i * G < row0 + valid_rows; i += Shape::THREADS) {
+  // (the second CTA of a short tile has no rows: where G does not divide 128, row0 / G * G is below row0, and its token may be
+  // behind the last one of the call)
+  const int past = valid_rows > 0 ? row0 + valid_rows : 0;
+  for (int i = row0 / G + threadIdx.x; i * G < past; i += Shape::THREADS) {
     const int n = p.q_kvlen[qstart + i];
     int end = n, from = 0;
     if (EXT && p.tree_mask) {
