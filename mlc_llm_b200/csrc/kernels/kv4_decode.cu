@@ -249,7 +249,12 @@ __global__ void __launch_bounds__(KV4_DEC_THREADS, Kv4DecShape<D, NT>::CTAS) kv4
     mbar_init(&merge_full[threadIdx.x], 3);
   }
   mbar_fence_init();
-  if (threadIdx.x == 0) abort_word = 0;
+  if (threadIdx.x == 0) {
+    abort_word = 0;
+    // "nothing cut here" until the producer's last piece says otherwise: the second kernel takes counts and addresses from this
+    // word, and runs as well after a wait that ran out has ended the producer early
+    p.part_unit[blockIdx.x * 4] = 0;
+  }
   // slots of every item (an item without a visible position takes one, so that its rows get written)
   for (int i = threadIdx.x; i < p.num_items; i += KV4_DEC_THREADS) scan[i] = max(1, (kv4_item<EXT>(p, i).npg + 1) >> 1);
   __syncthreads();
@@ -273,10 +278,7 @@ __global__ void __launch_bounds__(KV4_DEC_THREADS, Kv4DecShape<D, NT>::CTAS) kv4
   const long long total = static_cast<long long>(scan[p.num_items]) * per_item;
   const long long share = max((total + gridDim.x - 1) / gridDim.x, static_cast<long long>(KV4_DEC_MIN_SHARE));
   const long long begin = blockIdx.x * share, end = min(total, begin + share);
-  if (begin >= end) {
-    if (threadIdx.x == 0) p.part_unit[blockIdx.x * 4] = 0;
-    return;
-  }
+  if (begin >= end) return;
 
   if (warp == 4) {
     // ---------------------------------------------------------------- producer
@@ -839,6 +841,8 @@ int kv4_decode_launch(Kv4DecParams p, int num_items, int max_ctas, cudaStream_t 
     part.item_ntok += first;
     part.num_items = num_items - first < batch ? num_items - first : batch;
     kern<<<ctas, KV4_DEC_THREADS, Shape::OFF_SCAN + (part.num_items + 1) * 4, stream>>>(part);
+    err = cudaGetLastError();  // the second kernel reads what this one wrote
+    if (err != cudaSuccess) return static_cast<int>(err);
     count_launch();
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(ctas);
