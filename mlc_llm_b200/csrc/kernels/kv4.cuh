@@ -135,10 +135,12 @@ __device__ __forceinline__ void kv4_words(const uint8_t* p, uint32_t (&w)[N]) {
   }
 }
 
-// After a wait ran out: long enough (over 0.1 ms) for copies in flight to land in the shared memory that the CTA is about
-// to give up.
-__device__ __forceinline__ void kv4_linger() {
-  for (int i = 0; i < 64; ++i) __nanosleep(2000);
+// Waits until phase `parity` of a barrier is over, no matter whether a wait of some role ran out: before a CTA gives up its
+// shared memory and TMEM, the copies and products in flight have to land. They do so by themselves; the limit (about 50 ms)
+// is for a phase that the hardware never ends.
+__device__ __forceinline__ void kv4_drain(uint64_t* bar, uint32_t parity) {
+  for (int i = 0; i < 256 && !mbar_try_wait_parked(bar, parity); ++i) {
+  }
 }
 
 }  // namespace mlcb

@@ -378,7 +378,9 @@ __global__ void __launch_bounds__(KV4_DEC_THREADS, Kv4DecShape<D, NT>::CTAS) kv4
       }
       at += take;
     }
-    if (!ok) kv4_linger();
+    // all copies have landed before this warp leaves, also those that the consumers gave up waiting for
+    for (uint32_t n = g < SLOTS ? 0 : g - SLOTS; n < g; ++n) kv4_drain(&full[n % SLOTS], (n / SLOTS) & 1);
+    for (uint32_t n = k < 2 ? 0 : k - 2; n < k; ++n) kv4_drain(&piece_full[n & 1], (n >> 1) & 1);
     return;
   }
 
@@ -763,7 +765,6 @@ __global__ void __launch_bounds__(KV4_DEC_THREADS, Kv4DecShape<D, NT>::CTAS) kv4
     if (lane == 0) mbar_arrive(&piece_empty[e]);
     if (pc.last) break;
   }
-  if (*abort_flag) kv4_linger();
 }
 
 // Joins the pieces of the units that were cut: block c has the unit that began in CTA c's share, if any. Its first

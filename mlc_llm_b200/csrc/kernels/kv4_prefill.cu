@@ -145,7 +145,7 @@ __global__ void __launch_bounds__(Kv4PreShape<D>::THREADS, 1) kv4_prefill_kernel
   pdl_launch_dependents();
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  __shared__ uint64_t bars[2 * Shape::RAW_SLOTS + 2 * Shape::TILES + 8];
+  __shared__ uint64_t bars[2 * Shape::RAW_SLOTS + 2 * Shape::TILES + 9];
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_word;
   __shared__ Kv4Tile info;
@@ -160,6 +160,7 @@ __global__ void __launch_bounds__(Kv4PreShape<D>::THREADS, 1) kv4_prefill_kernel
   uint64_t* o_done = p_full + 2;                 // [SUB]
   uint64_t* pv_done = o_done + 2;                // D = 256 only
   uint64_t* q_ready = pv_done + 1;
+  uint64_t* mma_idle = q_ready + 1;              // every product of this CTA is over
   volatile int* abort_flag = &abort_word;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int G = p.group;
@@ -189,6 +190,7 @@ __global__ void __launch_bounds__(Kv4PreShape<D>::THREADS, 1) kv4_prefill_kernel
     }
     mbar_init(pv_done, 1);
     mbar_init(q_ready, 4 * SUB);
+    mbar_init(mma_idle, 1);
     abort_word = 0;
     mbar_fence_init();
     for (int i = 0; i < 2; ++i) {
@@ -291,6 +293,7 @@ __global__ void __launch_bounds__(Kv4PreShape<D>::THREADS, 1) kv4_prefill_kernel
         }
       }
     }
+    for (int n = max(0, m - Shape::RAW_SLOTS); n < m; ++n) kv4_drain(&raw_full[n % Shape::RAW_SLOTS], (n / Shape::RAW_SLOTS) & 1);
    } else if (warp == ISSUER) {
     // ---------------------------------------------------------------- tensor core
     if (nmax > 0) {
@@ -373,6 +376,8 @@ __global__ void __launch_bounds__(Kv4PreShape<D>::THREADS, 1) kv4_prefill_kernel
           if (SUB == 2 && j + 1 < nmax) umma_commit(&tile_empty[(2 * j + 2) % Shape::TILES]);
         });
       }
+      one([&] { umma_commit(mma_idle); });
+      kv4_drain(mma_idle, 0);
     }
    }
   } else if (warp >= SUB * 4) {
@@ -744,7 +749,6 @@ __global__ void __launch_bounds__(Kv4PreShape<D>::THREADS, 1) kv4_prefill_kernel
     }
   }
 
-  if (*abort_flag) kv4_linger();
   tc_fence_before();
   __syncthreads();
   if (warp == ISSUER) {

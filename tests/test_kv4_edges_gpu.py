@@ -36,6 +36,26 @@ def _check_rows(st, out, lse, rows):
     part.check(out[rows], lse[rows])
 
 
+# ------------------------------------------------------------------------------------------------- attention
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("lens,new", [([0], [1]), ([1], [1]), ([33], [1]), ([100], [3]), ([3000, 40, 5000] * 30, [1] * 90),
+                                      ([1, 2, 500], [1, 2, 4]), ([40], [40]), ([129], [129]), ([3000], [40]), ([900, 260], [300, 129])])
+def test_waiting_for_copies_in_flight_takes_no_time(lens, new, d):
+    """Before a CTA ends it waits for its last copies and products. They are over then: a wait on a wrong phase would
+    take its limit, some 50 ms each."""
+    st = Step(torch.float16, [max(n, 1) for n in lens], new, 8, 2, d, kvlen=[0] if lens == [0] else None)
+    st.run()
+    torch.cuda.synchronize()
+    a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    a.record()
+    out, lse = st.run()
+    b.record()
+    torch.cuda.synchronize()
+    assert a.elapsed_time(b) < 20.0
+    ops.check_status(out.device)
+    st.check(out, lse)
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("lens,new,hq,hkv,d", [([100, 40], [1, 1], 32, 1, 128), ([300, 40], [5, 1], 71, 1, 64),
                                                ([90, 900], [1, 1], 20, 1, 256), ([60, 30], [2, 1], 300, 1, 64),
