@@ -69,7 +69,8 @@ class AttentionPlan:
     tile_rows: int = 128  # most query rows of any tile
     dec_rows: int = 16  # most query rows (tokens x heads of a group) of any decode item
     tokens: int = 0  # what the plan was made for, where its maker says so: query tokens
-    group: int = 0  # ... and query heads per KV head
+    group: int = 0  # ... query heads per KV head
+    seqs: int = 0  # ... and sequences
 
 
 def attention_tcgen05(q: torch.Tensor, kv_pages: torch.Tensor, out: torch.Tensor,

@@ -173,7 +173,7 @@ def kv4_plan(q_indptr, q_kvlen: torch.Tensor, page_indptr: torch.Tensor, page_in
                          num_tiles, dec_seq=on["dec_seq"], dec_qstart=on["dec_qstart"], dec_ntok=on["dec_ntok"],
                          num_dec=num_dec, dec_splits=1, max_pages=(int(max_len) + 15) // 16, tile_rows=KV4_TILE_ROWS,
                          dec_rows=int(tiles["dec_ntok"].max()) * (hq // hkv) if num_dec else 16,
-                         tokens=int(q_indptr[-1]), group=hq // hkv)
+                         tokens=int(q_indptr[-1]), group=hq // hkv, seqs=len(q_indptr) - 1)
 
 
 def _decode_ctas(num_items: int, hkv: int, max_pages: int, device: torch.device) -> int:
@@ -211,10 +211,14 @@ def attend(q: torch.Tensor, kv_pages: torch.Tensor, q_seq: torch.Tensor, q_kvlen
         raise ValueError(f"paged_attention: the plan is for {plan.tokens} tokens and {plan.group} query heads per KV head, "
                          f"the call has {t} and {hq // hkv}")
     where = q.get_device()
+    if plan is not None and ((plan.num_dec and plan.dec_seq.device != q.device)
+                             or (plan.num_tiles and plan.tile_seq.device != q.device)):
+        raise ValueError(f"paged_attention: q is on {q.device}, the plan's items are not")
     _check_index(q_seq, t, where, "paged_attention: q_seq")
     _check_index(q_kvlen, t, where, "paged_attention: q_kvlen")
     _check_index(q_kvstart, t, where, "paged_attention: q_kvstart")
-    _check_index(page_indptr, 2 if t else 0, where, "paged_attention: page_indptr")
+    seqs = plan.seqs if plan is not None else 0
+    _check_index(page_indptr, max(seqs, 1) + 1 if t else 0, where, "paged_attention: page_indptr")
     _check_index(page_indices, 0, where, "paged_attention: page_indices")
     _check_index(tree_mask, t, where, "paged_attention: tree_mask", torch.int64)
     if not q.is_cuda:

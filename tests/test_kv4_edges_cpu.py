@@ -1,8 +1,14 @@
 """The 4-bit KV cache: what can be seen of its kernels, plans and engine wiring without a GPU."""
+import dataclasses
 import re
 from pathlib import Path
 
+import numpy as np
+import pytest
+import torch
+
 import mlc_llm_b200
+from mlc_llm_b200 import ops
 
 KERNELS = Path(mlc_llm_b200.__file__).parent / "csrc" / "kernels"
 
@@ -27,3 +33,24 @@ def test_the_join_of_cut_units_never_reads_a_count_that_was_not_written():
     assert "return" not in head[:at]
     launch = code[code.index("kern<<<"): code.index("kv4_decode_merge_kernel<T, D>, part")]
     assert re.search(r"err = cudaGetLastError\(\);\s*if \(err != cudaSuccess\) return", launch)
+
+
+def test_a_plan_of_other_sequences_or_another_device_is_refused():
+    """The kernels read the plan's items from its arrays and two entries of ``page_indptr`` per item."""
+    hq, hkv, d = 8, 2, 64
+    cache = ops.kv4_cache(8, hkv, d, 16, torch.float16, "cpu")
+    lens, new = [20, 30, 5], [1, 12, 1]                # 12 tokens of 4 heads: a prefill tile; the others: decode items
+    q = torch.zeros(14, hq * d, dtype=torch.float16)
+    seq = torch.tensor(np.repeat([0, 1, 2], new), dtype=torch.int32)
+    kvlen = torch.cat([torch.arange(n - m + 1, n + 1) for n, m in zip(lens, new)]).to(torch.int32)
+    indptr, indices = torch.tensor([0, 2, 4, 5], dtype=torch.int32), torch.arange(5, dtype=torch.int32)
+    plan = ops.kv4_plan([0, 1, 13, 14], kvlen, indptr, indices, hq, hkv, 30)
+    assert plan.num_dec == 2 and plan.num_tiles == 1
+    call = lambda p, ip: ops.paged_attention(q, cache, seq, kvlen, ip, indices, hq, hkv, d, 16, 0.125, plan=p)
+    assert call(plan, indptr).shape == q.shape
+    with pytest.raises(ValueError, match="page_indptr"):
+        call(plan, indptr[:3])
+    for name in ("dec_seq", "tile_seq"):
+        other = dataclasses.replace(plan, **{name: getattr(plan, name).to("meta")})
+        with pytest.raises(ValueError, match="plan's items"):
+            call(other, indptr)
