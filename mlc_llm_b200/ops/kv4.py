@@ -233,7 +233,7 @@ def attend(q: torch.Tensor, kv_pages: torch.Tensor, q_seq: torch.Tensor, q_kvlen
     return (out, lse) if return_lse else out
 
 
-def _decode(q, kv_pages, out, lse, q_kvlen, page_indptr, page_indices, hq, hkv, d, sm_scale, q_kvstart, sink, tree_mask,
+def _decode(q, q_stride, kv_pages, out, lse, q_kvlen, page_indptr, page_indices, hq, hkv, d, sm_scale, q_kvstart, sink, tree_mask,
             softcap, plan) -> None:
     # with one token per item the rows are the group's heads, whatever the plan was made for
     rows = hq // hkv if q.shape[0] == plan.num_dec else min(16, plan.dec_rows)
@@ -243,7 +243,7 @@ def _decode(q, kv_pages, out, lse, q_kvlen, page_indptr, page_indices, hq, hkv, 
     part = scratch.data_ptr()
     _call("mlcb_kv4_decode", q.data_ptr(), kv_pages.data_ptr(), out.data_ptr(), _at(lse), plan.dec_seq.data_ptr(),
           plan.dec_qstart.data_ptr(), plan.dec_ntok.data_ptr(), q_kvlen.data_ptr(), page_indptr.data_ptr(),
-          page_indices.data_ptr(), plan.num_dec, rows, q.stride(0), hq, hkv, d, kv_pages.shape[0], sm_scale,
+          page_indices.data_ptr(), plan.num_dec, rows, q_stride, hq, hkv, d, kv_pages.shape[0], sm_scale,
           DTYPE_CODE[q.dtype], ctas, part + ctas * 272, part + ctas * 16, part, *_env(q.device), _at(q_kvstart),
           _at(tree_mask), sink, softcap)
 
@@ -255,7 +255,7 @@ def _prefill_splits(ctas: int, blocks: int, device: torch.device) -> int:
     return 1 << (most.bit_length() - 1)
 
 
-def _prefill(q, kv_pages, out, lse, q_kvlen, page_indptr, page_indices, hq, hkv, d, sm_scale, q_kvstart, sink, tree_mask,
+def _prefill(q, q_stride, kv_pages, out, lse, q_kvlen, page_indptr, page_indices, hq, hkv, d, sm_scale, q_kvstart, sink, tree_mask,
              softcap, plan, decode_items: bool) -> None:
     if decode_items:
         seq, qstart, ntok, num, rows = plan.dec_seq, plan.dec_qstart, plan.dec_ntok, plan.num_dec, min(16, plan.dec_rows)
@@ -270,7 +270,7 @@ def _prefill(q, kv_pages, out, lse, q_kvlen, page_indptr, page_indices, hq, hkv,
         part_ml = scratch.data_ptr()
         part_o = part_ml + blocks * 2048
     _call("mlcb_kv4_prefill", q.data_ptr(), kv_pages.data_ptr(), out.data_ptr(), _at(lse), seq.data_ptr(), qstart.data_ptr(),
-          ntok.data_ptr(), q_kvlen.data_ptr(), page_indptr.data_ptr(), page_indices.data_ptr(), num, rows, q.stride(0), hq,
+          ntok.data_ptr(), q_kvlen.data_ptr(), page_indptr.data_ptr(), page_indices.data_ptr(), num, rows, q_stride, hq,
           hkv, d, kv_pages.shape[0], sm_scale, DTYPE_CODE[q.dtype], splits, part_o, part_ml, *_env(q.device),
           _at(q_kvstart), _at(tree_mask), sink, softcap)
 
@@ -278,11 +278,12 @@ def _prefill(q, kv_pages, out, lse, q_kvlen, page_indptr, page_indices, hq, hkv,
 def _launch(q, kv_pages, out, lse, q_seq, q_kvlen, page_indptr, page_indices, hq, hkv, d, page, sm_scale, q_kvstart, sink,
             tree_mask, softcap, plan) -> None:
     t = q.shape[0]
-    aligned = q.data_ptr() % 16 == 0 and (q.stride(0) % 8 == 0 or t == 1)
+    q_stride = q.stride(0) if t > 1 else hq * d  # of a single row nothing is read behind it, however wide its buffer
+    aligned = q.data_ptr() % 16 == 0 and q_stride % 8 == 0
     if plan is not None and plan.use_tensor_core and page == 16 and d in KV4_HEAD_DIMS and aligned \
             and hq // hkv <= plan.tile_rows:
-        args = (q, kv_pages, out, lse, q_kvlen, page_indptr, page_indices, hq, hkv, d, sm_scale, q_kvstart, sink, tree_mask,
-                softcap, plan)
+        args = (q, q_stride, kv_pages, out, lse, q_kvlen, page_indptr, page_indices, hq, hkv, d, sm_scale, q_kvstart, sink,
+                tree_mask, softcap, plan)
         if plan.num_dec:
             if d == 96:  # no decode kernel: its lanes own powers of two of channels
                 _prefill(*args, decode_items=True)
@@ -292,7 +293,7 @@ def _launch(q, kv_pages, out, lse, q_seq, q_kvlen, page_indptr, page_indices, hq
             _prefill(*args, decode_items=False)
         return
     _call("mlcb_kv4_attn_simt", q.data_ptr(), kv_pages.data_ptr(), out.data_ptr(), _at(lse), q_seq.data_ptr(),
-          q_kvlen.data_ptr(), _at(q_kvstart), _at(tree_mask), page_indptr.data_ptr(), page_indices.data_ptr(), t, q.stride(0),
+          q_kvlen.data_ptr(), _at(q_kvstart), _at(tree_mask), page_indptr.data_ptr(), page_indices.data_ptr(), t, q_stride,
           hq, hkv, d, page, kv_pages.shape[0], sink, sm_scale, softcap, DTYPE_CODE[q.dtype], *_env(q.device))
 
 

@@ -36,6 +36,21 @@ def _check_rows(st, out, lse, rows):
     part.check(out[rows], lse[rows])
 
 
+@pytest.mark.parametrize("hq,hkv,d", [(32, 8, 128), (8, 2, 64), (4, 2, 96), (8, 4, 256), (32, 1, 128), (4, 2, 32)])
+def test_one_token_of_a_row_of_any_width(hq, hkv, d):
+    """A single token's row has no next row: the width of the buffer it lies in does not matter."""
+    st = Step(torch.float16, [77], [1], hq, hkv, d)
+    for extra in (1, 4, 8):
+        wide = torch.zeros(1, hq * d + extra, dtype=torch.float16, device=DEV)
+        q = wide[:, : hq * d]
+        q.copy_(st.q)
+        assert q.stride(0) == hq * d + extra
+        for plan in (True, False):
+            out, lse = _attend(st, plan, q)
+            ops.check_status(out.device)
+            st.check(out, lse)
+
+
 # ------------------------------------------------------------------------------------------------- attention
 @pytest.mark.parametrize("d", [64, 128, 256])
 @pytest.mark.parametrize("lens,new", [([0], [1]), ([1], [1]), ([33], [1]), ([100], [3]), ([3000, 40, 5000] * 30, [1] * 90),
