@@ -439,14 +439,18 @@ MLCB_API int mlcb_kv4_append(void* qkv, void* pages, const int* pos, const int* 
   int parts = 1;
   while (parts < hkv && static_cast<long long>(tokens) * parts < 2LL * sm_count()) parts *= 2;
   if (parts > hkv) parts = hkv;
-  auto bytes = [&] { return static_cast<size_t>(rot_dim) * 8 + static_cast<size_t>((hkv + parts - 1) / parts) * d * 2; };
-  while (bytes() > 48 * 1024) parts *= 2;  // more kv heads than fit: ends at one head, under 3 KB
+  // Shared memory of a block: the keys of its heads, and 64-bit sines, which the kernel for whole heads holds in static arrays
+  // (with a 32-bit copy). Both count against the 48 KB that a launch gets without asking for more.
+  const bool whole = rot_dim == d && (d == 64 || d == 128 || d == 256);
+  const size_t fixed = static_cast<size_t>(whole ? 12 * d : 0), sines = whole ? 0 : static_cast<size_t>(rot_dim) * 8;
+  auto bytes = [&] { return sines + static_cast<size_t>((hkv + parts - 1) / parts) * d * 2; };
+  while (fixed + bytes() > 48 * 1024) parts *= 2;  // more kv heads than fit: ends at one head, under 4 KB
   const size_t smem = bytes();
   const dim3 grid(tokens, parts);
   auto run = [&](auto* rows) {
     using T = std::remove_pointer_t<decltype(rows)>;
     uint8_t* dst = static_cast<uint8_t*>(pages);
-    if (rot_dim == d && (d == 64 || d == 128 || d == 256)) {
+    if (whole) {
       auto kern = d == 64 ? kv4_append_whole_kernel<T, 64> : d == 128 ? kv4_append_whole_kernel<T, 128> : kv4_append_whole_kernel<T, 256>;
       kern<<<grid, KV4_APPEND_THREADS, smem, stream>>>(rows, dst, pos, slot, inv_freq, hq, hkv, page, attn_factor, num_slots, status);
     } else {

@@ -51,6 +51,24 @@ def test_one_token_of_a_row_of_any_width(hq, hkv, d):
             st.check(out, lse)
 
 
+# ------------------------------------------------------------------------------------------------- append
+@pytest.mark.parametrize("t,hkv,d,rot", [(300, 90, 256, 256), (300, 185, 128, 128), (300, 92, 256, 64), (4, 190, 256, 256),
+                                         (300, 94, 256, 256), (300, 500, 64, 64)])
+def test_append_of_many_heads(t, hkv, d, rot):
+    """Heads beyond what the shared memory of a block holds, at enough tokens that a block takes all heads of its token."""
+    g = torch.Generator().manual_seed(hkv)
+    x = _kv(g, t, hkv, d, torch.float16).contiguous()
+    pos = torch.randint(0, 4096, (t,), generator=g).to(torch.int32)
+    slot, inv = torch.arange(t, dtype=torch.int32), base.ref.rope_inv_freq(rot, 10000.0)
+    pages = (t + 15) // 16
+    cache, want_cache = (ops.kv4_cache(pages, hkv, d, 16, torch.float16, dev) for dev in (DEV, "cpu"))
+    mine, want = x.to(DEV), x.clone()
+    ops.rope_append(mine, cache, pos.to(DEV), slot.to(DEV), inv.to(DEV), 0, hkv, d, rot, 16)
+    ops.rope_append(want, want_cache, pos, slot, inv, 0, hkv, d, rot, 16)
+    ops.check_status(cache.device)
+    assert _same_bytes(mine, want) and _same_bytes(cache, want_cache)
+
+
 # ------------------------------------------------------------------------------------------------- attention
 @pytest.mark.parametrize("d", [64, 128, 256])
 @pytest.mark.parametrize("lens,new", [([0], [1]), ([1], [1]), ([33], [1]), ([100], [3]), ([3000, 40, 5000] * 30, [1] * 90),
