@@ -433,7 +433,7 @@ MLCB_API int mlcb_kv4_append(void* qkv, void* pages, const int* pos, const int* 
                              int dtype, int* status, cudaStream_t stream) {
   if (tokens <= 0) return 0;
   if (hq < 0 || hkv <= 0 || d <= 0 || d % 32 || d > 256 || rot_dim < 0 || rot_dim % 2 || rot_dim > d || page <= 0) return -1;
-  if ((reinterpret_cast<uintptr_t>(qkv) & 15) || (reinterpret_cast<uintptr_t>(pages) & 15)) return -2;
+  if ((reinterpret_cast<uintptr_t>(qkv) & 15) || (reinterpret_cast<uintptr_t>(pages) & 3)) return -2;
   if (dtype != 0 && dtype != 1) return -3;
   // fewer tokens than two blocks per SM: cut the heads so that the blocks still cover the GPU
   int parts = 1;
@@ -468,7 +468,7 @@ MLCB_API int mlcb_kv4_read(const void* pages, const int* slot, void* k, void* v,
                            long long num_slots, int dtype, int* status, cudaStream_t stream) {
   if (tokens <= 0) return 0;
   if (hkv <= 0 || d <= 0 || d % 32 || d > 256 || page <= 0) return -1;
-  if ((reinterpret_cast<uintptr_t>(pages) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15) return -2;
+  if (((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15) || (reinterpret_cast<uintptr_t>(pages) & 3)) return -2;
   if (dtype != 0 && dtype != 1) return -3;
   const int words = (2 * hkv * (d / 8) + 255) / 256;
   if (words > 65535) return -4;

@@ -279,7 +279,7 @@ def _launch(q, kv_pages, out, lse, q_seq, q_kvlen, page_indptr, page_indices, hq
             tree_mask, softcap, plan) -> None:
     t = q.shape[0]
     q_stride = q.stride(0) if t > 1 else hq * d  # of a single row nothing is read behind it, however wide its buffer
-    aligned = q.data_ptr() % 16 == 0 and q_stride % 8 == 0
+    aligned = (q.data_ptr() | kv_pages.data_ptr()) % 16 == 0 and q_stride % 8 == 0
     if plan is not None and plan.use_tensor_core and page == 16 and d in KV4_HEAD_DIMS and aligned \
             and hq // hkv <= plan.tile_rows:
         args = (q, q_stride, kv_pages, out, lse, q_kvlen, page_indptr, page_indices, hq, hkv, d, sm_scale, q_kvstart, sink,

@@ -69,6 +69,50 @@ def test_append_of_many_heads(t, hkv, d, rot):
     assert _same_bytes(mine, want) and _same_bytes(cache, want_cache)
 
 
+@pytest.mark.parametrize("d,page,pages", [(32, 1, 3), (32, 3, 1), (96, 1, 1), (160, 1, 3)])
+def test_layers_of_small_pages(d, page, pages):
+    """Layers that do not begin on 16 bytes: rows are whole 32-bit words, which is all that the kernels ask of them."""
+    dtype, hq, hkv, n = torch.float16, 2, 1, pages * page
+    cache = ops.kv4_cache(pages, hkv, d, page, dtype, DEV, layers=3)
+    want = ops.kv4_cache(pages, hkv, d, page, dtype, "cpu", layers=3)
+    assert any(c.data_ptr() % 16 for c in cache)
+    g = torch.Generator().manual_seed(d)
+    at = torch.arange(n, dtype=torch.int32)
+    indptr, indices = torch.tensor([0, pages], dtype=torch.int32), torch.arange(pages, dtype=torch.int32)
+    one, length = torch.zeros(1, dtype=torch.int32), torch.tensor([n], dtype=torch.int32)
+    for li in range(3):
+        x = _kv(g, n, hkv, d, dtype)
+        q = torch.randn(1, hq * d, generator=g).to(dtype)
+        res = []
+        for c, dev in ((cache[li], DEV), (want[li], "cpu")):
+            ops.rope_append(x.to(dev), c, at.to(dev), at.to(dev), None, 0, hkv, d, 0, page)
+            k, _ = ops.kv4_read(c, at.to(dev), d)
+            res.append((k.cpu(), ops.paged_attention(q.to(dev), c, one.to(dev), length.to(dev), indptr.to(dev),
+                                                     indices.to(dev), hq, hkv, d, page, d ** -0.5).cpu()))
+        # lo + s c rounded once against twice, in fp16; the weighted mean of at most three values rounded once more
+        assert bool(((res[0][0].double() - res[1][0].double()).abs() <= 2.0 ** -10 * res[1][0].double().abs() + 1e-6).all())
+        assert bool(((res[0][1].double() - res[1][1].double()).abs() <= 2.0 ** -8 * res[1][1].double().abs().max()).all())
+    ops.check_status(cache.device)
+    assert _same_bytes(cache, want)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_a_cache_that_begins_on_any_word(d):
+    """A cache that is a part of a larger buffer, 4 bytes behind a 16-byte boundary."""
+    st = Step(torch.float16, [300, 40, 33], [1, 30, 33], 8, 2, d, seed=2)
+    flat = torch.zeros(st.cache.numel() + 8, dtype=torch.float16, device=DEV)
+    moved = flat[2: 2 + st.cache.numel()].view(st.cache.shape)
+    moved.copy_(st.cache)
+    assert moved.is_contiguous() and moved.data_ptr() % 16 == 4
+    k, v = ops.kv4_read(st.cache, (st.indices[:3] * 16).contiguous(), d)
+    mk, mv = ops.kv4_read(moved, (st.indices[:3] * 16).contiguous(), d)
+    assert torch.equal(k, mk) and torch.equal(v, mv)
+    st.cache = moved
+    out, lse = st.run()
+    ops.check_status(out.device)
+    st.check(out, lse)
+
+
 # ------------------------------------------------------------------------------------------------- attention
 @pytest.mark.parametrize("d", [64, 128, 256])
 @pytest.mark.parametrize("lens,new", [([0], [1]), ([1], [1]), ([33], [1]), ([100], [3]), ([3000, 40, 5000] * 30, [1] * 90),
