@@ -62,17 +62,19 @@ struct Kv4DecParams {
 // What one item visits: pages [0, npg) of its list, less those that lie outside every row's window.
 struct Kv4Item {
   int qstart, ntok, npg;
+  int blocks;               // blocks of query rows
   int sink_pg, skip;        // pages [sink_pg, sink_pg + skip) of the list are never fetched
   int all_from, all_to;     // positions [all_from, all_to) are seen by every row (so is the sink below the window)
   const int* list;
 };
 
-template <bool EXT>
+template <bool EXT, int ROWS>
 __device__ __forceinline__ Kv4Item kv4_item(const Kv4DecParams& p, int item) {
   Kv4Item d;
   const int b = p.item_seq[item];
   d.qstart = p.item_qstart[item];
   d.ntok = p.item_ntok[item];
+  d.blocks = max(1, min(p.row_blocks, (d.ntok * p.group + ROWS - 1) / ROWS));
   int reach = 0, to = 0x7fffffff, from = 0, first = 0x7fffffff;
   for (int i = 0; i < d.ntok; ++i) {
     const int n = p.q_kvlen[d.qstart + i];
@@ -255,8 +257,11 @@ __global__ void __launch_bounds__(KV4_DEC_THREADS, Kv4DecShape<D, NT>::CTAS) kv4
     // word, and runs as well after a wait that ran out has ended the producer early
     p.part_unit[blockIdx.x * 4] = 0;
   }
-  // slots of every item (an item without a visible position takes one, so that its rows get written)
-  for (int i = threadIdx.x; i < p.num_items; i += KV4_DEC_THREADS) scan[i] = max(1, (kv4_item<EXT>(p, i).npg + 1) >> 1);
+  // slots of every item over its row blocks (an item without a visible position takes one, so that its rows get written)
+  for (int i = threadIdx.x; i < p.num_items; i += KV4_DEC_THREADS) {
+    const Kv4Item d = kv4_item<EXT, ROWS>(p, i);
+    scan[i] = max(1, (d.npg + 1) >> 1) * d.blocks;
+  }
   __syncthreads();
   if (warp == 0) {
     int sum = 0;
@@ -274,8 +279,7 @@ __global__ void __launch_bounds__(KV4_DEC_THREADS, Kv4DecShape<D, NT>::CTAS) kv4
     if (lane == 0) scan[p.num_items] = sum;
   }
   __syncthreads();
-  const int per_item = p.hkv * p.row_blocks;
-  const long long total = static_cast<long long>(scan[p.num_items]) * per_item;
+  const long long total = static_cast<long long>(scan[p.num_items]) * p.hkv;
   const long long share = max((total + gridDim.x - 1) / gridDim.x, static_cast<long long>(KV4_DEC_MIN_SHARE));
   const long long begin = blockIdx.x * share, end = min(total, begin + share);
   if (begin >= end) return;
@@ -285,22 +289,22 @@ __global__ void __launch_bounds__(KV4_DEC_THREADS, Kv4DecShape<D, NT>::CTAS) kv4
     int lo = 0, hi = p.num_items - 1;  // the item that holds slot `begin`
     while (lo < hi) {
       const int mid = (lo + hi + 1) >> 1;
-      if (static_cast<long long>(scan[mid]) * per_item <= begin) lo = mid;
+      if (static_cast<long long>(scan[mid]) * p.hkv <= begin) lo = mid;
       else hi = mid - 1;
     }
     int item = lo;
     long long at = begin;
     uint32_t g = 0, k = 0;
     bool ok = true;
-    Kv4Item d = kv4_item<EXT>(p, item);
+    Kv4Item d = kv4_item<EXT, ROWS>(p, item);
     while (at < end && ok) {
-      if (at >= static_cast<long long>(scan[item + 1]) * per_item) d = kv4_item<EXT>(p, ++item);
-      const int n = scan[item + 1] - scan[item];
-      const int local = static_cast<int>(at - static_cast<long long>(scan[item]) * per_item);
+      if (at >= static_cast<long long>(scan[item + 1]) * p.hkv) d = kv4_item<EXT, ROWS>(p, ++item);
+      const int n = (scan[item + 1] - scan[item]) / d.blocks;
+      const int local = static_cast<int>(at - static_cast<long long>(scan[item]) * p.hkv);
       const int unit = local / n, slot0 = local % n;
       const int take = static_cast<int>(min(static_cast<long long>(n - slot0), end - at));
       const bool begins = slot0 == 0, ends = slot0 + take == n;
-      const int hk = unit / p.row_blocks, row0 = unit % p.row_blocks * ROWS;
+      const int hk = unit / d.blocks, row0 = unit % d.blocks * ROWS;
       const int rows = min(ROWS, d.ntok * p.group - row0);
       // ---- descriptor and query rows
       const int e = k & 1;
@@ -393,7 +397,7 @@ __global__ void __launch_bounds__(KV4_DEC_THREADS, Kv4DecShape<D, NT>::CTAS) kv4
     ok = __all_sync(0xffffffffu, ok);
     const Kv4Piece pc = *reinterpret_cast<const Kv4Piece*>(reinterpret_cast<const uint8_t*>(pieces) + e * 64);
     if (!ok) break;  // a wait of some role ran out: the others find out by the abort flag
-    const int rows = min(ROWS, pc.ntok * p.group - pc.row0);  // may be <= 0: an empty row block
+    const int rows = min(ROWS, pc.ntok * p.group - pc.row0);  // 0: an item without tokens
     const int npg = pc.npg;
     // Q^T fragments: lane (r, t) has channels 8 t .. 8 t + 7 of every group of row r (+ 8 per n-tile), two k-steps each.
     // They stay in shared memory, one 16-byte load per group and slot. Rows behind the last hold anything: a column of

@@ -48,6 +48,13 @@ def build_tiles(q_indptr: np.ndarray, group: int, decode_items: bool = True, til
     return out
 
 
+def decode_rows(q_indptr: np.ndarray, group: int) -> int:
+    """Query rows (tokens x heads of a group) of the largest decode item that :func:`build_tiles` makes, 16 without any."""
+    rows = np.diff(np.asarray(q_indptr, dtype=np.int64)) * group
+    rows = rows[(rows > 0) & (rows <= 16)]
+    return int(rows.max()) if rows.size else 16
+
+
 @dataclasses.dataclass
 class AttentionPlan:
     """Device-resident tiling of one forward call (shared by all layers)."""

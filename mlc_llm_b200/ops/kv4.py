@@ -26,7 +26,7 @@ import torch
 
 from . import reference as ref
 from ._lib import DTYPE_CODE, check, lib, status_word
-from .attention import AttentionPlan, build_tiles, sm_count
+from .attention import AttentionPlan, build_tiles, decode_rows, sm_count
 from .reference import KV4_BOUND, KV4_GROUP, is_kv4, kv4_row
 
 _P, _I, _L, _F = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_float
@@ -172,8 +172,8 @@ def kv4_plan(q_indptr, q_kvlen: torch.Tensor, page_indptr: torch.Tensor, page_in
     return AttentionPlan(on["tile_seq"], on["tile_qstart"], on["tile_ntok"], q_kvlen, page_indptr, page_indices,
                          num_tiles, dec_seq=on["dec_seq"], dec_qstart=on["dec_qstart"], dec_ntok=on["dec_ntok"],
                          num_dec=num_dec, dec_splits=1, max_pages=(int(max_len) + 15) // 16, tile_rows=KV4_TILE_ROWS,
-                         dec_rows=int(tiles["dec_ntok"].max()) * (hq // hkv) if num_dec else 16,
-                         tokens=int(q_indptr[-1]), group=hq // hkv, seqs=len(q_indptr) - 1)
+                         dec_rows=decode_rows(q_indptr, hq // hkv), tokens=int(q_indptr[-1]), group=hq // hkv,
+                         seqs=len(q_indptr) - 1)
 
 
 def _decode_ctas(num_items: int, hkv: int, max_pages: int, device: torch.device) -> int:
@@ -183,14 +183,14 @@ def _decode_ctas(num_items: int, hkv: int, max_pages: int, device: torch.device)
     return min(4 * sm_count(device), 1 << max(0, (slots + 3) // 4 - 1).bit_length())
 
 
-def decode_launch(num_dec: int, hkv: int, d: int, max_pages: int, device: torch.device) -> int:
-    """What the launch of ``num_dec`` decode items depends on besides array shapes: a captured graph holds for equal
-    values of this number."""
+def decode_launch(num_dec: int, hkv: int, d: int, max_pages: int, rows: int, device: torch.device) -> int:
+    """What the launch of ``num_dec`` decode items of at most ``rows`` query rows depends on besides array shapes: a
+    captured graph holds for equal values of this number."""
     if d not in KV4_HEAD_DIMS:
         return 0
     if d == 96:
         return _prefill_splits(num_dec * hkv, max_pages // 8, device)
-    return _decode_ctas(num_dec, hkv, max_pages, device)
+    return _decode_ctas(num_dec, hkv, max_pages, device) * 2 + (rows > 8)  # more than 8 rows: another kernel, or two units
 
 
 def attend(q: torch.Tensor, kv_pages: torch.Tensor, q_seq: torch.Tensor, q_kvlen: torch.Tensor, page_indptr: torch.Tensor,

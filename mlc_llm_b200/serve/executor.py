@@ -366,7 +366,7 @@ class ModelExecutor:
         if "tile_seq" in dev and self._tc_attention_ok(model):
             from ..ops.attention import AttentionPlan  # pylint: disable=import-outside-toplevel
 
-            from ..ops.attention import choose_splits  # pylint: disable=import-outside-toplevel
+            from ..ops.attention import choose_splits, decode_rows  # pylint: disable=import-outside-toplevel
 
             n_dec = int(dev["dec_seq"].numel())
             max_pages = (int(plan["max_seq_len"]) + 15) // 16
@@ -375,7 +375,8 @@ class ModelExecutor:
                                         dec_seq=dev["dec_seq"], dec_qstart=dev["dec_qstart"],
                                         dec_ntok=dev["dec_ntok"], num_dec=n_dec,
                                         dec_splits=choose_splits(n_dec, model.hkv, max_pages, self.device)
-                                        if n_dec else 1, max_pages=max_pages, tile_rows=self._tile_rows(model))
+                                        if n_dec else 1, max_pages=max_pages, tile_rows=self._tile_rows(model),
+                                        dec_rows=decode_rows(plan["q_indptr"], model.hq // model.hkv))
         return b
 
     def _tc_attention_ok(self, model: DecoderModel) -> bool:
@@ -470,13 +471,13 @@ class ModelExecutor:
                 and dev["q_kvstart"].numel() == 0)
 
     def _run_graph(self, model_id: int, plan: dict, dev: Dict[str, torch.Tensor]) -> torch.Tensor:
-        from ..ops.attention import choose_splits  # pylint: disable=import-outside-toplevel
+        from ..ops.attention import choose_splits, decode_rows  # pylint: disable=import-outside-toplevel
 
         model = self.models[model_id]
         max_pages = (int(plan["max_seq_len"]) + 15) // 16
         n_dec = int(dev["dec_seq"].numel())
-        splits = ops.kv4.decode_launch(n_dec, model.hkv, model.d, max_pages, self.device) if model.kv4 \
-            else choose_splits(n_dec, model.hkv, max_pages, self.device)
+        splits = choose_splits(n_dec, model.hkv, max_pages, self.device) if not model.kv4 else ops.kv4.decode_launch(
+            n_dec, model.hkv, model.d, max_pages, decode_rows(plan["q_indptr"], model.hq // model.hkv), self.device)
         shape = tuple((k, int(v.numel())) for k, v in dev.items() if not k.startswith("s_") and k != "page_indices")
         key = (model_id, self.staging.generation, splits, shape)
         entry = self._graphs.get(key)

@@ -54,3 +54,18 @@ def test_a_plan_of_other_sequences_or_another_device_is_refused():
         other = dataclasses.replace(plan, **{name: getattr(plan, name).to("meta")})
         with pytest.raises(ValueError, match="plan's items"):
             call(other, indptr)
+
+
+def test_rows_of_the_largest_decode_item(monkeypatch):
+    from mlc_llm_b200.ops.attention import build_tiles, decode_rows
+
+    rng = np.random.default_rng(1)
+    for group in (1, 3, 4, 8, 16, 20):
+        for _ in range(50):
+            q_indptr = np.concatenate([[0], np.cumsum(rng.integers(0, 20, rng.integers(0, 6)))])
+            items = build_tiles(q_indptr, group)["dec_ntok"]
+            assert decode_rows(q_indptr, group) == (int(items.max()) * group if items.size else 16)
+    # the kernel that a captured step holds depends on it
+    monkeypatch.setattr(ops.kv4, "sm_count", lambda device: 148)
+    launch = lambda rows, d=128: ops.kv4.decode_launch(8, 2, d, 100, rows, torch.device("cuda"))
+    assert launch(4) == launch(8) != launch(9) == launch(16) and launch(4, 256) != launch(16, 256)
