@@ -134,6 +134,53 @@ def test_waiting_for_copies_in_flight_takes_no_time(lens, new, d):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+def test_more_decode_items_than_one_launch_takes(dtype):
+    g = torch.Generator().manual_seed(3)
+    lens = torch.randint(1, 41, (1100,), generator=g).tolist()
+    lens[5], lens[1060] = 900, 5000      # one unit cut between CTAs in either batch of items
+    st = Step(dtype, lens, [1] * 1100, 8, 2, 64, seed=9)
+    assert st.plan.num_dec == 1100
+    out, lse = st.run()
+    ops.check_status(out.device)
+    st.check(out, lse)
+    assert _same_bytes(out, st.run(lse=False))
+
+
+@pytest.mark.parametrize("lens,new,hq,hkv,d", [([1000, 300], [1, 1], 8, 2, 128), ([1000, 300], [3, 4], 8, 2, 64),
+                                               ([1000, 300], [40, 70], 8, 2, 128), ([1000, 300], [30, 50], 8, 4, 256),
+                                               ([500, 300], [1, 2], 4, 2, 32)])
+def test_pages_that_a_window_released(lens, new, hq, hkv, d):
+    """Pages between the sinks and the window of a sequence's first query row are given back: their numbers are -1."""
+    for dtype in TYPES:
+        st = Step(dtype, lens, new, hq, hkv, d, window=70, sink=4, seed=d)
+        kept = [st.run(plan=plan) for plan in (True, False)]
+        gone = 0
+        for i in range(len(lens)):
+            first = int(st.kvstart[int(st.q_indptr[i])])
+            for pg in range(1, first // 16):  # page 0 holds the sinks
+                st.indices[int(st.indptr[i]) + pg] = -1
+                gone += 1
+        assert gone > 20
+        for plan, want in zip((True, False), kept):
+            out, lse = st.run(plan=plan)
+            ops.check_status(out.device)
+            st.check(out, lse)
+            assert _same_bytes(out, want[0]) and _same_bytes(lse, want[1])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("lens,new,d,extra", [([200, 33], [1, 3], 128, {}), ([200, 90], [60, 33], 128, {}),
+                                              ([200, 90], [60, 33], 256, {"cap": 30.0}), ([200, 33], [1, 3], 64, {"cap": 30.0})])
+def test_negative_scale(dtype, lens, new, d, extra):
+    st = Step(dtype, lens, new, 8, 2, d, seed=4, **extra)
+    flipped = torch.empty_like(st.qkv).copy_(st.qkv).neg_()[:, : 8 * d]
+    for plan in (True, False):
+        out, lse = _attend(st, plan, flipped, -(d ** -0.5))
+        ops.check_status(out.device)
+        st.check(out, lse)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("lens,new,hq,hkv,d", [([100, 40], [1, 1], 32, 1, 128), ([300, 40], [5, 1], 71, 1, 64),
                                                ([90, 900], [1, 1], 20, 1, 256), ([60, 30], [2, 1], 300, 1, 64),
                                                ([200, 300, 60], [1, 4, 1], 16, 4, 256), ([200, 300], [4, 1], 16, 4, 128)])
@@ -144,3 +191,23 @@ def test_query_groups(dtype, lens, new, hq, hkv, d):
     out, lse = st.run()
     ops.check_status(out.device)
     st.check(out, lse)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("lens,new,d", [([200, 33], [1, 3], 128), ([200, 90], [60, 33], 128), ([200, 90], [60, 33], 256),
+                                        ([200, 33], [1, 3], 64), ([50, 20], [4, 1], 32)])
+def test_queries_that_are_not_finite(dtype, lens, new, d):
+    st = Step(dtype, lens, new, 8, 2, d, seed=7)
+    clean = st.run()
+    st.check(*clean)
+    bad = sum(new) - 2
+    others = [t for t in range(sum(new)) if t != bad]
+    for value in (math.nan, math.inf, -math.inf):
+        q = st.qkv.clone()
+        q[bad, 3: 8 * d: d] = value  # one channel of every head
+        for plan in (True, False):
+            out, lse = st.run(plan=plan, q=q[:, : 8 * d])
+            ops.check_status(out.device)
+            _check_rows(st, out, lse, others)
+            if value != value:
+                assert bool(torch.isnan(out[bad]).all()) and bool(torch.isnan(lse[bad]).all())
