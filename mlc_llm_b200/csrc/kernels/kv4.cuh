@@ -135,6 +135,139 @@ __device__ __forceinline__ void kv4_words(const uint8_t* p, uint32_t (&w)[N]) {
   }
 }
 
+// bf16 rows are scaled by a power of two into fp16's range, one for many positions. What a position needs: with
+// |lo| < 2^(e + 13) and s < 2^(e + 9) its scaled values, at most |lo| + 15 s, stay below 2^14. `top` is the largest pair
+// (|lo|, s) of its groups, halves apart.
+__device__ __forceinline__ int kv4_need(uint32_t top) {
+  return max(static_cast<int>(top >> 23) - 9, static_cast<int>((top & 0xffffu) >> 7) - 13) - 126;
+}
+constexpr int KV4_NEEDS_NONE = -135;  // of zeros (and of what is as small: below 2^-113)
+// What that rounds away is small against the largest value. A row is entitled to that of the largest value that it sees, which
+// positions that only other rows see must not push out of fp16's range: later tokens, other branches of a draft tree, tokens below
+// its window, an infinity among them. Where those need 2^KV4_WIDE times more than what the row is sure to see, all rows of the tile
+// are computed again by kv4_rows_exact. Below that the largest value that a row sees keeps its 11 bits, and others are off by
+// 2^-22 of it at most.
+constexpr int KV4_WIDE = 12;
+
+// KV4_EXACT query rows over positions at(i), 0 <= i < to (-1: none there), of which row r sees sees(r, position), in fp32 from the
+// packed rows as they are, by one warp: lane = position for the scores, then lane = code word for the values, SHARE positions side
+// by side. Gives per row the maximum (log2), the sum of the weights against it, and in the first D / 8 lanes the weighted sums of
+// channels 8 lane .. 8 lane + 7. The rows share what is read and unpacked (64 verify chunks of four tokens at 4000 positions, 32 / 8
+// heads of 128: 10 ms, one row at a time 30). It reads global memory with nothing to hide that behind, 40 to 100 times slower than
+// the tensor cores, and is no path for ordinary values: 16 rows take 2 us per position, so that a million positions in one CTA would
+// exhaust the waits of its other warps.
+constexpr int KV4_EXACT = 4;
+template <typename T, int D, typename At, typename Sees>
+__device__ __forceinline__ void kv4_rows_exact(const uint8_t* pages, long long num_pages, const int* list, int hkv, int hk,
+                                               const T* const (&q)[KV4_EXACT], float sign, float scale_log2, float cap_k, float cap_log2,
+                                               int to, At&& at, Sees&& sees, float (&m)[KV4_EXACT], float (&l)[KV4_EXACT],
+                                               float (&acc)[KV4_EXACT][8]) {
+  constexpr int GROUPS = D / KV4_GROUP, ROW = kv4_row_bytes(D), WORDS = D / 8, SHARE = 32 / WORDS, R = KV4_EXACT;
+  const int lane = threadIdx.x & 31, word = lane % WORDS;
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    m[r] = -INFINITY;
+    l[r] = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) acc[r][j] = 0.f;
+  }
+  const size_t to_v = static_cast<size_t>(hkv) * KV4_PAGE * ROW;
+#pragma unroll 1
+  for (int base = 0; base < to; base += 32) {
+    const int pos = base + lane < to ? at(base + lane) : -1;
+    bool see[R];
+    unsigned long long key = 0;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      see[r] = pos >= 0 && sees(r, pos);
+      if (see[r]) key = 1;
+    }
+    if (key) {
+      const int pg = list[pos / KV4_PAGE];
+      key = 0;
+      if (pg >= 0 && pg < num_pages)  // others are reported where the pages are copied
+        key = reinterpret_cast<unsigned long long>(pages + ((static_cast<size_t>(pg) * 2 * hkv + hk) * KV4_PAGE + pos % KV4_PAGE) * ROW);
+    }
+    if (!__any_sync(0xffffffffu, key != 0)) continue;
+    float score[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) score[r] = 0.f;
+    if (key) {
+      const uint32_t* row = reinterpret_cast<const uint32_t*>(key);
+#pragma unroll 1
+      for (int g = 0; g < GROUPS; ++g) {
+        const uint32_t meta = row[WORDS + g];
+        const T* pair = reinterpret_cast<const T*>(&meta);
+        const float lo = Cvt<T>::to_f(pair[0]), st = Cvt<T>::to_f(pair[1]);
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const uint32_t w = row[g * 4 + x];
+          float k[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) k[j] = fmaf(st, static_cast<float>(kv4_code(w, j)), lo);
+#pragma unroll
+          for (int r = 0; r < R; ++r) {
+            const uint4 v = reinterpret_cast<const uint4*>(q[r])[g * 4 + x];
+            const T* e = reinterpret_cast<const T*>(&v);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) score[r] = fmaf(Cvt<T>::to_f(e[j]), k[j], score[r]);
+          }
+        }
+      }
+    }
+    float weight[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      float sc = score[r] * sign;
+      sc = cap_log2 != 0.f ? kv4_softcap(sc, cap_k, cap_log2) : sc * scale_log2;
+      if (!see[r] || !key) sc = -INFINITY;
+      const float mn = fmaxf(m[r], warp_max(sc)), f = m[r] == -INFINITY ? 0.f : exp2f(m[r] - mn);
+      weight[r] = see[r] && key ? exp2f(sc - (mn == -INFINITY ? 0.f : mn)) : 0.f;
+      m[r] = mn;
+      l[r] = l[r] * f + weight[r];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) acc[r][j] *= f;
+    }
+#pragma unroll 2
+    for (int x = 0; x < 32; x += SHARE) {
+      const int from = (x + lane / WORDS) & 31;
+      float w[R];
+#pragma unroll
+      for (int r = 0; r < R; ++r) w[r] = __shfl_sync(0xffffffffu, weight[r], from);
+      const unsigned long long row = __shfl_sync(0xffffffffu, key, from);
+      if (lane >= SHARE * WORDS || !row) continue;
+      const uint32_t* v = reinterpret_cast<const uint32_t*>(row + to_v);
+      const uint32_t code = v[word], meta = v[WORDS + word / 4];
+      const T* pair = reinterpret_cast<const T*>(&meta);
+      const float lo = Cvt<T>::to_f(pair[0]), st = Cvt<T>::to_f(pair[1]);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float y = fmaf(st, static_cast<float>(kv4_code(code, j)), lo);
+#pragma unroll
+        for (int r = 0; r < R; ++r) acc[r][j] = fmaf(w[r], y, acc[r][j]);
+      }
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    l[r] = warp_sum(l[r]);
+#pragma unroll
+    for (int o = SHARE / 2 * WORDS; o >= WORDS; o /= 2)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) acc[r][j] += __shfl_down_sync(0xffffffffu, acc[r][j], o);
+  }
+}
+// 8 neighbouring channels of a row, as fp32 and in the rows' type.
+__device__ __forceinline__ void kv4_put8(float* dst, const float (&v)[8]) {
+  reinterpret_cast<float4*>(dst)[0] = make_float4(v[0], v[1], v[2], v[3]);
+  reinterpret_cast<float4*>(dst)[1] = make_float4(v[4], v[5], v[6], v[7]);
+}
+template <typename T>
+__device__ __forceinline__ void kv4_put8(T* dst, const float (&v)[8], float by) {
+  *reinterpret_cast<uint4*>(dst) = make_uint4(Kv4Type<T>::pack(v[0] * by, v[1] * by), Kv4Type<T>::pack(v[2] * by, v[3] * by),
+                                              Kv4Type<T>::pack(v[4] * by, v[5] * by), Kv4Type<T>::pack(v[6] * by, v[7] * by));
+}
+
 // Waits until phase `parity` of a barrier is over, no matter whether a wait of some role ran out: before a CTA gives up its
 // shared memory and TMEM, the copies and products in flight have to land. They do so by themselves; the limit (about 50 ms)
 // is for a phase that the hardware never ends.

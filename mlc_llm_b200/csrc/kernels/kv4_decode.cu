@@ -116,6 +116,7 @@ struct Kv4Piece {
   int qstart, ntok, hk, row0;
   int slot0, slots;         // slots of the unit: first, count (0: nothing visible)
   int npg, sink_pg, skip, all_from, all_to;
+  int list0;                // the sequence's first entry of page_indices
   int part;                 // -1: the whole unit, written to out; else the row block of part_o it goes to
   int last;                 // the share ends here
 };
@@ -199,6 +200,50 @@ __device__ __forceinline__ void kv4_finish_row(const Kv4DecParams& p, int qstart
   if (p.lse && lane == 0) p.lse[at] = L == 0.f ? -INFINITY : (M + log2f(L)) * 0.6931471805599453f;
 }
 
+// The rows of one piece by kv4_rows_exact. A call of its own, so that it takes no registers from the ordinary path.
+template <typename T, int D, bool EXT>
+__device__ __noinline__ void kv4_piece_exact(const Kv4DecParams& p, const Kv4Piece* piece, int rows) {
+  const Kv4Piece pc = *piece;
+  const int lane = threadIdx.x & 31, npg = pc.npg;
+  auto at = [&](int i) {
+    const int pi = pc.slot0 * 2 + i / KV4_PAGE;
+    return pi >= npg ? -1 : (!EXT || pi < pc.sink_pg ? pi : pi + pc.skip) * KV4_PAGE + i % KV4_PAGE;
+  };
+#pragma unroll 1
+  for (int first = 0; first < rows; first += KV4_EXACT) {
+    int tok[KV4_EXACT], kvlen[KV4_EXACT], start[KV4_EXACT];
+    size_t to[KV4_EXACT];  // the row of (token, head)
+    unsigned long long tm[KV4_EXACT];
+    const T* q[KV4_EXACT];
+#pragma unroll
+    for (int i = 0; i < KV4_EXACT; ++i) {
+      const int row = pc.row0 + min(first + i, rows - 1), head = pc.hk * p.group + row % p.group;
+      tok[i] = pc.qstart + row / p.group;
+      to[i] = static_cast<size_t>(tok[i]) * p.hq + head;
+      q[i] = reinterpret_cast<const T*>(p.q) + static_cast<size_t>(tok[i]) * p.q_stride + head * D;
+      kvlen[i] = p.q_kvlen[tok[i]];
+      start[i] = EXT && p.q_kvstart ? p.q_kvstart[tok[i]] : 0;
+      tm[i] = EXT && p.tree_mask ? p.tree_mask[tok[i]] : 0ull;
+    }
+    auto sees = [&](int i, int pos) { return kv4_visible(pos, kvlen[i], start[i], p.sink, tm[i]); };
+    float M[KV4_EXACT], L[KV4_EXACT], acc[KV4_EXACT][8];
+    kv4_rows_exact<T, D>(p.pages, p.num_pages, p.page_indices + pc.list0, p.hkv, pc.hk, q, 1.f, p.scale_log2,
+                         EXT ? p.cap_k : 0.f, EXT ? p.cap_log2 : 0.f, pc.slots * 2 * KV4_PAGE, at, sees, M, L, acc);
+#pragma unroll
+    for (int i = 0; i < KV4_EXACT; ++i) {
+      if (first + i >= rows) continue;
+      if (pc.part >= 0) {
+        const size_t part = static_cast<size_t>(pc.part) * 16 + first + i;
+        if (lane < D / 8) kv4_put8(p.part_o + part * D + lane * 8, acc[i]);
+        if (lane == 0) reinterpret_cast<float2*>(p.part_ml)[part] = make_float2(M[i], L[i]);
+      } else {
+        if (lane < D / 8) kv4_put8(reinterpret_cast<T*>(p.out) + to[i] * D + lane * 8, acc[i], L[i] == 0.f ? 0.f : 1.f / L[i]);
+        if (p.lse && lane == 0) p.lse[to[i]] = L[i] == 0.f ? -INFINITY : (M[i] + log2f(L[i])) * 0.6931471805599453f;
+      }
+    }
+  }
+}
+
 template <int D, int NT>
 struct Kv4DecShape {
   static constexpr int ROW = kv4_row_bytes(D);
@@ -221,8 +266,9 @@ struct Kv4DecShape {
   static_assert(sizeof(Kv4Piece) <= 64, "a piece descriptor has 64 bytes");
 };
 
-template <typename T, int D, int NT, bool EXT>
-__global__ void __launch_bounds__(KV4_DEC_THREADS, Kv4DecShape<D, NT>::CTAS) kv4_decode_kernel(const Kv4DecParams p) {
+// EXT: masks or a soft cap. GUARD: bf16 items of several tokens, whose rows see different positions (kv4.cuh).
+template <typename T, int D, int NT, bool EXT, bool GUARD>
+__global__ void __launch_bounds__(KV4_DEC_THREADS, Kv4DecShape<D, NT>::CTAS) kv4_decode_kernel(const __grid_constant__ Kv4DecParams p) {
   using Shape = Kv4DecShape<D, NT>;
   constexpr int ROW = Shape::ROW, PB = Shape::PAGE_BYTES, SLOTS = Shape::SLOTS, ROWS = Shape::ROWS;
   constexpr int GROUPS = D / KV4_GROUP;
@@ -239,6 +285,7 @@ __global__ void __launch_bounds__(KV4_DEC_THREADS, Kv4DecShape<D, NT>::CTAS) kv4
   Kv4Piece* pieces = reinterpret_cast<Kv4Piece*>(smem + Shape::OFF_PIECE);  // [2], 64 bytes apart
   int* scan = reinterpret_cast<int*>(smem + Shape::OFF_SCAN);               // [num_items + 1]
   __shared__ int abort_word;
+  __shared__ int wide[2];  // bf16: a piece's rows do not share a scale (kv4.cuh)
   volatile int* abort_flag = &abort_word;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x < SLOTS) {
@@ -326,6 +373,8 @@ __global__ void __launch_bounds__(KV4_DEC_THREADS, Kv4DecShape<D, NT>::CTAS) kv4
         pc->skip = d.skip;
         pc->all_from = d.all_from;
         pc->all_to = d.all_to;
+        pc->list0 = static_cast<int>(d.list - p.page_indices);
+        wide[e] = 0;
         pc->part = begins && ends ? -1 : static_cast<int>(blockIdx.x) * 2 + (begins ? 1 : 0);
         pc->last = at + take >= end;
         if (at + take >= end) {
@@ -448,6 +497,7 @@ __global__ void __launch_bounds__(KV4_DEC_THREADS, Kv4DecShape<D, NT>::CTAS) kv4
     float o[NT][D / 16][4];
     float m[NT][2], l[NT][2];
     int v_exp = -1000;  // bf16: V is scaled by 2^-v_exp into fp16's range
+    int v_all = -1000, v_part = -1000;  // the largest need of positions that every row sees (a lane's), and of others
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       // A column behind the last row has an infinite maximum, weights of 0 and never asks for a rescaling: it holds the
@@ -552,9 +602,24 @@ __global__ void __launch_bounds__(KV4_DEC_THREADS, Kv4DecShape<D, NT>::CTAS) kv4
                 if (!live || !sees((pg ? at1 : at0) + r + h * 8, tok)) sc[pg][nt][c + 2 * h] = -INFINITY;
           }
         const int pos = (lane < 16 ? at0 : at1) + (lane & 15);  // lane = token of the slot
-        bool any = false;
-        for (int q = 0; q < pc.ntok; ++q) any = any || sees(pos, pc.qstart + q);
+        bool any = false, every = true;
+        for (int q = 0; q < pc.ntok; ++q) {
+          const bool it = sees(pos, pc.qstart + q);
+          any = any || it;
+          every = every && it;
+        }
         seen = __ballot_sync(0xffffffffu, any);
+        if (GUARD && pc.ntok > 1) {
+          // what only some rows see must not crowd out what others see when V is scaled (kv4.cuh)
+          uint32_t vm[GROUPS], most = 0;
+          kv4_words<GROUPS>(slot + ((lane >> 4) * 2 + 1) * PB + (lane & 15) * ROW + D / 2, vm);
+#pragma unroll
+          for (int grp = 0; grp < GROUPS; ++grp) most = __vmaxu2(most, vm[grp] & 0xffff7fffu);
+          const int one = any ? kv4_need(most) : KV4_NEEDS_NONE;
+          v_part = max(v_part, __reduce_max_sync(0xffffffffu, one > KV4_NEEDS_NONE && !every ? one : -1000));
+          const int low = __reduce_min_sync(0xffffffffu, one > KV4_NEEDS_NONE ? one : 1000);
+          if (v_part > max(__reduce_max_sync(0xffffffffu, v_all), low) + KV4_WIDE && lane == 0) wide[e] = 1;
+        }
       }
       // ---- running maximum (raised lazily) and P
       bool raise = false;
@@ -615,14 +680,15 @@ __global__ void __launch_bounds__(KV4_DEC_THREADS, Kv4DecShape<D, NT>::CTAS) kv4
         }
       float shrink = 1.f;
       if constexpr (BF16) {
-        // |v| <= |lo| + 15 s: with |lo| < 2^(v_exp + 13) and s < 2^(v_exp + 9) the scaled values stay below 2^14. A larger
-        // one raises v_exp for good (O is rescaled); smaller ones keep their 11 bits down to 2^-28 of the largest.
+        // A larger value raises v_exp for good (O is rescaled). The largest lies between 2^9 and 2^14 then (v_exp is a multiple
+        // of 4): values keep their 11 bits down to 2^-23 of it.
         uint32_t top = 0;
 #pragma unroll
         for (int pg = 0; pg < 2; ++pg)
 #pragma unroll
           for (int x = 0; x < 4; ++x) top = __vmaxu2(top, meta[pg][x] & 0xffff7fffu);
-        const int need = max(static_cast<int>(top >> 23) - 9, static_cast<int>((top & 0xffffu) >> 7) - 13) - 126;
+        const int need = kv4_need(top);
+        if (GUARD && plain) v_all = max(v_all, need);
         if (__any_sync(0xffffffffu, need > v_exp)) {
           const int e2 = (__reduce_max_sync(0xffffffffu, need) + 1027) / 4 * 4 - 1024;  // in steps of 4
           const float f = v_exp == -1000 ? 1.f : exp2f(static_cast<float>(max(v_exp - e2, -126)));
@@ -687,6 +753,10 @@ __global__ void __launch_bounds__(KV4_DEC_THREADS, Kv4DecShape<D, NT>::CTAS) kv4
         l[nt][c] += __shfl_xor_sync(0xffffffffu, l[nt][c], 16);
       }
     if constexpr (BF16) {
+      if (GUARD && v_part > -1000) {
+        const int all = __reduce_max_sync(0xffffffffu, v_all);
+        if (all > KV4_NEEDS_NONE && v_part > all + KV4_WIDE && lane == 0) wide[e] = 1;
+      }
       const float f = exp2f(static_cast<float>(max(v_exp, -126)));  // untouched (-1000): o is 0
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
@@ -739,31 +809,37 @@ __global__ void __launch_bounds__(KV4_DEC_THREADS, Kv4DecShape<D, NT>::CTAS) kv4
       ok = mbar_wait(&merge_full[e], (k >> 1) & 1, abort_flag, p.status, ERR_WAIT_EPILOGUE);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
+      __syncwarp();
+      if (GUARD && wide[e]) {
+        if constexpr (GUARD)
+          kv4_piece_exact<T, D, EXT>(p, reinterpret_cast<const Kv4Piece*>(reinterpret_cast<const uint8_t*>(pieces) + e * 64), rows);
+      } else {
 #pragma unroll 1
-      for (int b = 0; b < 3; ++b) take(e * 3 + b);
+        for (int b = 0; b < 3; ++b) take(e * 3 + b);
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          const int row = nt * 8 + 2 * t + c;
-          if (row >= rows) continue;
-          if (pc.part >= 0) {
-            const size_t at = static_cast<size_t>(pc.part) * 16 + row;
-            float2* dst = reinterpret_cast<float2*>(p.part_o + at * D + r * (D / 8));
+          for (int c = 0; c < 2; ++c) {
+            const int row = nt * 8 + 2 * t + c;
+            if (row >= rows) continue;
+            if (pc.part >= 0) {
+              const size_t at = static_cast<size_t>(pc.part) * 16 + row;
+              float2* dst = reinterpret_cast<float2*>(p.part_o + at * D + r * (D / 8));
 #pragma unroll
-            for (int j = 0; j < D / 16; ++j) dst[j] = make_float2(o[nt][j][c], o[nt][j][c + 2]);
-            if (r == 0) reinterpret_cast<float2*>(p.part_ml)[at] = make_float2(m[nt][c], l[nt][c]);
-          } else {
-            // a row that sees nothing is 0; NaN stays NaN
-            const float L = l[nt][c], inv = L == 0.f ? 0.f : 1.f / L;
-            const size_t at = static_cast<size_t>(pc.qstart + (pc.row0 + row) / p.group) * p.hq + pc.hk * p.group +
-                              (pc.row0 + row) % p.group;
-            uint32_t* dst = reinterpret_cast<uint32_t*>(reinterpret_cast<T*>(p.out) + at * D + r * (D / 8));
+              for (int j = 0; j < D / 16; ++j) dst[j] = make_float2(o[nt][j][c], o[nt][j][c + 2]);
+              if (r == 0) reinterpret_cast<float2*>(p.part_ml)[at] = make_float2(m[nt][c], l[nt][c]);
+            } else {
+              // a row that sees nothing is 0; NaN stays NaN
+              const float L = l[nt][c], inv = L == 0.f ? 0.f : 1.f / L;
+              const size_t at = static_cast<size_t>(pc.qstart + (pc.row0 + row) / p.group) * p.hq + pc.hk * p.group +
+                                (pc.row0 + row) % p.group;
+              uint32_t* dst = reinterpret_cast<uint32_t*>(reinterpret_cast<T*>(p.out) + at * D + r * (D / 8));
 #pragma unroll
-            for (int j = 0; j < D / 16; ++j) dst[j] = Kv4Type<T>::pack(o[nt][j][c] * inv, o[nt][j][c + 2] * inv);
-            if (p.lse && r == 0) p.lse[at] = L == 0.f ? -INFINITY : (m[nt][c] + log2f(L)) * 0.6931471805599453f;
+              for (int j = 0; j < D / 16; ++j) dst[j] = Kv4Type<T>::pack(o[nt][j][c] * inv, o[nt][j][c + 2] * inv);
+              if (p.lse && r == 0) p.lse[at] = L == 0.f ? -INFINITY : (m[nt][c] + log2f(L)) * 0.6931471805599453f;
+            }
           }
-        }
+      }
     }
     __syncwarp();
     if (lane == 0) mbar_arrive(&piece_empty[e]);
@@ -818,10 +894,10 @@ __global__ void __launch_bounds__(128) kv4_decode_merge_kernel(const Kv4DecParam
   }
 }
 
-template <typename T, int D, int NT, bool EXT>
+template <typename T, int D, int NT, bool EXT, bool GUARD>
 int kv4_decode_launch(Kv4DecParams p, int num_items, int max_ctas, cudaStream_t stream) {
   using Shape = Kv4DecShape<D, NT>;
-  auto kern = kv4_decode_kernel<T, D, NT, EXT>;
+  auto kern = kv4_decode_kernel<T, D, NT, EXT, GUARD>;
   const int batch = num_items < KV4_DEC_ITEMS ? num_items : KV4_DEC_ITEMS;
   const int most = Shape::OFF_SCAN + (KV4_DEC_ITEMS + 1) * 4;
   static int per_sm[64] = {};
@@ -865,20 +941,32 @@ int kv4_decode_launch(Kv4DecParams p, int num_items, int max_ctas, cudaStream_t 
   return static_cast<int>(cudaGetLastError());
 }
 
+template <typename T, int D, int NT>
+int kv4_decode_kind(const Kv4DecParams& p, bool ext, bool several, int num_items, int max_ctas, cudaStream_t stream) {
+  if constexpr (Kv4Type<T>::IS_BF16) {
+    // Items of one token skip the guard: 256 sequences of 512 to 2048, bf16, 133 us without and 141 with it; 64 causal verify
+    // chunks of four tokens 117 without (and wrong beside an infinity) and 121 with it.
+    if (several)
+      return ext ? kv4_decode_launch<T, D, NT, true, true>(p, num_items, max_ctas, stream)
+                 : kv4_decode_launch<T, D, NT, false, true>(p, num_items, max_ctas, stream);
+  }
+  return ext ? kv4_decode_launch<T, D, NT, true, false>(p, num_items, max_ctas, stream)
+             : kv4_decode_launch<T, D, NT, false, false>(p, num_items, max_ctas, stream);
+}
+
 template <typename T, int D>
 int kv4_decode_shape(Kv4DecParams& p, int rows, bool ext, int num_items, int max_ctas, cudaStream_t stream) {
   // Up to 8 query rows need one n-tile. 9 to 16 rows take two, which share the expanded V; at D = 256 the
   // accumulators of two would not fit the register file, and two units read the same pages instead.
+  const bool several = rows > p.group;  // tokens in an item
   if constexpr (D < 256) {
     if (rows > 8) {
       p.row_blocks = 1;
-      return ext ? kv4_decode_launch<T, D, 2, true>(p, num_items, max_ctas, stream)
-                 : kv4_decode_launch<T, D, 2, false>(p, num_items, max_ctas, stream);
+      return kv4_decode_kind<T, D, 2>(p, ext, several, num_items, max_ctas, stream);
     }
   }
   p.row_blocks = (rows + 7) / 8;
-  return ext ? kv4_decode_launch<T, D, 1, true>(p, num_items, max_ctas, stream)
-             : kv4_decode_launch<T, D, 1, false>(p, num_items, max_ctas, stream);
+  return kv4_decode_kind<T, D, 1>(p, ext, several, num_items, max_ctas, stream);
 }
 
 }  // namespace mlcb

@@ -145,11 +145,12 @@ __global__ void __launch_bounds__(Kv4PreShape<D>::THREADS, 1) kv4_prefill_kernel
   pdl_launch_dependents();
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  __shared__ uint64_t bars[2 * Shape::RAW_SLOTS + 2 * Shape::TILES + 9];
+  __shared__ uint64_t bars[2 * Shape::RAW_SLOTS + 2 * Shape::TILES + 10];
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_word;
   __shared__ Kv4Tile info;
   __shared__ int exps[4][2];  // bf16: exponents of a block's K and V; blocks j - 3 .. j are live
+  __shared__ int wide_from;   // bf16: the first block at which the rows of the tile share no scale (kv4.cuh)
   uint64_t* raw_full = bars;
   uint64_t* raw_empty = raw_full + Shape::RAW_SLOTS;
   uint64_t* tile_full = raw_empty + Shape::RAW_SLOTS;
@@ -161,6 +162,7 @@ __global__ void __launch_bounds__(Kv4PreShape<D>::THREADS, 1) kv4_prefill_kernel
   uint64_t* pv_done = o_done + 2;                // D = 256 only
   uint64_t* q_ready = pv_done + 1;
   uint64_t* mma_idle = q_ready + 1;              // every product of this CTA is over
+  uint64_t* looked = mma_idle + 1;               // wide_from is final
   volatile int* abort_flag = &abort_word;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int G = p.group;
@@ -174,10 +176,12 @@ __global__ void __launch_bounds__(Kv4PreShape<D>::THREADS, 1) kv4_prefill_kernel
   const int p0 = p.page_indptr[seq];
   const int held = p.page_indptr[seq + 1] - p0;
 
+  // rows of several tokens see different positions: the copying warp looks out for sizes that no common scale serves (kv4.cuh)
+  const bool guard = BF16 && ntok > 1;
   if (threadIdx.x == 0) {
     for (int i = 0; i < Shape::RAW_SLOTS; ++i) {
       mbar_init(&raw_full[i], 1);
-      mbar_init(&raw_empty[i], 4);
+      mbar_init(&raw_empty[i], guard ? 5 : 4);
     }
     for (int i = 0; i < Shape::TILES; ++i) {
       mbar_init(&tile_full[i], 4);
@@ -191,7 +195,9 @@ __global__ void __launch_bounds__(Kv4PreShape<D>::THREADS, 1) kv4_prefill_kernel
     mbar_init(pv_done, 1);
     mbar_init(q_ready, 4 * SUB);
     mbar_init(mma_idle, 1);
+    mbar_init(looked, 1);
     abort_word = 0;
+    wide_from = 0x7fffffff;
     mbar_fence_init();
     for (int i = 0; i < 2; ++i) {
       info.reach[i] = 0;
@@ -264,7 +270,45 @@ __global__ void __launch_bounds__(Kv4PreShape<D>::THREADS, 1) kv4_prefill_kernel
    if (warp == COPIER) {
     // ---------------------------------------------------------------- packed rows -> raw ring
     bool ok = true;
-    int m = 0;  // raw slots so far
+    int m = 0, seen = 0;  // raw slots so far, and those of them that were looked at
+    int v_part = -1000, v_all = -1000;  // the largest needs of V: of positions that only some rows see, and of others behind those
+    const int all_to = min(info.all_to[0], info.all_to[1]), all_from = max(info.all_from[0], info.all_from[1]);
+    auto look = [&](int n) {
+      const int s = n % Shape::RAW_SLOTS, j = n >> 1, base = base_of(j);
+      const bool plain = base + BLK <= all_to && (!EXT || base >= all_from || base + BLK <= p.sink);
+      if (!plain || ((n & 1) && v_part > -1000)) {  // most blocks are seen by every row, and nothing else came before them
+        if (!__all_sync(0xffffffffu, mbar_wait(&raw_full[s], (n / Shape::RAW_SLOTS) & 1, abort_flag, p.status, ERR_WAIT_TMA))) return false;
+        const int reach = static_cast<int>(min(static_cast<long long>(max(info.reach[0], info.reach[1])), room));
+        const int first = EXT && p.q_kvstart ? info.first : 0;
+        int all = KV4_NEEDS_NONE, part = -1000, low = 1000;  // of the block: seen by every row, others, the smallest
+        for (int t = lane; t < BLK; t += 32) {
+          const int pos = base + t;
+          const uint32_t* pr = reinterpret_cast<const uint32_t*>(smem + Shape::OFF_RAW + s * Shape::RAW_BYTES + t * ROW + D / 2);
+          uint32_t top = 0;
+#pragma unroll
+          for (int g = 0; g < GROUPS; ++g) top = __vmaxu2(top, pr[g] & 0xffff7fffu);
+          const int need = kv4_need(top);
+          if (need <= KV4_NEEDS_NONE || pos >= reach || (pos < first && pos >= p.sink)) continue;
+          if (plain) all = max(all, need);
+          else if (pos >= all_to || (EXT && pos < all_from && pos >= p.sink)) part = max(part, need);
+          low = min(low, need);
+        }
+        __syncwarp();
+        all = __reduce_max_sync(0xffffffffu, all);
+        part = __reduce_max_sync(0xffffffffu, part);
+        low = __reduce_min_sync(0xffffffffu, low);
+        bool wide = part > low + KV4_WIDE;  // K has an exponent per block
+        if (n & 1) {                        // V that of the largest so far
+          if (plain && all > KV4_NEEDS_NONE) v_all = max(v_all, all);
+          v_part = max(v_part, part);
+          wide = low < 1000 && v_part > max(v_all, plain ? -1000 : low) + KV4_WIDE;
+        }
+        if (wide && lane == 0 && wide_from > j) wide_from = j;
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&raw_empty[s]);
+      return true;
+    };
     for (int j = 0; j < nmax && ok; ++j) {
       const int pg0 = base_of(j) / KV4_PAGE;
       int mine = 0;  // lane i: page number of the block's page i
@@ -291,7 +335,15 @@ __global__ void __launch_bounds__(Kv4PreShape<D>::THREADS, 1) kv4_prefill_kernel
           bulk_load(smem + Shape::OFF_RAW + s * Shape::RAW_BYTES + lane * Shape::PAGE_BYTES,
                     p.pages + block * Shape::PAGE_BYTES, Shape::PAGE_BYTES, &raw_full[s]);
         }
+        if (guard && m + 1 - seen == Shape::RAW_SLOTS) {
+          ok = look(seen++);
+          if (!ok) break;
+        }
       }
+    }
+    if (guard) {
+      while (ok && seen < m) ok = look(seen++);
+      if (ok && lane == 0) mbar_arrive(looked);
     }
     for (int n = max(0, m - Shape::RAW_SLOTS); n < m; ++n) kv4_drain(&raw_full[n % Shape::RAW_SLOTS], (n / Shape::RAW_SLOTS) & 1);
    } else if (warp == ISSUER) {
@@ -418,8 +470,8 @@ __global__ void __launch_bounds__(Kv4PreShape<D>::THREADS, 1) kv4_prefill_kernel
       if constexpr (BF16) {
         // One exponent per block for K, and for V that of the largest block so far, so that weights need no scale. Every warp
         // looks at all positions of the block: all come to the same exponent without meeting. (With one per 32 positions and
-        // the weights carrying the difference P lost bits, and it took 2 % longer.) Values below 2^-28 of the largest lose bits.
-        // |v| <= |lo| + 15 s: with |lo| < 2^(e + 13) and s < 2^(e + 9) the scaled values stay below 2^14; in steps of 4
+        // the weights carrying the difference P lost bits, and it took 2 % longer.) In steps of 4: the largest value lies between
+        // 2^9 and 2^14 then, and values below 2^-23 of it lose bits.
         uint32_t top = 0;
 #pragma unroll
         for (int c = 0; c < Shape::CHUNKS; ++c) {
@@ -437,8 +489,7 @@ __global__ void __launch_bounds__(Kv4PreShape<D>::THREADS, 1) kv4_prefill_kernel
           for (int g = 0; g < GROUPS; ++g) most = __vmaxu2(most, m[g] & 0xffff7fffu);
           if (pos < reach && pos < room && (pos >= first || pos < p.sink)) top = __vmaxu2(top, most);
         }
-        const int need = max(static_cast<int>(top >> 23) - 9, static_cast<int>((top & 0xffffu) >> 7) - 13) - 126;
-        int e = max((__reduce_max_sync(0xffffffffu, need) + 1027) / 4 * 4 - 1024, -120);
+        int e = max((__reduce_max_sync(0xffffffffu, kv4_need(top)) + 1027) / 4 * 4 - 1024, -120);
         if (n & 1) e = v_most = max(v_most, e);
         if (w == 0 && lane == 0) exps[j & 3][n & 1] = e;
         shrink = exp2f(static_cast<float>(-e));
@@ -673,7 +724,54 @@ __global__ void __launch_bounds__(Kv4PreShape<D>::THREADS, 1) kv4_prefill_kernel
       ok = mbar_wait(&o_done[sub], 0, abort_flag, p.status, ERR_WAIT_MMA);
       ok = __all_sync(0xffffffffu, ok);
     }
-    if (ok && warp_active) {
+    if (ok && guard) ok = __all_sync(0xffffffffu, mbar_wait(looked, 0, abort_flag, p.status, ERR_WAIT_PRODUCER));
+    const bool exact = BF16 && ok && wide_from < mine;
+    if (ok && warp_active && exact) {
+      if constexpr (BF16) {
+        const int wrow0 = sub * 128 + (warp & 3) * 32;
+        const int end = min(wrow0 + 32, valid_rows);
+        auto at = [&](int i) {
+          const int pos = base_of(i / BLK) + i % BLK;
+          return pos < room ? pos : -1;
+        };
+#pragma unroll 1
+        for (int first = wrow0; first < end; first += KV4_EXACT) {
+          int len[KV4_EXACT], from[KV4_EXACT];
+          size_t to[KV4_EXACT];  // the row of (token, head)
+          unsigned long long bits[KV4_EXACT];
+          const T* q[KV4_EXACT];
+#pragma unroll
+          for (int i = 0; i < KV4_EXACT; ++i) {
+            const int r = row0 + min(first + i, end - 1), ahead = token_of(r), t = qstart + ahead, h = hk * G + r - ahead * G;
+            to[i] = static_cast<size_t>(t) * p.hq + h;
+            q[i] = reinterpret_cast<const T*>(p.q) + static_cast<size_t>(t) * p.q_stride + h * D;
+            len[i] = p.q_kvlen[t];
+            from[i] = EXT && p.q_kvstart ? p.q_kvstart[t] : 0;
+            bits[i] = EXT && p.tree_mask ? p.tree_mask[t] : 0ull;
+          }
+          auto sees = [&](int i, int pos) { return kv4_visible(pos, len[i], from[i], EXT ? p.sink : 0, bits[i]); };
+          float M[KV4_EXACT], L[KV4_EXACT], acc[KV4_EXACT][8];
+          kv4_rows_exact<T, D>(p.pages, p.num_pages, list, p.hkv, hk, q, p.q_flip ? -1.f : 1.f, p.scale_log2, EXT ? p.cap_k : 0.f,
+                               EXT ? p.cap_log2 : 0.f, mine * BLK, at, sees, M, L, acc);
+#pragma unroll
+          for (int i = 0; i < KV4_EXACT; ++i) {
+            if (first + i >= end) continue;
+            if (p.splits > 1) {
+              const size_t prow = ((static_cast<size_t>(work) * p.hkv + hk) * p.splits + split) * (SUB * 128) + first + i;
+              if (lane < D / 8) kv4_put8(p.part_o + prow * D + lane * 8, acc[i]);
+              if (lane == 0) {
+                p.part_ml[prow * 2] = M[i];
+                p.part_ml[prow * 2 + 1] = L[i];
+              }
+            } else {
+              if (lane < D / 8) kv4_put8(reinterpret_cast<T*>(p.out) + to[i] * D + lane * 8, acc[i], L[i] == 0.f ? 0.f : 1.f / L[i]);
+              if (lane == 0 && p.lse) p.lse[to[i]] = L[i] == 0.f ? -INFINITY : (M[i] + log2f(L[i])) * 0.6931471805599453f;
+            }
+          }
+        }
+      }
+    }
+    if (ok && warp_active && !exact) {
       tc_fence_after();
       const float grow_v = BF16 && mine > 0 ? exp2f(static_cast<float>(v_exp)) : 1.f;
       const float inv = l == 0.f ? 0.f : 1.f / l * grow_v;  // a row that sees nothing is 0; NaN stays NaN

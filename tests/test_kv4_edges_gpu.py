@@ -211,3 +211,42 @@ def test_queries_that_are_not_finite(dtype, lens, new, d):
             _check_rows(st, out, lse, others)
             if value != value:
                 assert bool(torch.isnan(out[bad]).all()) and bool(torch.isnan(lse[bad]).all())
+
+
+@pytest.mark.parametrize("by", [2.0 ** 30, math.inf])
+@pytest.mark.parametrize("what", ["k", "v"])
+@pytest.mark.parametrize("d", [64, 96, 128, 256])
+@pytest.mark.parametrize("lens,new,at,extra", [
+    ([200, 50], [4, 3], 199, {}), ([200, 50], [4, 4], 249, {}), ([120, 70], [4, 4], 119, {"tree": True}),
+    ([100], [4], 81, {"window": 16}), ([2000], [2], 1999, {}), ([4], [4], 2, {}),
+    ([300], [300], 150, {}), ([700, 90], [200, 40], 600, {}), ([3000], [40], 2985, {}), ([400], [60], 380, {"tree": True}),
+    ([300], [300], 100, {"window": 64}), ([300], [300], 3, {"window": 64, "sink": 2}), ([500], [130], 499, {"cap": 30.0})])
+def test_a_huge_value_that_a_row_does_not_see(lens, new, at, extra, d, what, by, monkeypatch):
+    """bf16: what later tokens, other branches of a draft tree or tokens below a row's window hold does not touch that row,
+    however large it is (infinity is cached as 2^126)."""
+    plain = base._kv
+
+    def planted(g, n, hkv, d, dtype):
+        rows = plain(g, n, hkv, d, dtype)
+        col = hkv * d if what == "v" else 0
+        rows[at, col + 5: col + hkv * d: 32] = by
+        return rows
+
+    monkeypatch.setattr(base, "_kv", planted)
+    st = Step(torch.bfloat16, lens, new, 8, 2, d, seed=d + len(lens), **extra)
+    # which sequence and position the planted row is
+    seq, pos = (0, at) if at < lens[0] else (1, at - lens[0])
+    blind = []
+    for t in range(sum(new)):
+        n, start = int(st.kvlen[t]), int(st.kvstart[t]) if st.kvstart is not None else 0
+        sees = st.seq[t] == seq and (start <= pos < n or (pos < min(n, st.sink) and st.kvstart is not None))
+        if st.tree is not None and st.seq[t] == seq and 0 <= pos - n < 63:
+            sees = bool((int(st.tree[t]) >> (pos - n)) & 1)
+        if not sees:
+            blind.append(t)
+    assert 0 < len(blind) < sum(new)
+    out, lse = st.run()
+    ops.check_status(out.device)
+    _check_rows(st, out, lse, blind)
+    assert what == "k" or bool(torch.isfinite(out).all())
+    assert _same_bytes(out, st.run(lse=False))
