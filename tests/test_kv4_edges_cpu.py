@@ -24,7 +24,7 @@ def test_the_join_of_cut_units_never_reads_a_count_that_was_not_written():
     piece of its share, which a wait that ran out can keep it from reaching, and the scratch is not cleared by the caller: so
     every CTA has to write 0 rows before any role starts, and the join must not run after a launch that failed."""
     code = _code("kv4_decode.cu")
-    body = code[code.index("kv4_decode_kernel(const Kv4DecParams p) {"):]
+    body = code[re.search(r"kv4_decode_kernel\(const [^)]*Kv4DecParams p\) {", code).end():]
     head = body[: body.index("__syncthreads()")]
     at = head.index("p.part_unit[blockIdx.x * 4] = 0;")
     # by thread 0, outside of any other condition
