@@ -21,9 +21,11 @@
 //
 // P is rounded to fp16; sums, maxima and accumulators are fp32.
 //
-// Measured, 32 / 8 heads of 128 (CUDA graph): 256 sequences of 512 to 2048, fp16 118 us (3.5 TB/s of the cached bytes, the
-// 16-bit cache's kernel would read 3.2 times as many), bf16 127; 8 of 16300, bf16 53 us; one of 1000 9.8 us. Bound by issue
-// slots (56 %) and the integer pipe (47 %) of 12 consumer warps per SM, not by DRAM.
+// Measured, 32 / 8 heads of 128 (ten launches in a CUDA graph): 256 sequences of 512 to 2048, fp16 123 us (3.4 TB/s of the cached
+// bytes, the 16-bit cache's kernel would read 3.2 times as many); 8 of 16300, bf16 53 us; one of 1000 9.9 us; 64 trees of four
+// tokens behind 100 to 4000, fp16 98 us. No unit is full at 256 sequences: issue slots 56 %, integer pipe 47 %, DRAM 42 %, tensor pipe
+// 20 %. It is latency: a warp issues every 6.4 clocks, 2.1 of them waiting for memory and copies, 1.3 for the previous instruction, and
+// three consumer warps per scheduler do not cover that.
 //
 // Work: a unit is one (sequence, kv head, block of 8 or 16 query rows). All units' slots of 32 tokens (two pages),
 // laid end to end, are cut into equal shares, one per persistent CTA, so ragged batches and single long sequences

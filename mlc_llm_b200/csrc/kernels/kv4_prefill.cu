@@ -24,9 +24,12 @@
 // joined by a second kernel. Bounds: the tensor core (4 D flops per query row and position) and, as slow, the exponentials
 // (one per row and position: 2048 clocks each per block at 16 per clock and SM and 8 K flops per clock).
 //
-// Measured, 32 / 8 heads of 128: 16384 causal tokens fp16 2.07 ms (1060 TFLOP/s), bf16 2.18 ms; 512 to 2048 new tokens
-// behind 0 to 8192, bf16 474 us (920 TFLOP/s); 4 x 1024 74 us. A block takes 4000 clocks there: a tile's softmax (2100,
-// latency of one warp per scheduler and tile) and then its products and hand-overs (1900), the other tile in between.
+// Measured, 32 / 8 heads of 128: 16384 causal tokens fp16 2.08 ms (1057 TFLOP/s), bf16 2.20 ms (one launch; back to back the power
+// limit makes it 2.2 to 2.3 ms); chunks of 2000, 1500, 700 and 1800 new tokens behind 7000, 0, 0 and 3200, bf16 454 us; four
+// of 512 to 2048 behind up to 8192 (641 Gflop) 710 us (903 TFLOP/s); 4 x 1024 fp16 76 us. A block takes some 4200
+// clocks: a tile's softmax (2050 to 2330, latency of one warp per scheduler and tile) and then its products and hand-overs (1670
+// to 2050), one after the other: P overwrites the tile's only S, so that the next scores are computed behind P V. (Two S buffers
+// of 64 columns per tile, as with D = 256, would overlap them; not built.)
 // Tried and slower at 16384 (2.15 ms then): 16 softmax warps 2.23, eight expanding warps 3.26, P handed over in halves 2.21;
 // a quarter of the exponentials as polynomials 2.13 against 2.07.
 //

@@ -4,7 +4,7 @@ A row is the ``d`` values of one (token, K or V, KV head), cut into groups of 32
 ``lo`` and a step ``s = T((max - lo) * r)``, both in the cache's type ``T`` (``r`` is 1 / 15 in fp32), and per value the code
 ``c = clamp(rint((x - lo) / s), 0, 15)``; it stands for ``lo + s * c`` (``s == 0``: for ``lo``). Before that NaN becomes 0
 and values are clamped to a finite bound (``KV4_BOUND``), so a cache never holds anything but finite numbers and a
-token's NaN cannot reach the tokens after it. That is 5 bits per value with 16-bit steps: 80 bytes for ``d = 128``.
+token's NaN cannot reach the tokens after it. (On a GPU bf16 numbers below 2^-126 count as 0.) That is 5 bits per value with 16-bit steps: 80 bytes for ``d = 128``.
 
 A packed cache has the shape of the 16-bit one, ``[num_pages, 2, hkv, page, row]`` and its type, with
 ``row = kv4_row(d, dtype)`` elements of raw bytes in place of ``d`` values: ``d / 2`` code bytes, then ``d / 32`` pairs

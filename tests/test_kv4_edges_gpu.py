@@ -113,6 +113,22 @@ def test_a_cache_that_begins_on_any_word(d):
     st.check(out, lse)
 
 
+def test_bf16_numbers_below_the_normal_ones_count_as_zero():
+    row = torch.tensor([2.0 ** -130, -2.0 ** -128, 2.0 ** -133, 0.0] * 8 + [2.0 ** -100, 2.0 ** -130, 0.0, -2.0 ** -101] * 8
+                       + [2.0 ** -126] * 32 + [1.0] * 32).to(torch.bfloat16).view(1, 128).repeat(1, 2)
+    cache = ops.kv4_cache(1, 1, 128, 16, torch.bfloat16, DEV)
+    zero = torch.zeros(1, dtype=torch.int32, device=DEV)
+    ops.rope_append(row.to(DEV), cache, zero, zero, None, 0, 1, 128, 0, 16)
+    k, v = ops.kv4_read(cache, zero, 128)
+    ops.check_status(cache.device)
+    assert torch.equal(k, v)
+    k = k.view(4, 32).cpu().double()
+    # the group's whole range is below the smallest normal number; in the second, half a step of 1.5 * 2^-100 / 15 each way
+    assert bool((k[0].abs() < 2.0 ** -126).all())
+    assert bool(((k[1] - row[0, 32:64].double()).abs() <= 2.0 ** -100 * 1.5 / 15 * (0.5 + 15 * 2.0 ** -9)).all())
+    assert bool((k[2] == 2.0 ** -126).all()) and bool((k[3] == 1).all())
+
+
 # ------------------------------------------------------------------------------------------------- attention
 @pytest.mark.parametrize("d", [64, 128, 256])
 @pytest.mark.parametrize("lens,new", [([0], [1]), ([1], [1]), ([33], [1]), ([100], [3]), ([3000, 40, 5000] * 30, [1] * 90),
