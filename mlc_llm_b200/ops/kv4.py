@@ -229,7 +229,7 @@ def attend(q: torch.Tensor, kv_pages: torch.Tensor, q_seq: torch.Tensor, q_kvlen
     lse = torch.empty(t, hq, dtype=torch.float32, device=q.device) if return_lse else None
     with _guard(q.device):
         _launch(q, kv_pages, out, lse, q_seq, q_kvlen, page_indptr, page_indices, hq, hkv, d, page, sm_scale, q_kvstart,
-                int(sink), tree_mask, float(softcap), plan)
+                max(0, min(int(sink), 1 << 30)), tree_mask, float(softcap), plan)  # room for rounding up to whole blocks
     return (out, lse) if return_lse else out
 
 

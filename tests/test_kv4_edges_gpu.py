@@ -184,6 +184,16 @@ def test_pages_that_a_window_released(lens, new, hq, hkv, d):
             assert _same_bytes(out, want[0]) and _same_bytes(lse, want[1])
 
 
+@pytest.mark.parametrize("lens,new,d", [([900, 33], [1, 3], 128), ([900, 90], [60, 33], 128), ([900, 90], [60, 33], 256), ([90, 9], [2, 1], 32)])
+def test_sinks_beyond_every_length(lens, new, d):
+    """A window with more sinks than there are positions hides nothing."""
+    for sink in (2 ** 31 - 1, 2 ** 31 - 20, 1000):
+        st = Step(torch.float16, lens, new, 8, 2, d, seed=3, window=20, sink=sink)
+        out, lse = st.run()
+        ops.check_status(out.device)
+        st.check(out, lse)
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("lens,new,d,extra", [([200, 33], [1, 3], 128, {}), ([200, 90], [60, 33], 128, {}),
                                               ([200, 90], [60, 33], 256, {"cap": 30.0}), ([200, 33], [1, 3], 64, {"cap": 30.0})])
