@@ -376,7 +376,7 @@ class ModelExecutor:
                                         dec_ntok=dev["dec_ntok"], num_dec=n_dec,
                                         dec_splits=choose_splits(n_dec, model.hkv, max_pages, self.device)
                                         if n_dec else 1, max_pages=max_pages, tile_rows=self._tile_rows(model),
-                                        dec_rows=decode_rows(plan["q_indptr"], model.hq // model.hkv))
+                                        dec_rows=decode_rows(plan["q_indptr"], model.hq // model.hkv) if model.kv4 else 16)
         return b
 
     def _tc_attention_ok(self, model: DecoderModel) -> bool:
