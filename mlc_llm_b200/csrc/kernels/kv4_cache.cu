@@ -114,7 +114,7 @@ template <typename T>
 __global__ void __launch_bounds__(KV4_APPEND_THREADS)
 kv4_append_kernel(T* __restrict__ qkv, uint8_t* __restrict__ pages, const int* __restrict__ pos,
                   const int* __restrict__ slot, const float* __restrict__ inv_freq, int hq, int hkv, int d,
-                  int rot_dim, int page, float attn_factor, long long num_slots, int* status) {
+                  int rot_dim, int page, double attn_factor, long long num_slots, int* status) {
   extern __shared__ __align__(16) uint8_t smem[];
   const int half = rot_dim / 2;
   double* sn = reinterpret_cast<double*>(smem);  // [half]
@@ -186,7 +186,7 @@ template <typename T, int D>
 __global__ void __launch_bounds__(KV4_APPEND_THREADS)
 kv4_append_whole_kernel(T* __restrict__ qkv, uint8_t* __restrict__ pages, const int* __restrict__ pos,
                         const int* __restrict__ slot, const float* __restrict__ inv_freq, int hq, int hkv, int page,
-                        float attn_factor, long long num_slots, int* status) {
+                        double attn_factor, long long num_slots, int* status) {
   constexpr int HALF = D / 2, JG = HALF / 8, CPR = D / 8, RB = kv4_row_bytes(D), STEP = KV4_APPEND_THREADS;
   __shared__ __align__(16) double sn[HALF], cs[HALF];
   __shared__ float snf[HALF], csf[HALF];
@@ -429,7 +429,7 @@ using namespace mlcb;
 
 // Return codes of the kv4 entry points: -1 shape, -2 alignment, -3 type, -4 out of grid range, > 0 a CUDA error.
 MLCB_API int mlcb_kv4_append(void* qkv, void* pages, const int* pos, const int* slot, const float* inv_freq, int tokens,
-                             int hq, int hkv, int d, int rot_dim, int page, float attn_factor, long long num_slots,
+                             int hq, int hkv, int d, int rot_dim, int page, double attn_factor, long long num_slots,
                              int dtype, int* status, cudaStream_t stream) {
   if (tokens <= 0) return 0;
   if (hq < 0 || hkv <= 0 || d <= 0 || d % 32 || d > 256 || rot_dim < 0 || rot_dim % 2 || rot_dim > d || page <= 0) return -1;

@@ -29,9 +29,9 @@ from ._lib import DTYPE_CODE, check, lib, status_word
 from .attention import AttentionPlan, build_tiles, decode_rows, sm_count
 from .reference import KV4_BOUND, KV4_GROUP, is_kv4, kv4_row
 
-_P, _I, _L, _F = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_float
+_P, _I, _L, _F, _D = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_float, ctypes.c_double
 _ARGS = {
-    "mlcb_kv4_append": [_P] * 5 + [_I] * 6 + [_F, _L, _I, _P, _P],
+    "mlcb_kv4_append": [_P] * 5 + [_I] * 6 + [_D, _L, _I, _P, _P],
     "mlcb_kv4_read": [_P] * 4 + [_I] * 4 + [_L, _I, _P, _P],
     "mlcb_kv4_decode": [_P] * 10 + [_I, _I, _L, _I, _I, _I, _L, _F, _I, _I] + [_P] * 7 + [_I, _F],
     "mlcb_kv4_prefill": [_P] * 10 + [_I, _I, _L, _I, _I, _I, _L, _F, _I, _I] + [_P] * 6 + [_I, _F],

@@ -69,6 +69,24 @@ def test_append_of_many_heads(t, hkv, d, rot):
     assert _same_bytes(mine, want) and _same_bytes(cache, want_cache)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d,rot", [(128, 128), (64, 64), (256, 256), (128, 64), (192, 192)])
+def test_append_scales_angles_in_64_bits(dtype, d, rot):
+    """The factor on sines and cosines (YaRN: 0.1 ln s + 1) keeps its 64 bits: rounded to 32 it moves keys across borders."""
+    t, hkv = 2000, 4
+    g = torch.Generator().manual_seed(d + rot)
+    x = _kv(g, t, hkv, d, dtype).contiguous()
+    pos = torch.randint(0, 131072, (t,), generator=g).to(torch.int32)
+    slot, inv = torch.arange(t, dtype=torch.int32), base.ref.rope_inv_freq(rot, 500000.0)
+    factor = 0.1 * math.log(40.0) + 1.0
+    cache, want_cache = (ops.kv4_cache(t // 16, hkv, d, 16, dtype, dev) for dev in (DEV, "cpu"))
+    mine, want = x.to(DEV), x.clone()
+    ops.rope_append(mine, cache, pos.to(DEV), slot.to(DEV), inv.to(DEV), 0, hkv, d, rot, 16, factor)
+    ops.rope_append(want, want_cache, pos, slot, inv, 0, hkv, d, rot, 16, factor)
+    ops.check_status(cache.device)
+    assert _same_bytes(mine, want) and _same_bytes(cache, want_cache)
+
+
 @pytest.mark.parametrize("d,page,pages", [(32, 1, 3), (32, 3, 1), (96, 1, 1), (160, 1, 3)])
 def test_layers_of_small_pages(d, page, pages):
     """Layers that do not begin on 16 bytes: rows are whole 32-bit words, which is all that the kernels ask of them."""
